@@ -316,6 +316,81 @@ typedef struct {
 } pdb_score_program_desc;
 int pdb_score_program_f32(const pdb_score_program_desc* d, void* stream);
 
+/* ---- layer norm for training -------------------------------------------------
+ * The row-statistics template in training: f32 or bf16 rows with the rows'
+ * statistics, and its gradients.  The reference has the region and derives the
+ * gradient by autodiff (autodiff.py:102); neither has a template row of its own.
+ *   y = (x - mean) * rstd * gamma + beta,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * dtype is the type of x / y / dout / dx; param_dtype that of gamma / beta /
+ * dgamma / dbeta: PDB_F32, or dtype.  Statistics and all sums are f32.  mean and
+ * rstd (f32 [rows]) are optional outputs of the forward and inputs of the
+ * backward.  gamma / beta may be NULL (identity scale / zero shift).
+ * The backward writes dx, and dgamma[c] = sum_r dout * z, dbeta[c] = sum_r dout
+ * when both are given (both NULL: dx alone), in a fixed order of summation; its
+ * workspace (f32 partial sums) is sized by pdb_layernorm_bwd_workspace_size.
+ * dx may be dout or x.  With rows == 0 the weight gradients are zeros. */
+typedef struct {
+  const void* x;
+  const void* gamma; /* nullable */
+  const void* beta;  /* nullable */
+  void* y;
+  float* mean; /* nullable */
+  float* rstd; /* nullable */
+  int64_t rows, cols;
+  int64_t x_row_stride, y_row_stride;
+  double eps;
+  int32_t dtype, param_dtype; /* enum pdb_dtype */
+} pdb_layernorm_fwd_desc;
+int pdb_layernorm_fwd(const pdb_layernorm_fwd_desc* d, void* stream);
+
+typedef struct {
+  const void* dout;
+  const void* x;
+  const float* mean;
+  const float* rstd;
+  const void* gamma; /* nullable */
+  void* dx;
+  void* dgamma; /* nullable, with dbeta */
+  void* dbeta;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t rows, cols;
+  int64_t dout_row_stride, x_row_stride, dx_row_stride;
+  int32_t dtype, param_dtype;
+} pdb_layernorm_bwd_desc;
+size_t pdb_layernorm_bwd_workspace_size(const pdb_layernorm_bwd_desc* d);
+int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream);
+
+/* ---- rotary positions --------------------------------------------------------
+ * No counterpart in the reference.  Turns pairs of features of the heads that
+ * pdb_flash_fwd reads, in one launch for up to two tensors (q and k):
+ *   a' = (a cos - b sin) * amplitude,  b' = (b cos + a sin) * amplitude,
+ *   angle = position * inv_freq[j],  j < rotary_dim / 2,
+ * over (a, b) = (x[j], x[rotary_dim/2 + j]), or (x[2j], x[2j+1]) when
+ * interleaved; features from rotary_dim on pass through.  `inverse` turns
+ * backwards, which is the gradient.  Tensors are [batch, heads[i], seqlen,
+ * head_dim] views (strides per batch, head, row; feature stride 1); heads[1] =
+ * 0 for one tensor; y[i] may be x[i] with the same strides.  positions: int64
+ * on the device, read at strides (batch, row); NULL means start + row.  Any
+ * int64 position is exact up to whole turns.  inv_freq (radians per position)
+ * is read on the host during the call. */
+#define PDB_ROTARY_MAX_PAIRS 128
+typedef struct {
+  const void* x[2];
+  void* y[2];
+  int64_t heads[2];
+  int64_t x_stride[2][3], y_stride[2][3]; /* (b, h, row) */
+  const int64_t* positions;               /* nullable */
+  int64_t pos_stride[2];
+  int64_t start;
+  int64_t batch, seqlen, head_dim, rotary_dim;
+  double amplitude;
+  double inv_freq[PDB_ROTARY_MAX_PAIRS];
+  int32_t interleaved, inverse;
+  int32_t dtype, reserved;
+} pdb_rotary_desc;
+int pdb_rotary(const pdb_rotary_desc* d, void* stream);
+
 /* ---- status --------------------------------------------------------------------
  * pdb_check_error synchronises `stream`, reads and clears the device error flag
  * of the current device (set by bounded waits that expired; its address is

@@ -37,6 +37,10 @@ EXPORTS = (
     "pdb_contract",
     "pdb_pointwise_f32",
     "pdb_score_program_f32",
+    "pdb_layernorm_fwd",
+    "pdb_layernorm_bwd",
+    "pdb_layernorm_bwd_workspace_size",
+    "pdb_rotary",
     "pdb_check_error",
     "pdb_selftest_wait_timeout",
     "pdb_last_error_string",
@@ -261,6 +265,72 @@ class ScoreProgramDesc(C.Structure):
     ]
 
 
+class LayerNormFwdDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("gamma", C.c_void_p),
+        ("beta", C.c_void_p),
+        ("y", C.c_void_p),
+        ("mean", C.c_void_p),
+        ("rstd", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("x_row_stride", C.c_int64),
+        ("y_row_stride", C.c_int64),
+        ("eps", C.c_double),
+        ("dtype", C.c_int32),
+        ("param_dtype", C.c_int32),
+    ]
+
+
+class LayerNormBwdDesc(C.Structure):
+    _fields_ = [
+        ("dout", C.c_void_p),
+        ("x", C.c_void_p),
+        ("mean", C.c_void_p),
+        ("rstd", C.c_void_p),
+        ("gamma", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dgamma", C.c_void_p),
+        ("dbeta", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("dout_row_stride", C.c_int64),
+        ("x_row_stride", C.c_int64),
+        ("dx_row_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("param_dtype", C.c_int32),
+    ]
+
+
+ROTARY_MAX_PAIRS = 128
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p * 2),
+        ("y", C.c_void_p * 2),
+        ("heads", C.c_int64 * 2),
+        ("x_stride", I64x3 * 2),
+        ("y_stride", I64x3 * 2),
+        ("positions", C.c_void_p),
+        ("pos_stride", C.c_int64 * 2),
+        ("start", C.c_int64),
+        ("batch", C.c_int64),
+        ("seqlen", C.c_int64),
+        ("head_dim", C.c_int64),
+        ("rotary_dim", C.c_int64),
+        ("amplitude", C.c_double),
+        ("inv_freq", C.c_double * ROTARY_MAX_PAIRS),
+        ("interleaved", C.c_int32),
+        ("inverse", C.c_int32),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 _LIB = None
 
 
@@ -292,6 +362,11 @@ def load(path: Path | None = None) -> C.CDLL:
     lib.pdb_contract.argtypes = [C.POINTER(ContractDesc), vp]
     lib.pdb_pointwise_f32.argtypes = [C.POINTER(PointwiseDesc), vp]
     lib.pdb_score_program_f32.argtypes = [C.POINTER(ScoreProgramDesc), vp]
+    lib.pdb_layernorm_fwd.argtypes = [C.POINTER(LayerNormFwdDesc), vp]
+    lib.pdb_layernorm_bwd.argtypes = [C.POINTER(LayerNormBwdDesc), vp]
+    lib.pdb_layernorm_bwd_workspace_size.argtypes = [C.POINTER(LayerNormBwdDesc)]
+    lib.pdb_layernorm_bwd_workspace_size.restype = C.c_size_t
+    lib.pdb_rotary.argtypes = [C.POINTER(RotaryDesc), vp]
     lib.pdb_check_error.argtypes = [vp]
     lib.pdb_selftest_wait_timeout.argtypes = [C.c_int64, vp]
     lib.pdb_last_error_string.restype = C.c_char_p
@@ -299,6 +374,7 @@ def load(path: Path | None = None) -> C.CDLL:
     for name in EXPORTS:
         f = getattr(lib, name)
         if name not in ("pdb_flash_bwd_workspace_size", "pdb_flash_bwd_noalloc_max_scratch",
+                        "pdb_layernorm_bwd_workspace_size",
                         "pdb_last_error_string", "pdb_version"):
             f.restype = C.c_int
     if path is None:

@@ -8,6 +8,7 @@ missing ``libpdb_sm100.so`` raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 
@@ -39,6 +40,42 @@ def _rows2d(x: torch.Tensor) -> torch.Tensor:
     return x2
 
 
+def _on_device_of(t: torch.Tensor):
+    """The library launches on the current device: make it the tensor's where it is another."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _param_dtype(what: str, x: torch.Tensor, cols: int, **vectors) -> torch.dtype:
+    """The one dtype of the given per-column vectors (float32, or x's)."""
+    ptype = None
+    for nm, t in vectors.items():
+        if t is None:
+            continue
+        if t.dtype not in (torch.float32, x.dtype) or t.numel() != cols or t.device != x.device:
+            raise ValueError(f"{what}: {nm} must be a CUDA f32 vector of length {cols} (or of x's dtype)")
+        if ptype not in (None, t.dtype):
+            raise ValueError(f"{what}: gamma and beta must share one dtype")
+        ptype = t.dtype
+    return ptype or torch.float32
+
+
+def _out_rows(what: str, out: torch.Tensor, x2: torch.Tensor) -> torch.Tensor:
+    if out.dtype != x2.dtype or out.device != x2.device or out.numel() != x2.numel():
+        raise ValueError(f"{what}: out must have x's size, dtype and device")
+    y = out.view(x2.shape)
+    if y.shape[-1] > 1 and y.stride(-1) != 1:
+        raise ValueError(f"{what}: out must have unit stride along its last dim")
+    return y
+
+
+def _own_rows(x: torch.Tensor) -> torch.Tensor:
+    """x as 2-D rows that do not overlap (an expanded gradient is laid out first)."""
+    x2 = _rows2d(x)
+    return x2.contiguous() if x2.shape[0] > 1 and x2.stride(0) < x2.shape[1] else x2
+
+
 def row_softmax(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """softmax over the last dim of an f32 CUDA tensor (row-normalization)."""
     _need_cuda(x)
@@ -53,24 +90,80 @@ def row_softmax(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tenso
 
 
 def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None,
-              eps: float = 1e-5, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Two-pass layernorm over the last dim (row-statistics), f32."""
+              eps: float = 1e-5, out: torch.Tensor | None = None, return_stats: bool = False):
+    """Two-pass layernorm over the last dim (row-statistics), f32 or bf16 (sums and statistics in f32).
+
+    gamma / beta are f32 vectors, or of x's dtype.  ``return_stats`` returns
+    (y, mean, rstd), the rows' float32 statistics that ``layernorm_backward`` reads."""
     _need_cuda(x)
-    if x.dtype != torch.float32:
-        raise TypeError("layernorm: float32 only")
+    if x.dtype not in _DTYPES:
+        raise TypeError("layernorm: float32 or bfloat16")
     x2 = _rows2d(x)
     C_ = x2.shape[1]
-    for nm, t in (("gamma", gamma), ("beta", beta)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != C_ or not t.is_cuda):
-            raise ValueError(f"layernorm: {nm} must be a CUDA f32 vector of length {C_}")
+    ptype = _param_dtype("layernorm", x, C_, gamma=gamma, beta=beta)
     g = gamma.contiguous() if gamma is not None else None
     b = beta.contiguous() if beta is not None else None
-    y = torch.empty_like(x2) if out is None else out.view(x2.shape)
-    d = LayerNormDesc(x2.data_ptr(), g.data_ptr() if g is not None else None, b.data_ptr() if b is not None else None,
-                      y.data_ptr(), x2.shape[0], C_, x2.stride(0) if x2.shape[0] else C_,
-                      y.stride(0) if y.shape[0] else C_, float(eps))
-    check(load().pdb_layernorm_f32(C.byref(d), _stream(x)), "pdb_layernorm_f32")
+    y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
+    if x.dtype == torch.float32 and ptype == torch.float32 and not return_stats:
+        d = LayerNormDesc(x2.data_ptr(), g.data_ptr() if g is not None else None,
+                          b.data_ptr() if b is not None else None, y.data_ptr(), x2.shape[0], C_,
+                          x2.stride(0) if x2.shape[0] else C_, y.stride(0) if y.shape[0] else C_, float(eps))
+        with _on_device_of(x):
+            check(load().pdb_layernorm_f32(C.byref(d), _stream(x)), "pdb_layernorm_f32")
+        return y.view(x.shape)
+    x2 = _own_rows(x2)
+    R = x2.shape[0]
+    stats = torch.empty((2, R), dtype=torch.float32, device=x.device) if return_stats else None
+    at = stats.data_ptr() if return_stats else None
+    d = _lib.LayerNormFwdDesc(x2.data_ptr(), g.data_ptr() if g is not None else None,
+                              b.data_ptr() if b is not None else None, y.data_ptr(), at,
+                              at + 4 * R if return_stats else None, R, C_, x2.stride(0), y.stride(0), float(eps),
+                              _DTYPES[x.dtype], _DTYPES[ptype])
+    with _on_device_of(x):
+        check(load().pdb_layernorm_fwd(C.byref(d), _stream(x)), "pdb_layernorm_fwd")
+    if return_stats:
+        lead = x.shape[:-1]
+        return y.view(x.shape), stats[0].view(lead), stats[1].view(lead)
     return y.view(x.shape)
+
+
+def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                       gamma: torch.Tensor | None = None, *, weight_grads: bool = True):
+    """(dx, dgamma, dbeta) of layernorm from the forward's statistics.
+
+    dgamma / dbeta are vectors of gamma's dtype (float32 without gamma), summed in
+    float32 in a fixed order; None without ``weight_grads``."""
+    _need_cuda(dout, x, mean, rstd)
+    if x.dtype not in _DTYPES or dout.dtype != x.dtype:
+        raise TypeError("layernorm_backward: dout and x must both be float32 or bfloat16")
+    if dout.shape != x.shape:
+        raise ValueError(f"layernorm_backward: dout {tuple(dout.shape)} does not match x {tuple(x.shape)}")
+    x2, do2 = _own_rows(x), _own_rows(dout)
+    R, C_ = x2.shape
+    for nm, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or t.numel() != R or t.device != x.device:
+            raise ValueError(f"layernorm_backward: {nm} must be the forward's float32 statistic of {R} rows")
+    if dout.device != x.device:
+        raise ValueError("layernorm_backward: tensors on different devices")
+    ptype = _param_dtype("layernorm_backward", x, C_, gamma=gamma)
+    g = gamma.contiguous() if gamma is not None else None
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dx = torch.empty((R, C_), dtype=x.dtype, device=x.device)
+    dw = torch.empty((2, C_), dtype=ptype, device=x.device) if weight_grads else None
+    d = _lib.LayerNormBwdDesc(do2.data_ptr(), x2.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                              g.data_ptr() if g is not None else None, dx.data_ptr(), None, None, None, 0, R, C_,
+                              do2.stride(0), x2.stride(0), C_, _DTYPES[x.dtype], _DTYPES[ptype])
+    lib = load()
+    with _on_device_of(x):
+        if weight_grads:
+            d.dgamma = dw.data_ptr()
+            d.dbeta = d.dgamma + dw.element_size() * C_ if C_ else d.dgamma
+            nbytes = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
+            ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=x.device)
+            d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
+        check(lib.pdb_layernorm_bwd(C.byref(d), _stream(x)), "pdb_layernorm_bwd")
+    dx = dx.view(x.shape)
+    return (dx, dw[0], dw[1]) if weight_grads else (dx, None, None)
 
 
 def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -179,6 +272,89 @@ def flash_attention_backward(q, k, v, o, dout, lse=None, *, scale=None, causal=F
     d.workspace, d.workspace_bytes = ws.data_ptr(), int(nbytes)
     check(lib.pdb_flash_bwd(C.byref(d), _stream(q)), "pdb_flash_bwd")
     return dq.view(shape_q), dk.view(shape_k), dv.view(shape_v)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, positions: torch.Tensor | None = None,
+           start: int = 0, interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False, out=None):
+    """Rotary positions on the heads that flash_attention reads: q (B, H, T, D), and k (B, Hkv, T, D) in the same
+    launch; 2-D and 3-D inputs drop the leading dims, as there.  float32 or bfloat16 (turned in float32).
+
+    Pair j of a head's first 2 * len(inv_freq) features turns by position * inv_freq[j] radians and is multiplied
+    by ``amplitude``; the pairs are (j, j + len(inv_freq)), or (2j, 2j + 1) when ``interleaved``; later features
+    pass through.  ``inv_freq`` is a host sequence of up to 128 numbers (see ``rotary_frequencies``).
+    ``positions`` is an integer CUDA tensor (T,) or (B, T) (either may be broadcast), else row t has position
+    start + t.  ``inverse`` turns backwards: the gradient of the forward turn.  ``out`` (a tensor, or a pair with k)
+    may be the inputs themselves.  Returns the turned q, or (q, k)."""
+    ts = (q,) if k is None else (q, k)
+    _need_cuda(*ts)
+    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+        raise TypeError("rotary: q and k must both be float32 or bfloat16")
+    xs = [_as4d(t, n) for t, n in zip(ts, ("q", "k"))]
+    B, _, T, D = xs[0].shape
+    if k is not None and (xs[1].shape[0] != B or xs[1].shape[2:] != (T, D) or k.device != q.device):
+        raise ValueError(f"rotary: incompatible q {tuple(q.shape)} and k {tuple(k.shape)}")
+    freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
+    if freq.ndim != 1 or len(freq) > _lib.ROTARY_MAX_PAIRS or 2 * len(freq) > D:
+        raise ValueError(f"rotary: inv_freq must be a vector of at most {_lib.ROTARY_MAX_PAIRS} pairs within the head's {D} features")
+    if out is None:
+        ys = [torch.empty_like(t) for t in xs]
+    else:
+        outs = (out,) if k is None else tuple(out)
+        if len(outs) != len(ts) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device
+                                       or any(n > 1 and (st == 0 or (i == o.dim() - 1 and st != 1))
+                                              for i, (n, st) in enumerate(zip(o.shape, o.stride())))
+                                       for o, t in zip(outs, ts)):
+            raise ValueError("rotary: out must match the inputs, with unit stride along the features and no broadcast dim")
+        ys = [_as4d(o, "out") for o in outs]
+    d = _lib.RotaryDesc()
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        d.x[i], d.y[i], d.heads[i] = x.data_ptr(), y.data_ptr(), x.shape[1]
+        d.x_stride[i], d.y_stride[i] = _s3(x), _s3(y)
+    if positions is not None:
+        if positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
+            raise TypeError("rotary: positions must be an integer tensor on q's device")
+        if positions.dim() not in (1, 2):
+            raise ValueError("rotary: positions must be (T,) or (B, T)")
+        p = positions.to(torch.int64).expand(B, T)
+        d.positions, d.pos_stride[0], d.pos_stride[1] = p.data_ptr(), p.stride(0), p.stride(1)
+    d.start, d.batch, d.seqlen, d.head_dim, d.rotary_dim = int(start), B, T, D, 2 * len(freq)
+    d.amplitude, d.interleaved, d.inverse, d.dtype = float(amplitude), int(bool(interleaved)), int(bool(inverse)), _DTYPES[q.dtype]
+    C.memmove(d.inv_freq, freq.ctypes.data, freq.nbytes)
+    with _on_device_of(q):
+        check(load().pdb_rotary(C.byref(d), _stream(q)), "pdb_rotary")
+    rets = [y.view(t.shape) for y, t in zip(ys, ts)] if out is None else list(outs)
+    return rets[0] if k is None else tuple(rets)
+
+
+def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       context: int = 0, fast: float = 32.0, slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """(inv_freq, amplitude) for ``rotary``: base^(-2j / rotary_dim), scaled for contexts ``factor`` times as long as
+    the ``context`` that a model was trained on.
+
+    scaling "none"; "linear": every angle divided by factor (position interpolation); "ntk": the base grown to
+    base * factor^(rotary_dim / (rotary_dim - 2)), which divides the slowest pair's angle by factor and leaves the
+    fastest; "by_parts" (YaRN, Peng et al. 2023): pairs that make at least ``fast`` turns over the context keep their
+    frequency, those with at most ``slow`` are divided by factor, a ramp between, and amplitude 0.1 ln(factor) + 1."""
+    if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > 2 * _lib.ROTARY_MAX_PAIRS:
+        raise ValueError(f"rotary_frequencies: rotary_dim must be even and at most {2 * _lib.ROTARY_MAX_PAIRS}")
+    if not base > 0 or not factor > 0:
+        raise ValueError("rotary_frequencies: base and factor must be positive")
+    j2 = np.arange(0, rotary_dim, 2, dtype=np.float64)
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("rotary_frequencies: ntk scaling needs rotary_dim > 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-j2 / max(rotary_dim, 1))
+    if scaling in ("none", "ntk"):
+        return freq, 1.0
+    if scaling == "linear":
+        return freq / factor, 1.0
+    if scaling != "by_parts":
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    if context <= 0 or not fast > slow:
+        raise ValueError("rotary_frequencies: by_parts needs the trained context and fast > slow")
+    keep = np.clip((context * freq / (2 * math.pi) - slow) / (fast - slow), 0.0, 1.0)
+    return freq * keep + freq / factor * (1.0 - keep), (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
 
 
 def check_device_errors() -> None:

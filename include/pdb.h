@@ -391,6 +391,59 @@ typedef struct {
 } pdb_rotary_desc;
 int pdb_rotary(const pdb_rotary_desc* d, void* stream);
 
+/* ---- cross entropy of a linear head -----------------------------------------
+ * No counterpart in the reference (a contraction, a row softmax and a gather
+ * there).  x [tokens, width] hidden states, w [vocab, width] the head's weight,
+ * both bf16 (PDB_ERR_UNSUPPORTED otherwise), width and row strides multiples of
+ * 8; logit[n, v] = x[n] . w[v] in f32, never stored:
+ *   lse[n]  = log sum_v exp(logit[n, v])
+ *   loss[n] = lse[n] - logit[n, target[n]]
+ * loss and lse are f32 [tokens], either may be NULL.  target is int64 [tokens] on
+ * the device; rows whose target is ignore_index have loss 0 and no gradient, and
+ * any other target outside [0, vocab) makes the row's loss NaN (and NaN its
+ * gradient).  The backward takes the forward's lse and dloss (f32, element stride
+ * dloss_stride, 0 broadcasts one value):
+ *   G[n, v] = (exp(logit[n, v] - lse[n]) - [v == target[n]]) * dloss[n]
+ *   dx = G w,  dw = G^T x      (bf16, f32 accumulate; dx or dw may be NULL)
+ * piece by piece of the vocabulary: its workspace holds one piece of G in bf16
+ * (at most 512 MiB, or 256 columns) and f32 partial sums.  Sums are taken in a
+ * fixed order.  Workspaces are sized by the *_workspace_size calls (0 for a
+ * descriptor that is refused or has no tokens) on the device that runs the call. */
+typedef struct {
+  const void* x;
+  const void* w;
+  const int64_t* target;
+  float* loss; /* nullable */
+  float* lse;  /* nullable */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t tokens, vocab, width;
+  int64_t x_stride, w_stride; /* rows */
+  int64_t ignore_index;
+  int32_t dtype, reserved;
+} pdb_linear_ce_fwd_desc;
+size_t pdb_linear_ce_fwd_workspace_size(const pdb_linear_ce_fwd_desc* d);
+int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream);
+
+typedef struct {
+  const void* x;
+  const void* w;
+  const int64_t* target;
+  const float* lse;
+  const float* dloss;
+  void* dx; /* nullable */
+  void* dw; /* nullable */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t tokens, vocab, width;
+  int64_t x_stride, w_stride, dx_stride, dw_stride; /* rows */
+  int64_t dloss_stride;
+  int64_t ignore_index;
+  int32_t dtype, reserved;
+} pdb_linear_ce_bwd_desc;
+size_t pdb_linear_ce_bwd_workspace_size(const pdb_linear_ce_bwd_desc* d);
+int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream);
+
 /* ---- status --------------------------------------------------------------------
  * pdb_check_error synchronises `stream`, reads and clears the device error flag
  * of the current device (set by bounded waits that expired; its address is

@@ -41,6 +41,10 @@ EXPORTS = (
     "pdb_layernorm_bwd",
     "pdb_layernorm_bwd_workspace_size",
     "pdb_rotary",
+    "pdb_linear_ce_fwd",
+    "pdb_linear_ce_fwd_workspace_size",
+    "pdb_linear_ce_bwd",
+    "pdb_linear_ce_bwd_workspace_size",
     "pdb_check_error",
     "pdb_selftest_wait_timeout",
     "pdb_last_error_string",
@@ -331,6 +335,51 @@ class RotaryDesc(C.Structure):
     ]
 
 
+class LinearCeFwdDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("target", C.c_void_p),
+        ("loss", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("tokens", C.c_int64),
+        ("vocab", C.c_int64),
+        ("width", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("w_stride", C.c_int64),
+        ("ignore_index", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class LinearCeBwdDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("target", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("dloss", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("tokens", C.c_int64),
+        ("vocab", C.c_int64),
+        ("width", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("w_stride", C.c_int64),
+        ("dx_stride", C.c_int64),
+        ("dw_stride", C.c_int64),
+        ("dloss_stride", C.c_int64),
+        ("ignore_index", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 _LIB = None
 
 
@@ -367,6 +416,12 @@ def load(path: Path | None = None) -> C.CDLL:
     lib.pdb_layernorm_bwd_workspace_size.argtypes = [C.POINTER(LayerNormBwdDesc)]
     lib.pdb_layernorm_bwd_workspace_size.restype = C.c_size_t
     lib.pdb_rotary.argtypes = [C.POINTER(RotaryDesc), vp]
+    lib.pdb_linear_ce_fwd.argtypes = [C.POINTER(LinearCeFwdDesc), vp]
+    lib.pdb_linear_ce_fwd_workspace_size.argtypes = [C.POINTER(LinearCeFwdDesc)]
+    lib.pdb_linear_ce_fwd_workspace_size.restype = C.c_size_t
+    lib.pdb_linear_ce_bwd.argtypes = [C.POINTER(LinearCeBwdDesc), vp]
+    lib.pdb_linear_ce_bwd_workspace_size.argtypes = [C.POINTER(LinearCeBwdDesc)]
+    lib.pdb_linear_ce_bwd_workspace_size.restype = C.c_size_t
     lib.pdb_check_error.argtypes = [vp]
     lib.pdb_selftest_wait_timeout.argtypes = [C.c_int64, vp]
     lib.pdb_last_error_string.restype = C.c_char_p
@@ -374,7 +429,8 @@ def load(path: Path | None = None) -> C.CDLL:
     for name in EXPORTS:
         f = getattr(lib, name)
         if name not in ("pdb_flash_bwd_workspace_size", "pdb_flash_bwd_noalloc_max_scratch",
-                        "pdb_layernorm_bwd_workspace_size",
+                        "pdb_layernorm_bwd_workspace_size", "pdb_linear_ce_fwd_workspace_size",
+                        "pdb_linear_ce_bwd_workspace_size",
                         "pdb_last_error_string", "pdb_version"):
             f.restype = C.c_int
     if path is None:

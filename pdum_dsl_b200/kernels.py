@@ -432,3 +432,85 @@ def pointwise(x: torch.Tensor, program, out: torch.Tensor | None = None) -> torc
     check(load().pdb_pointwise_f32(C.byref(d), _stream(x)), "pdb_pointwise_f32")
     del keep
     return y
+
+
+def _head_operand(name: str, t: torch.Tensor) -> torch.Tensor:
+    """A 2-D bf16 matrix as the tensor maps take it: 16-byte aligned rows with unit stride, laid out anew otherwise."""
+    R, W = t.shape
+    ok = t.data_ptr() % 16 == 0 and (W <= 1 or t.stride(1) == 1) and (R <= 1 or (t.stride(0) >= W and t.stride(0) % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _head_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _head_args(what: str, x, weight, target):
+    _need_cuda(x, weight, target)
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"{what}: x and weight must be bfloat16, got {x.dtype} / {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1]:
+        raise ValueError(f"{what}: incompatible x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"{what}: target must be int64")
+    if weight.device != x.device or target.device != x.device:
+        raise ValueError(f"{what}: tensors on different devices")
+    return _head_operand("x", x.reshape(-1, x.shape[-1])), _head_operand("weight", weight), target.reshape(-1).contiguous()
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
+                         return_lse: bool = False):
+    """The cross entropy of a linear head, per token, without storing its logits.
+
+    x (..., width) and weight (vocab, width) bf16, width a multiple of 8; target (...) int64.  Returns the float32
+    loss logsumexp_v(x . weight[v]) - x . weight[target], 0 where the target is ``ignore_index`` and NaN where it is
+    another index outside the vocabulary; with ``return_lse`` (loss, lse), which the backward takes."""
+    x2, w, t = _head_args("linear_cross_entropy", x, weight, target)
+    N, W = x2.shape
+    out = torch.empty((2 if return_lse else 1, N), dtype=torch.float32, device=x.device)
+    at = out.data_ptr()
+    d = _lib.LinearCeFwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), at, at + 4 * N if return_lse else None, None, 0,
+                             N, w.shape[0], W, _head_stride(x2), _head_stride(w), int(ignore_index), _lib.PDB_BF16, 0)
+    lib = load()
+    with _on_device_of(x):
+        ws = torch.empty(lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        check(lib.pdb_linear_ce_fwd(C.byref(d), _stream(x)), "pdb_linear_ce_fwd")
+    lead = x.shape[:-1]
+    return (out[0].view(lead), out[1].view(lead)) if return_lse else out[0].view(lead)
+
+
+def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, dloss: torch.Tensor,
+                                  lse: torch.Tensor | None = None, *, ignore_index: int = -100, need_dx: bool = True,
+                                  need_dweight: bool = True):
+    """(dx, dweight) of linear_cross_entropy, bf16, from the per-token float32 gradient of the loss.
+
+    ``dloss`` broadcasts to target's shape (for a mean over n tokens: a tensor holding 1 / n); ``lse`` None recomputes
+    it.  A gradient that is not needed is None."""
+    x2, w, t = _head_args("linear_cross_entropy_backward", x, weight, target)
+    if not dloss.is_cuda or dloss.dtype != torch.float32 or dloss.device != x.device:
+        raise TypeError("linear_cross_entropy_backward: dloss must be a float32 tensor on x's device")
+    if not (need_dx or need_dweight):
+        return None, None
+    N, W = x2.shape
+    V = w.shape[0]
+    if lse is None:
+        _, lse = linear_cross_entropy(x, weight, target, ignore_index=ignore_index, return_lse=True)
+    elif lse.dtype != torch.float32 or lse.shape != target.shape or lse.device != x.device:
+        raise ValueError("linear_cross_entropy_backward: lse must be the forward's float32 logsumexp")
+    lse = lse.reshape(-1).contiguous()
+    if dloss.numel() == 1:
+        g, gs = dloss, 0
+    else:
+        g, gs = dloss.expand(target.shape).reshape(-1).contiguous(), 1
+    dx = torch.empty((N, W), dtype=torch.bfloat16, device=x.device) if need_dx else None
+    dw = torch.empty((V, W), dtype=torch.bfloat16, device=x.device) if need_dweight else None
+    d = _lib.LinearCeBwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), lse.data_ptr(), g.data_ptr(),
+                             dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dweight else None, None, 0,
+                             N, V, W, _head_stride(x2), _head_stride(w), W, W, gs, int(ignore_index), _lib.PDB_BF16, 0)
+    lib = load()
+    with _on_device_of(x):
+        ws = torch.empty(lib.pdb_linear_ce_bwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        check(lib.pdb_linear_ce_bwd(C.byref(d), _stream(x)), "pdb_linear_ce_bwd")
+    return dx.view(x.shape) if need_dx else None, dw

@@ -12,7 +12,8 @@ from pdum_dsl_b200 import _lib
 from tests.test_abi import REPO
 
 _STRUCTS = {"pdb_layernorm_fwd_desc": "LayerNormFwdDesc", "pdb_layernorm_bwd_desc": "LayerNormBwdDesc",
-            "pdb_rotary_desc": "RotaryDesc"}
+            "pdb_rotary_desc": "RotaryDesc", "pdb_linear_ce_fwd_desc": "LinearCeFwdDesc",
+            "pdb_linear_ce_bwd_desc": "LinearCeBwdDesc"}
 
 
 def test_descriptor_layouts_match_the_header(tmp_path):
@@ -106,6 +107,72 @@ def test_rotary_refusals():
     assert lib.pdb_rotary(C.byref(d), None) == _lib.PDB_ERR_ARG
 
 
+def _ce(**kw):
+    d = _lib.LinearCeFwdDesc(16, 16, 16, 16, 16, None, 0, 4, 300, 64, 64, 64, -100, _lib.PDB_BF16, 0)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _ce_bwd(**kw):
+    d = _lib.LinearCeBwdDesc(16, 16, 16, 16, 16, 16, 16, None, 0, 4, 300, 64, 64, 64, 64, 64, 1, -100, _lib.PDB_BF16, 0)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_linear_cross_entropy_refusals():
+    lib = _lib.load()
+    assert lib.pdb_linear_ce_fwd(None, None) == lib.pdb_linear_ce_bwd(None, None) == _lib.PDB_ERR_ARG
+    assert lib.pdb_linear_ce_fwd_workspace_size(None) == lib.pdb_linear_ce_bwd_workspace_size(None) == 0
+    for kw, want in (({"tokens": -1}, _lib.PDB_ERR_SHAPE), ({"vocab": 0}, _lib.PDB_ERR_SHAPE),
+                     ({"width": 0}, _lib.PDB_ERR_SHAPE), ({"tokens": (1 << 24) + 1}, _lib.PDB_ERR_SHAPE),
+                     ({"vocab": 1 << 40}, _lib.PDB_ERR_SHAPE), ({"width": 1 << 17, "x_stride": 1 << 17}, _lib.PDB_ERR_SHAPE),
+                     ({"width": 60}, _lib.PDB_ERR_ALIGN), ({"x_stride": 68}, _lib.PDB_ERR_ALIGN),
+                     ({"w_stride": 56}, _lib.PDB_ERR_ALIGN), ({"dtype": _lib.PDB_F32}, _lib.PDB_ERR_UNSUPPORTED),
+                     ({"x": None}, _lib.PDB_ERR_ARG), ({"target": None}, _lib.PDB_ERR_ARG)):
+        for d, run, size in ((_ce(**kw), lib.pdb_linear_ce_fwd, lib.pdb_linear_ce_fwd_workspace_size),
+                             (_ce_bwd(**kw), lib.pdb_linear_ce_bwd, lib.pdb_linear_ce_bwd_workspace_size)):
+            assert run(C.byref(d), None) == want, kw
+            if want != _lib.PDB_ERR_ARG:
+                assert size(C.byref(d)) == 0
+    assert lib.pdb_linear_ce_fwd(C.byref(_ce(loss=None, lse=None)), None) == _lib.PDB_ERR_ARG
+    assert lib.pdb_linear_ce_bwd(C.byref(_ce_bwd(dx=None, dw=None)), None) == _lib.PDB_ERR_ARG
+    for kw in ({"dx": 8}, {"dw": 8}, {"dx_stride": 68}, {"dw_stride": 56}):
+        assert lib.pdb_linear_ce_bwd(C.byref(_ce_bwd(**kw)), None) == _lib.PDB_ERR_ALIGN, kw
+    for d, run, size in ((_ce(), lib.pdb_linear_ce_fwd, lib.pdb_linear_ce_fwd_workspace_size),
+                         (_ce_bwd(), lib.pdb_linear_ce_bwd, lib.pdb_linear_ce_bwd_workspace_size)):
+        need = size(C.byref(d))
+        assert need > 0
+        d.workspace, d.workspace_bytes = 256, need - 1
+        assert run(C.byref(d), None) == _lib.PDB_ERR_ARG
+        d.workspace, d.workspace_bytes = 264, need
+        assert run(C.byref(d), None) == _lib.PDB_ERR_ARG
+        assert b"workspace" in lib.pdb_last_error_string()
+
+
+def test_linear_cross_entropy_without_tokens():
+    """No division by the number of tiles there are not."""
+    lib = _lib.load()
+    d, b = _ce(tokens=0), _ce_bwd(tokens=0, dw=None)
+    assert lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) == lib.pdb_linear_ce_bwd_workspace_size(C.byref(b)) == 0
+    assert lib.pdb_linear_ce_fwd(C.byref(d), None) == lib.pdb_linear_ce_bwd(C.byref(b), None) == _lib.PDB_OK
+
+
+@pytest.mark.parametrize("tokens,vocab,width", [(1, 1, 8), (8192, 128000, 4096), (1 << 24, 1 << 24, 1 << 16), (1, 1 << 24, 8)])
+def test_linear_cross_entropy_workspaces(tokens, vocab, width):
+    """The gradient's workspace holds one piece of G (512 MiB, or 256 columns) and f32 sums of dx (and shares of dw
+    while the tiles are fewer than the pairs of SMs)."""
+    lib = _lib.load()
+    kw = dict(tokens=tokens, vocab=vocab, width=width, x_stride=width, w_stride=width)
+    al = lambda n: (n + 255) // 256 * 256
+    tiles = -(-vocab // 256)
+    assert lib.pdb_linear_ce_fwd_workspace_size(C.byref(_ce(**kw))) == al(2 * tiles * tokens * 8) + al(4 * tokens)
+    need = lib.pdb_linear_ce_bwd_workspace_size(C.byref(_ce_bwd(dx_stride=width, dw_stride=width, **kw)))
+    piece = max(512 << 20, tokens * 512)
+    assert 0 < need <= al(piece) + al(80 * 4 * max(tokens * width, 256 * 256) * (1 if tokens < 1 << 20 else 0))         + 4 * tokens * width + 80 * 4 * (1 << 24) * 8 + 4096
+
+
 def test_host_tensors_are_refused():
     import torch
 
@@ -118,6 +185,11 @@ def test_host_tensors_are_refused():
         kernels.layernorm_backward(x, x, v, v)
     with pytest.raises(ValueError, match="CUDA"):
         kernels.rotary(x, inv_freq=[1.0])
+    b, t = x.bfloat16(), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.linear_cross_entropy(b, b, t)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.linear_cross_entropy_backward(b, b, t, v)
 
 
 def test_frequency_refusals():

@@ -1,0 +1,255 @@
+"""The linear head's cross entropy and its gradients against the formulas in 64 bits.
+
+Tolerances, u = 2^-24.  A logit, a dot product of `width` bf16 products summed in f32, is off by at most
+e = (width + 16) u sum|x w|.  exp takes an approximation of 2^-22 and a rounded argument of 2 u |logit|; a row's sum
+of `vocab` positive terms takes at most 8 + vocab / 4096 + 140 steps, so lse is off by
+e + 2^-21 + (150 + vocab / 4096) u + 4 u |lse|.  G is rounded to bf16 (half a step, 2^-8 of itself) after a
+probability with the same relative error; the products that follow sum in f32 and round once more.
+"""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+IGN = -100
+
+
+def _inputs(dev, N, V, W, seed, ignored=0.2, spread=1.5):
+    import torch
+
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    x = torch.randn(N, W, generator=g)
+    w = torch.randn(V, W, generator=g) * spread / W ** 0.5
+    t = torch.randint(0, V, (N,), generator=g)
+    x[::2] += 1.5 * w[t[::2]]
+    t[torch.rand(N, generator=g) < ignored] = IGN
+    dl = torch.randn(N, generator=g) / max(N, 1)
+    return x.to(torch.bfloat16).to(dev), w.to(torch.bfloat16).to(dev), t.to(dev), dl.to(dev)
+
+
+def _logits(x, w):
+    """Logits and their possible error, in 64 bits."""
+    xd, wd = x.double(), w.double()
+    e = (x.shape[1] + 16) * U * (xd.abs() @ wd.abs().T).amax(1)
+    return xd @ wd.T, e
+
+
+def _check_forward(x, w, t, loss, lse):
+    import torch
+
+    z, e = _logits(x, w)
+    ref = torch.logsumexp(z, 1)
+    tol = e + 2.0 ** -21 + (150 + w.shape[0] / 4096) * U + 4 * U * ref.abs()
+    assert ((lse.double() - ref).abs() <= tol).all(), ((lse.double() - ref).abs() / tol).max()
+    valid = t != IGN
+    want = torch.where(valid, ref - z.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+    err = (loss.double() - want).abs()
+    assert (err <= (tol + e + 2 * U * ref.abs()) * valid).all(), (err / tol).max()
+
+
+def _check_backward(x, w, t, dl, lse, dx, dw):
+    import torch
+
+    N, W = x.shape
+    V = w.shape[0]
+    z, e = _logits(x, w)
+    valid = t != IGN
+    up = (dl.double() * valid)[:, None]
+    p = torch.exp(z - lse.double()[:, None])
+    rel = e[:, None] + 2.0 ** -21 + 6 * U * z.abs().amax(1, keepdim=True)
+    perr = p * rel * (1 + rel)
+    G = p.clone()
+    G.scatter_add_(1, t.clamp(min=0)[:, None], torch.full((N, 1), -1.0, dtype=torch.float64, device=x.device))
+    G *= up
+    gerr = up.abs() * (perr + 3 * U) * 1.01 + 2.0 ** -8 * G.abs()
+    wd, xd = w.double(), x.double()
+    if dx is not None:
+        ref = G @ wd
+        tol = (gerr + (V + 16) * U * G.abs()) @ wd.abs() * 1.01 + 2.0 ** -8 * ref.abs() + 1e-38
+        assert ((dx.double() - ref).abs() <= tol).all(), ((dx.double() - ref).abs() / tol).max()
+        assert (dx[~valid] == 0).all()
+    if dw is not None:
+        ref = G.T @ xd
+        tol = (gerr + (N + 16) * U * G.abs()).T @ xd.abs() * 1.01 + 2.0 ** -8 * ref.abs() + 1e-38
+        assert ((dw.double() - ref).abs() <= tol).all(), ((dw.double() - ref).abs() / tol).max()
+
+
+SHAPES = [(1, 1, 8), (1, 500, 64), (3, 257, 72), (130, 1000, 128), (257, 256, 64), (256, 255, 256), (300, 777, 1000),
+          (512, 4099, 256), (1021, 2000, 520), (5, 33000, 16), (2048, 300, 64), (4100, 511, 40), (64, 20000, 2048)]
+
+
+@pytest.mark.parametrize("N,V,W", SHAPES)
+def test_loss_and_gradients(cuda, N, V, W):
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, N, V, W, N + V + W, ignored=0.2 if N > 1 else 0.0)
+    loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    kernels.check_device_errors()
+    _check_forward(x, w, t, loss, lse)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    kernels.check_device_errors()
+    _check_backward(x, w, t, dl, lse, dx, dw)
+
+
+def test_several_pieces(cuda):
+    """A vocabulary that one piece of the gradient's workspace does not hold."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 8192, 70001, 16, 1)
+    loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    _check_forward(x, w, t, loss, lse)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    kernels.check_device_errors()
+    _check_backward(x, w, t, dl, lse, dx, dw)
+
+
+def test_one_gradient_alone_and_lse_recomputed(cuda):
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 200, 900, 128, 2)
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    a, none = kernels.linear_cross_entropy_backward(x, w, t, dl, need_dweight=False)
+    assert none is None and torch.equal(a, dx)
+    none, b = kernels.linear_cross_entropy_backward(x, w, t, dl, need_dx=False)
+    assert none is None and torch.equal(b, dw)
+    assert kernels.linear_cross_entropy_backward(x, w, t, dl, lse, need_dx=False, need_dweight=False) == (None, None)
+
+
+def test_mean_leading_dims_and_strides(cuda):
+    """One dloss for all tokens; (batch, row) tokens; rows of wider matrices, aligned or not; any ignore index."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, _ = _inputs(cuda, 66, 400, 136, 3)
+    lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)[1]
+    mean = torch.full((), 1 / 50, device=cuda)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, mean, lse)
+    _check_backward(x, w, t, mean.expand(66), lse, dx, dw)
+    l3, e3 = kernels.linear_cross_entropy(x.view(6, 11, 136), w, t.view(6, 11), return_lse=True)
+    assert l3.shape == (6, 11) and torch.equal(e3.view(-1), lse)
+    d3, w3 = kernels.linear_cross_entropy_backward(x.view(6, 11, 136), w, t.view(6, 11), mean, e3)
+    assert torch.equal(d3.view(66, 136), dx) and torch.equal(w3, dw)
+    for lo, hi in ((0, 128), (8, 136), (1, 129)):
+        xs, ws = x[:, lo:hi], w[:, lo:hi]
+        ls, es = kernels.linear_cross_entropy(xs, ws, t, return_lse=True)
+        _check_forward(xs, ws, t, ls, es)
+        gx, gw = kernels.linear_cross_entropy_backward(xs, ws, t, mean, es)
+        _check_backward(xs, ws, t, mean.expand(66), es, gx, gw)
+    t0 = t.clone()
+    t0[t == IGN] = 7  # an entry of the vocabulary as the index that is ignored
+    keep = t0 != 7
+    l0 = kernels.linear_cross_entropy(x, w, t0, ignore_index=7)
+    assert (l0[~keep] == 0).all() and torch.equal(l0[keep], kernels.linear_cross_entropy(x, w, t)[keep])
+
+
+def test_nothing_to_do(cuda):
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 40, 300, 64, 4)
+    t[:] = IGN
+    loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    assert (loss == 0).all()
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    assert (dx == 0).all() and (dw == 0).all()
+    x[3] = float("inf")  # in an ignored row: no gradient still
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dx, _ = kernels.linear_cross_entropy_backward(x, w, t, dl, lse, need_dweight=False)
+    assert (dx == 0).all()
+    none = x[:0]
+    loss, lse = kernels.linear_cross_entropy(none, w, t[:0], return_lse=True)
+    dx, dw = kernels.linear_cross_entropy_backward(none, w, t[:0], dl[:0], lse)
+    assert loss.shape == (0,) and dx.shape == (0, 64) and dw.shape == w.shape and (dw == 0).all()
+
+
+def test_targets_outside_the_vocabulary_give_nan(cuda):
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 40, 300, 64, 5, ignored=0.0)
+    good = kernels.linear_cross_entropy(x, w, t)
+    for bad in (300, -1, 2 ** 40, -(2 ** 62)):
+        t2 = t.clone()
+        t2[11] = bad
+        loss, lse = kernels.linear_cross_entropy(x, w, t2, return_lse=True)
+        assert loss[11].isnan() and torch.equal(loss[:11], good[:11]) and torch.equal(loss[12:], good[12:])
+        dx, _ = kernels.linear_cross_entropy_backward(x, w, t2, dl, lse, need_dweight=False)
+        assert dx[11].isnan().all() and dx[:11].isfinite().all() and dx[12:].isfinite().all()
+
+
+def test_large_logits(cuda):
+    """Logits of hundreds, one entry holding all of a row's probability; nothing overflows."""
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 129, 600, 64, 6, spread=150.0)
+    loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    _check_forward(x, w, t, loss, lse)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    _check_backward(x, w, t, dl, lse, dx, dw)
+
+
+def test_the_same_bits_every_time_on_two_streams_and_in_a_graph(cuda):
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 700, 5000, 256, 7)
+
+    def both():
+        loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+        return (loss, lse, *kernels.linear_cross_entropy_backward(x, w, t, dl, lse))
+
+    first = both()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs.append(both())
+    torch.cuda.synchronize()
+    for got in outs:
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    x2, _, t2, dl2 = _inputs(cuda, 700, 5000, 256, 8)
+    x.copy_(x2), t.copy_(t2), dl.copy_(dl2)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(held, both()))
+
+
+def test_gradient_against_differences(cuda):
+    """<dx, a> + <dw, b> against a central difference of sum(dloss * loss) along (a, b), evaluated in 64 bits."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 50, 90, 32, 9)
+    a, b, _, _ = _inputs(cuda, 50, 90, 32, 10)
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    valid = t != IGN
+
+    def at(h):
+        z = (x.double() + h * a.double()) @ (w.double() + h * b.double()).T
+        loss = torch.logsumexp(z, 1) - z.gather(1, t.clamp(min=0)[:, None])[:, 0]
+        return (dl.double() * loss * valid).sum()
+
+    h = 1e-4
+    slope = (at(h) - at(-h)) / (2 * h)
+    got = (dx.double() * a.double()).sum() + (dw.double() * b.double()).sum()
+    # each gradient element is off by at most 2^-8 of itself and 2^-8 of the |G| |operand| sums behind it
+    p = torch.softmax(x.double() @ w.double().T, 1)
+    p.scatter_add_(1, t.clamp(min=0)[:, None], torch.ones(50, 1, dtype=torch.float64, device=cuda))
+    G = p * (dl.double().abs() * valid)[:, None]
+    size = ((G @ w.double().abs()) * a.double().abs()).sum() + ((G.T @ x.double().abs()) * b.double().abs()).sum()
+    assert abs(got - slope) <= (2.0 ** -7 * 1.1 + 100 * h * h) * size

@@ -10,6 +10,8 @@
 // Both directions are HBM-bound: the forward reads x and writes y, the backward
 // reads x and dy and writes dx, each once.  A row belongs to TPR threads, which
 // keep it in registers between its two reductions.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace pdb {
@@ -29,6 +31,25 @@ struct alignas(sizeof(T) * VEC) Pack {
 __device__ __forceinline__ float param_at(const void* p, int bf16, int64_t c) {
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c]) : static_cast<const float*>(p)[c];
 }
+// VEC consecutive parameters from c on; vec: the vectors are 16-byte aligned and so is element c.
+template <int VEC>
+__device__ __forceinline__ void params_at(const void* p, int bf16, int vec, int64_t c, float (&out)[VEC]) {
+  if (VEC > 1 && vec && !bf16) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + i));
+      out[i] = q.x, out[i + 1] = q.y, out[i + 2] = q.z, out[i + 3] = q.w;
+    }
+  } else if (VEC == 8 && vec) {
+    const Pack<__nv_bfloat16, VEC> q =
+        *reinterpret_cast<const Pack<__nv_bfloat16, VEC>*>(static_cast<const __nv_bfloat16*>(p) + c);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = to_f32(q.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = param_at(p, bf16, c + i);
+  }
+}
 __device__ __forceinline__ void param_store(void* p, int bf16, int64_t c, float v) {
   if (bf16)
     static_cast<__nv_bfloat16*>(p)[c] = __float2bfloat16_rn(v);
@@ -43,8 +64,8 @@ struct FwdArgs {
   void* y;
   float* mean;
   float* rstd;
-  int64_t rows, xs, ys;
-  int cols, param_bf16;
+  int64_t rows, xs, ys, chunk;  // chunk: rows per block
+  int cols, param_bf16, param_vec, groups, period, classes;
   float eps, inv_cols;
 };
 
@@ -56,8 +77,8 @@ struct BwdArgs {
   const void* gamma;
   void* dx;
   float* partial;  // [2][groups][cols]: the scale's sums, then the shift's; null without weight gradients
-  int64_t rows, dos, xs, dxs;
-  int cols, param_bf16, groups;
+  int64_t rows, dos, xs, dxs, chunk;  // chunk: rows per block
+  int cols, param_bf16, param_vec, groups, period, classes;
   float inv_cols;
 };
 
@@ -91,61 +112,287 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int slot, int
   }
 }
 
+// The N elements that a thread holds of a row as N / 2 pairs, so that the arithmetic
+// runs on two elements per instruction (with scalar arithmetic both directions were
+// bound by instructions, not by memory: 33 per element in the backward pass).
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void unpack(const Pack<T, VEC> (&raw)[NV], uint64_t (&v)[NV * VEC / 2]) {
+#pragma unroll
+  for (int e = 0; e < NV * VEC; e += 2)
+    v[e / 2] = f2_pack(to_f32(raw[e / VEC].v[e % VEC]), to_f32(raw[(e + 1) / VEC].v[(e + 1) % VEC]));
+}
+template <int VEC, int NV>
+__device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, VEC> (&raw)[NV], uint64_t (&v)[NV * VEC / 2]) {
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) v[i / 2] = f2_pack(to_f32(raw[i].v[0]), to_f32(raw[i + 1].v[0]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j)  // a bf16 is the upper half of its f32
+        v[i * VEC / 2 + j] = f2_pack(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+    }
+  }
+}
+// first: the column of the thread's first element; the vectors lie `step` columns apart.  RAG: a vector may begin
+// before the row or end behind it.
+template <typename T, int VEC, int NV, bool RAG>
+__device__ __forceinline__ void store_pairs(T* row, int first, int step, int cols, const uint64_t (&v)[NV * VEC / 2]) {
+  Pack<T, VEC> o[NV];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < NV * VEC; e += 2)
+      f2_unpack(v[e / 2], o[e / VEC].v[e % VEC], o[(e + 1) / VEC].v[(e + 1) % VEC]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < NV * VEC; e += 2) {
+      float lo, hi;
+      f2_unpack(v[e / 2], lo, hi);
+      const uint32_t w = pack_bf16(lo, hi);
+      if constexpr (VEC > 1) {
+        reinterpret_cast<uint32_t*>(&o[e / VEC])[e % VEC / 2] = w;
+      } else {
+        o[e].v[0] = __ushort_as_bfloat16((unsigned short)w);
+        o[e + 1].v[0] = __ushort_as_bfloat16((unsigned short)(w >> 16));
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = first + i * step;
+    if (RAG ? c >= 0 && c + VEC <= cols : c < cols) {
+      *reinterpret_cast<Pack<T, VEC>*>(row + c) = o[i];
+    } else if (RAG) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c + j >= 0 && c + j < cols) row[c + j] = o[i].v[j];
+    }
+  }
+}
+template <int VEC, int NV, bool RAG>
+__device__ __forceinline__ void load_params(const void* p, int bf16, int vec, int first, int step, int cols, float other,
+                                            uint64_t (&v)[NV * VEC / 2]) {
+  float f[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = first + i * step;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[i][j] = other;
+    if (!p) continue;
+    if constexpr (RAG) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c + j >= 0 && c + j < cols) f[i][j] = param_at(p, bf16, c + j);
+    } else {
+      if (c < cols) params_at<VEC>(p, bf16, vec, c, f[i]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < NV * VEC; e += 2) v[e / 2] = f2_pack(f[e / VEC][e % VEC], f[(e + 1) / VEC][(e + 1) % VEC]);
+}
+__device__ __forceinline__ float f2_total(uint64_t v) {
+  float lo, hi;
+  f2_unpack(v, lo, hi);
+  return lo + hi;
+}
+
+// Each thread copies its own elements of the rows to come into its own slots of
+// shared memory (cp.async) and reads them back itself: loads STAGES rows ahead
+// without registers and without barriers.  Of a copy, the first n bytes are read and
+// the rest is filled with 0: elements past the end of a row, and rows past the end.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int n) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The rows of a block's run, slot by slot (RPB rows at a time), of NT tensors.
+//
+// RAG: rows whose length or distance is no multiple of a 16-byte access.  All rows
+// `period` apart start equally far (`shift` elements) behind a 16-byte boundary, and a
+// block takes rows of one such class only: its threads own aligned vectors, the first
+// one beginning `shift` elements before the row, and the columns of a thread stay the
+// same from row to row.  (Element by element, 32768 rows of 1001 bf16 took 70 us in
+// the backward pass, and this way 45.)
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, int NT, bool RAG>
+struct Rows {
+  // cp.async moves 4 bytes at least; smaller elements come one row ahead through registers
+  static constexpr bool kAsync = sizeof(T) * VEC >= 4;
+  static constexpr int RPB = BT / TPR;
+  static constexpr int kBytes = kAsync ? BT * STAGES * NT * NV * VEC * (int)sizeof(T) : 0;
+  using P = Pack<T, VEC>;
+  P* slots;  // [STAGES][NT][NV][BT]
+  const T* base[NT];
+  const T* src[NT];  // this thread's first element in the row that is fetched next
+  int64_t step[NT], ahead, last;
+  int first_col, cols, head, tail;
+  P reg[NT][NV];
+
+  __device__ __forceinline__ void init(int n, const void* p, int64_t stride, int64_t row, int period) {
+    base[n] = static_cast<const T*>(p);
+    src[n] = base[n] + row * stride + first_col;
+    step[n] = RPB * period * stride;
+  }
+  // `at` and `end` count rows of the block's class
+  __device__ __forceinline__ void start(void* smem, int64_t at, int64_t end) {
+    slots = static_cast<P*>(smem);
+    ahead = at, last = end;
+    head = tail = 0;
+#pragma unroll
+    for (int i = 0; i < (kAsync ? STAGES - 1 : 1); ++i) fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    const bool in = ahead < last;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = first_col + i * TPR * VEC;
+        const bool read = in && c < cols;
+        const T* s = read ? src[n] + i * TPR * VEC : base[n];
+        if constexpr (kAsync) {
+          const int count = !read ? 0 : RAG ? min(VEC, cols - c) : VEC;
+          copy_async<sizeof(P)>(smem_u32(slots + ((head * NT + n) * NV + i) * BT + threadIdx.x), s, count * (int)sizeof(T));
+        } else {
+          reg[n][i] = {};
+          if (read) reg[n][i] = *reinterpret_cast<const P*>(s);
+        }
+      }
+      src[n] += step[n];
+    }
+    if constexpr (kAsync) copy_commit();
+    head = head + 1 == STAGES ? 0 : head + 1;
+    ahead += RPB;
+  }
+  // The oldest row's elements as f32 pairs (0 outside the row), and the next fetch.  A slot is filled again a row
+  // after it was read.
+  __device__ __forceinline__ void take(uint64_t (&v)[NT][NV * VEC / 2]) {
+    if constexpr (kAsync) copy_wait<STAGES - 2>();
+    P c[NT][NV];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c[n][i] = kAsync ? slots[((tail * NT + n) * NV + i) * BT + threadIdx.x] : reg[n][i];
+    tail = tail + 1 == STAGES ? 0 : tail + 1;
+    if (RAG && first_col < 0) {  // the end of the row before
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (first_col + j < 0) from_f32(c[n][0].v[j], 0.f);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) unpack(c[n], v[n]);
+    fetch();
+  }
+  __device__ __forceinline__ void drain() {
+    if constexpr (kAsync) copy_wait<0>();
+  }
+};
+
+// A block's rows: the rows r = cls + period * j, j in [first, last).
+struct Run {
+  int cls, period;
+  int64_t first, last;
+  __device__ __forceinline__ Run(int64_t rows, int period_, int classes, int64_t chunk) : period(period_) {
+    cls = blockIdx.x % classes;
+    first = blockIdx.x / classes * chunk;
+    last = min((rows - cls + period - 1) / period, first + chunk);
+  }
+  __device__ __forceinline__ int64_t row(int64_t j) const { return cls + period * j; }
+};
+
+// How many elements row `cls` starts behind a 16-byte boundary.
+template <typename T, bool RAG>
+__device__ __forceinline__ int row_shift(const void* p, int64_t stride, int cls) {
+  if constexpr (!RAG) return 0;
+  return (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T) + cls * stride) % (16 / sizeof(T)));
+}
+
 // ---------------------------------------------------------------- forward
-template <typename T, int VEC, int NV, int TPR, int BT>
+// A block takes a run of rows; scale and shift stay in registers.
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 __global__ void __launch_bounds__(BT) layernorm_fwd_kernel(const FwdArgs p) {
-  constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1;
+  constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
   __shared__ float red[RPB * 2 * NW];
+  extern __shared__ __align__(16) uint8_t dyn[];
   const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + slot;
-  if (TPR >= 32 && row >= p.rows) return;  // whole warps (and whole barrier groups) leave together
-  const bool live = row < p.rows;
-  const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.xs;
-  T* yr = static_cast<T*>(p.y) + (live ? row : 0) * p.ys;
-  Pack<T, VEC> raw[NV];
-  float s[1] = {0.f};
+  const Run run(p.rows, p.period, p.classes, p.chunk);
+  const int first_col = l * VEC - row_shift<T, RAG>(p.x, p.xs, run.cls);
+  Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG> rows;
+  rows.first_col = first_col;
+  rows.cols = p.cols;
+  rows.init(0, p.x, p.xs, run.row(run.first + slot), run.period);
+  rows.start(dyn, run.first + slot, run.last);
+  uint64_t g[N2], b[N2];
+  load_params<VEC, NV, RAG>(p.gamma, p.param_bf16, p.param_vec, first_col, TPR * VEC, p.cols, 1.f, g);
+  load_params<VEC, NV, RAG>(p.beta, p.param_bf16, p.param_vec, first_col, TPR * VEC, p.cols, 0.f, b);
   int phase = 0;
+  for (int64_t j0 = run.first; j0 < run.last; j0 += RPB) {
+    if (TPR >= 32 && j0 + slot >= run.last) break;  // whole warps (and whole barrier groups) leave together
+    uint64_t v[1][N2];
+    rows.take(v);
+    uint64_t a = f2_pack(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (l + i * TPR) * VEC;
-    if (c < p.cols) {
-      raw[i] = *reinterpret_cast<const Pack<T, VEC>*>(xr + c);
+    for (int e = 0; e < N2; ++e) a = f2_add(a, v[0][e]);
+    float s[1] = {f2_total(a)};
+    row_sum<TPR, 1>(s, red, slot, phase);
+    const float mean = s[0] * p.inv_cols;
+    const uint64_t m2 = f2_pack(mean, mean);
+    a = f2_pack(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s[0] += to_f32(raw[i].v[j]);
+    for (int e = 0; e < N2; ++e) v[0][e] = f2_sub(v[0][e], m2);
+    // elements outside the row hold 0 - mean and must not count
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = first_col + i * TPR * VEC;
+      if constexpr (VEC == 1) {
+        if (i % 2 == 0) {
+          float lo, hi;
+          f2_unpack(v[0][i / 2], lo, hi);
+          const uint64_t d = f2_pack(c < p.cols ? lo : 0.f, c + TPR < p.cols ? hi : 0.f);
+          a = f2_fma(d, d, a);
+        }
+      } else if (RAG && (c < 0 || c + VEC > p.cols)) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          float lo, hi;
+          f2_unpack(v[0][(i * VEC + j) / 2], lo, hi);
+          const uint64_t d = f2_pack(c + j >= 0 && c + j < p.cols ? lo : 0.f, c + j + 1 >= 0 && c + j + 1 < p.cols ? hi : 0.f);
+          a = f2_fma(d, d, a);
+        }
+      } else {
+        uint64_t q = f2_pack(0.f, 0.f);
+#pragma unroll
+        for (int j = i * VEC / 2; j < (i + 1) * VEC / 2; ++j) q = f2_fma(v[0][j], v[0][j], q);
+        if (c < p.cols) a = f2_add(a, q);
+      }
+    }
+    s[0] = f2_total(a);
+    row_sum<TPR, 1>(s, red, slot, phase);
+    const float rstd = 1.0f / sqrtf(s[0] * p.inv_cols + p.eps);
+    if (j0 + slot < run.last) {
+      const int64_t row = run.row(j0 + slot);
+      if (l == 0) {
+        if (p.mean) p.mean[row] = mean;
+        if (p.rstd) p.rstd[row] = rstd;
+      }
+      const uint64_t r2 = f2_pack(rstd, rstd);
+#pragma unroll
+      for (int e = 0; e < N2; ++e) v[0][e] = f2_fma(f2_mul(v[0][e], r2), g[e], b[e]);
+      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.y) + row * p.ys, first_col, TPR * VEC, p.cols, v[0]);
     }
   }
-  row_sum<TPR, 1>(s, red, slot, phase);
-  const float mean = s[0] * p.inv_cols;
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((l + i * TPR) * VEC < p.cols)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = to_f32(raw[i].v[j]) - mean;
-        s[0] = fmaf(d, d, s[0]);
-      }
-  row_sum<TPR, 1>(s, red, slot, phase);
-  const float rstd = 1.0f / sqrtf(s[0] * p.inv_cols + p.eps);
-  if (!live) return;
-  if (l == 0) {
-    if (p.mean) p.mean[row] = mean;
-    if (p.rstd) p.rstd[row] = rstd;
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (l + i * TPR) * VEC;
-    if (c < p.cols) {
-      Pack<T, VEC> o;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float g = p.gamma ? param_at(p.gamma, p.param_bf16, c + j) : 1.f;
-        const float b = p.beta ? param_at(p.beta, p.param_bf16, c + j) : 0.f;
-        from_f32(o.v[j], fmaf((to_f32(raw[i].v[j]) - mean) * rstd, g, b));
-      }
-      *reinterpret_cast<Pack<T, VEC>*>(yr + c) = o;
-    }
-  }
+  rows.drain();
 }
 
 // Rows too long for registers: one block per row, re-read in each of three passes.
@@ -196,102 +443,107 @@ __global__ void __launch_bounds__(kLoopThreads) layernorm_fwd_loop_kernel(const 
 }
 
 // --------------------------------------------------------------- backward
-// A block takes rows at a stride of the grid and keeps, per thread, the sums of
-// dy z and dy over its rows for the columns that the thread owns; the row slots
-// of the block are added in shared memory at the end, one partial row per block.
-template <typename T, int VEC, int NV, int TPR, int BT>
-__global__ void __launch_bounds__(BT) layernorm_bwd_kernel(const BwdArgs p) {
-  constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1;
+// Bytes of dynamic shared memory: the slots, or the columns' sums at the end.
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES>
+constexpr int bwd_smem() {
+  const int slots = Rows<T, VEC, NV, TPR, BT, STAGES, 2, false>::kBytes;
+  const int sums = BT > TPR ? BT * NV * VEC * (int)sizeof(float) : 0;
+  return slots > sums ? slots : sums;
+}
+
+// A block takes a run of rows and keeps, per thread, the sums of dy z and dy over its
+// rows for the columns that the thread owns; the row slots of the block are added in
+// shared memory at the end, one partial row per block.
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+__global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernorm_bwd_kernel(const BwdArgs p) {
+  constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
   __shared__ float red[RPB * 2 * NW * 2];
-  extern __shared__ float cols_s[];  // [RPB][TPR * NV * VEC], when RPB > 1
+  extern __shared__ __align__(16) uint8_t dyn[];
   const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
-  float ag[NV][VEC], ab[NV][VEC], g[NV][VEC];
+  const Run run(p.rows, p.period, p.classes, p.chunk);
+  const int first_col = l * VEC - row_shift<T, RAG>(p.x, p.xs, run.cls);
+  Rows<T, VEC, NV, TPR, BT, STAGES, 2, RAG> rows;
+  rows.first_col = first_col;
+  rows.cols = p.cols;
+  rows.init(0, p.x, p.xs, run.row(run.first + slot), run.period);
+  rows.init(1, p.dout, p.dos, run.row(run.first + slot), run.period);
+  rows.start(dyn, run.first + slot, run.last);
+  uint64_t ag[N2], ab[N2], g[N2];
+  const uint64_t zero2 = f2_pack(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int c = (l + i * TPR) * VEC + j;
-      ag[i][j] = ab[i][j] = 0.f;
-      g[i][j] = (p.gamma && c < p.cols) ? param_at(p.gamma, p.param_bf16, c) : 1.f;
+  for (int e = 0; e < N2; ++e) ag[e] = ab[e] = zero2;
+  load_params<VEC, NV, RAG>(p.gamma, p.param_bf16, p.param_vec, first_col, TPR * VEC, p.cols, 1.f, g);
+  // the statistics of this row slot's next W rows, one row per lane, and of the W rows after
+  constexpr int W = TPR < 32 ? TPR : 32;
+  const int lane = l % W;
+  auto stat = [&](const float* s, int64_t j) {
+    j += slot + lane * RPB;
+    return j < run.last ? s[run.row(j)] : 0.f;
+  };
+  float mean_w = stat(p.mean, run.first), rstd_w = stat(p.rstd, run.first);
+  float mean_n = stat(p.mean, run.first + W * RPB), rstd_n = stat(p.rstd, run.first + W * RPB);
+  int phase = 0, it = 0;
+  for (int64_t j0 = run.first; j0 < run.last; j0 += RPB, ++it) {
+    if (TPR >= 32 && j0 + slot >= run.last) break;
+    if (it == W) {
+      it = 0;
+      mean_w = mean_n, rstd_w = rstd_n;
+      mean_n = stat(p.mean, j0 + W * RPB), rstd_n = stat(p.rstd, j0 + W * RPB);
     }
-  int phase = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = r0 + slot;
-    if (TPR >= 32 && row >= p.rows) break;
-    const bool live = row < p.rows;
-    const int64_t rr = live ? row : 0;
-    const T* xr = static_cast<const T*>(p.x) + rr * p.xs;
-    const T* dr = static_cast<const T*>(p.dout) + rr * p.dos;
-    T* wr = static_cast<T*>(p.dx) + rr * p.dxs;
-    const float mean = p.mean[rr], rstd = p.rstd[rr];
-    Pack<T, VEC> xv[NV], dv[NV];
-    float s[2] = {0.f, 0.f};
+    const float mean = __shfl_sync(0xffffffffu, mean_w, it, W), rstd = __shfl_sync(0xffffffffu, rstd_w, it, W);
+    uint64_t v[2][N2];
+    rows.take(v);
+    auto &z = v[0], &dz = v[1];
+    // z as one fused step: the rounding of mean * rstd is of the size of mean's own
+    const uint64_t r2 = f2_pack(rstd, rstd), mr2 = f2_pack(-mean * rstd, -mean * rstd);
+    uint64_t s0 = zero2, s1 = zero2;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (l + i * TPR) * VEC;
-      if (live && c < p.cols) {
-        xv[i] = *reinterpret_cast<const Pack<T, VEC>*>(xr + c);
-        dv[i] = *reinterpret_cast<const Pack<T, VEC>*>(dr + c);
-      }
+    for (int e = 0; e < N2; ++e) {
+      z[e] = f2_fma(z[e], r2, mr2);
+      ab[e] = f2_add(ab[e], dz[e]);
+      ag[e] = f2_fma(dz[e], z[e], ag[e]);
+      dz[e] = f2_mul(dz[e], g[e]);
+      s0 = f2_add(s0, dz[e]);
+      s1 = f2_fma(dz[e], z[e], s1);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (live && (l + i * TPR) * VEC < p.cols)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float z = (to_f32(xv[i].v[j]) - mean) * rstd, dy = to_f32(dv[i].v[j]);
-          const float dz = dy * g[i][j];
-          s[0] += dz;
-          s[1] = fmaf(dz, z, s[1]);
-          ab[i][j] += dy;
-          ag[i][j] = fmaf(dy, z, ag[i][j]);
-        }
-    }
+    float s[2] = {f2_total(s0), f2_total(s1)};
     row_sum<TPR, 2>(s, red, slot, phase);
-    const float m0 = s[0] * p.inv_cols, m1 = s[1] * p.inv_cols;
+    const float k0 = -s[0] * p.inv_cols * rstd, k1 = -s[1] * p.inv_cols * rstd;
+    const uint64_t k02 = f2_pack(k0, k0), k12 = f2_pack(k1, k1);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (l + i * TPR) * VEC;
-      if (live && c < p.cols) {
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float z = (to_f32(xv[i].v[j]) - mean) * rstd;
-          from_f32(o.v[j], rstd * (fmaf(to_f32(dv[i].v[j]), g[i][j], -m0) - z * m1));
-        }
-        *reinterpret_cast<Pack<T, VEC>*>(wr + c) = o;
-      }
-    }
+    for (int e = 0; e < N2; ++e) dz[e] = f2_fma(z[e], k12, f2_fma(dz[e], r2, k02));
+    if (j0 + slot < run.last)
+      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.dx) + run.row(j0 + slot) * p.dxs, first_col, TPR * VEC, p.cols, dz);
   }
+  rows.drain();
   if (!p.partial) return;
   const int64_t half = (int64_t)p.groups * p.cols;
   float* out = p.partial + (int64_t)blockIdx.x * p.cols;
-  if constexpr (RPB == 1) {
+  float* sums = reinterpret_cast<float*>(dyn);  // [RPB][TPR * NV * VEC]
+  constexpr int WIDTH = TPR * NV * VEC;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+  for (int which = 0; which < 2; ++which) {
+    float f[NV * VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int c = (l + i * TPR) * VEC + j;
-        if (c < p.cols) {
-          out[c] = ag[i][j];
-          out[half + c] = ab[i][j];
-        }
+    for (int e = 0; e < N2; ++e) f2_unpack(which ? ab[e] : ag[e], f[2 * e], f[2 * e + 1]);
+    if constexpr (RPB == 1) {
+#pragma unroll
+      for (int e = 0; e < NV * VEC; ++e) {
+        const int c = first_col + e / VEC * TPR * VEC + e % VEC;
+        if (c >= 0 && c < p.cols) out[which * half + c] = f[e];
       }
-  } else {
-    constexpr int WIDTH = TPR * NV * VEC;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
+    } else {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          cols_s[slot * WIDTH + (l + i * TPR) * VEC + j] = which ? ab[i][j] : ag[i][j];
+      for (int e = 0; e < NV * VEC; ++e) {
+        const int c = first_col + e / VEC * TPR * VEC + e % VEC;
+        if (c >= 0) sums[slot * WIDTH + c] = f[e];
+      }
       __syncthreads();
       for (int c = threadIdx.x; c < p.cols; c += BT) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < RPB; ++r) s += cols_s[r * WIDTH + c];
+        for (int r = 0; r < RPB; ++r) s += sums[r * WIDTH + c];
         out[which * half + c] = s;
       }
     }
@@ -339,31 +591,48 @@ __global__ void __launch_bounds__(kColThreads) layernorm_bwd_columns_kernel(cons
   p.partial[((int64_t)p.groups + blockIdx.y) * p.cols + c] = b;
 }
 
-// The partial rows of all blocks, added in a fixed order: a warp takes 32 columns
-// of one of the two gradients, 8 warps of a block share the partial rows.
-constexpr int kFinWarps = 8;
+// The partial rows of all blocks, added in a fixed order: a block takes 32 columns
+// of one of the two gradients, its 32 warps a share of the partial rows each, eight
+// loads in flight (one after another, 300 rows took longer than the pass before).
+constexpr int kFinWarps = 32, kFinUnroll = 8;
 
 __global__ void __launch_bounds__(32 * kFinWarps)
     layernorm_bwd_finish_kernel(const float* partial, int groups, int cols, void* dgamma, void* dbeta, int param_bf16) {
-  __shared__ float s[kFinWarps][32];
+  __shared__ float s[kFinWarps][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
-  const float* src = partial + (int64_t)blockIdx.y * groups * cols;
+  grid_dep_wait();
+  const float* src = partial + (int64_t)blockIdx.y * groups * cols + c;
   float v = 0.f;
-  if (c < cols)
-    for (int r = w; r < groups; r += kFinWarps) v += src[(int64_t)r * cols + c];
+  if (c < cols) {
+    int r = w;
+    for (; r + (kFinUnroll - 1) * kFinWarps < groups; r += kFinUnroll * kFinWarps) {
+      float q[kFinUnroll];
+#pragma unroll
+      for (int i = 0; i < kFinUnroll; ++i) q[i] = src[(int64_t)(r + i * kFinWarps) * cols];
+#pragma unroll
+      for (int i = 0; i < kFinUnroll; ++i) v += q[i];
+    }
+    for (; r < groups; r += kFinWarps) v += src[(int64_t)r * cols];
+  }
   s[w][lane] = v;
   __syncthreads();
-  if (w == 0 && c < cols) {
+  // the block's 32 x 32 sums turned: a warp adds one column's 32 shares
+  v = s[lane][w];
 #pragma unroll
-    for (int i = 1; i < kFinWarps; ++i) v += s[i][lane];
-    param_store(blockIdx.y ? dbeta : dgamma, param_bf16, c, v);
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0 && blockIdx.x * 32 + w < cols) param_store(blockIdx.y ? dbeta : dgamma, param_bf16, blockIdx.x * 32 + w, v);
 }
 
 // ------------------------------------------------------------------- host
 bool aligned(const void* p, int64_t stride, int vec, int size) {
   return reinterpret_cast<uintptr_t>(p) % (uintptr_t)(vec * size) == 0 && stride % vec == 0;
+}
+
+bool typed(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == PDB_F32 ? 4 : 2) == 0; }
+
+int param_vec(const void* g, const void* b) {
+  return ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
 constexpr int kMaxCols = 1 << 30;
@@ -378,71 +647,130 @@ int check(int64_t rows, int64_t cols, int32_t dtype, int32_t param_dtype) {
   return PDB_OK;
 }
 
-// The widths that a row's threads and registers give: VEC elements x NV vectors x
-// TPR threads.  The smallest that holds the row is taken.
-template <typename T, int VEC, int NV, int TPR, int BT>
-void launch_fwd(const FwdArgs& p, cudaStream_t s) {
-  const int64_t grid = (p.rows + BT / TPR - 1) / (BT / TPR);
-  layernorm_fwd_kernel<T, VEC, NV, TPR, BT><<<(unsigned)grid, BT, 0, s>>>(p);
+// A launch's shape: NV vectors of VEC elements per thread, TPR threads per row, BT per
+// block; `blocks` of them per SM share the rows of every class in runs.
+template <typename Args>
+void share_rows(Args& p, int rpb, int64_t blocks) {
+  p.classes = (int)std::min<int64_t>(p.period, p.rows);
+  const int64_t each = (p.rows + p.period - 1) / p.period, sets = (each + rpb - 1) / rpb;
+  const int64_t runs = std::max<int64_t>(1, blocks / p.classes);
+  p.chunk = (sets + runs - 1) / runs * rpb;
+  p.groups = (int)((each + p.chunk - 1) / p.chunk * p.classes);
 }
 
-template <typename T, int VEC>
-bool dispatch_fwd(const FwdArgs& p, cudaStream_t s) {
-  const int64_t nv = ((int64_t)p.cols + VEC - 1) / VEC;
-  if (nv <= 16) launch_fwd<T, VEC, 1, 16, 256>(p, s);
-  else if (nv <= 32) launch_fwd<T, VEC, 1, 32, 256>(p, s);
-  else if (nv <= 64) launch_fwd<T, VEC, 2, 32, 256>(p, s);
-  else if (nv <= 128) launch_fwd<T, VEC, 4, 32, 256>(p, s);
-  else if (nv <= 256) launch_fwd<T, VEC, 2, 128, 256>(p, s);
-  else if (nv <= 512) launch_fwd<T, VEC, 2, 256, 256>(p, s);
-  else if (nv <= 1024) launch_fwd<T, VEC, 4, 256, 256>(p, s);
-  else if (nv <= 2048) launch_fwd<T, VEC, 4, 512, 512>(p, s);
-  else if (nv <= 4096) launch_fwd<T, VEC, 4, 1024, 1024>(p, s);
-  else return false;
-  return true;
+int sms() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return sm_count(dev);
 }
+
+// The most blocks that share the rows of the backward pass.
+int64_t bwd_groups(int64_t rows, int sms) { return std::max<int64_t>(8, std::min<int64_t>(rows + 8, 4 * sms)); }
 
 template <typename T>
-int forward(const FwdArgs& p, cudaStream_t s) {
+bool rag_fits(const void* a, int64_t as, const void* b, int64_t bs) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.cols % V == 0 && aligned(p.x, p.xs, V, sizeof(T)) && aligned(p.y, p.ys, V, sizeof(T));
-  if (!(vec ? dispatch_fwd<T, V>(p, s) : dispatch_fwd<T, 1>(p, s)))
-    layernorm_fwd_loop_kernel<T><<<(unsigned)p.rows, kLoopThreads, 0, s>>>(p);
-  return cuda_status(cudaGetLastError(), "layernorm forward launch");
+  return reinterpret_cast<uintptr_t>(a) % 16 == reinterpret_cast<uintptr_t>(b) % 16 && (as - bs) % V == 0;
+}
+template <typename T>
+int rag_period(int64_t stride) {
+  int p = 16 / sizeof(T);
+  while (p > 1 && stride * (p / 2) % (16 / (int)sizeof(T)) == 0) p /= 2;
+  return p;
 }
 
-// Blocks that share the rows of the backward pass: two per SM, never more than there are rows.
-int bwd_groups(int64_t rows, int sms) {
-  const int64_t g = 2 * (int64_t)sms;
-  return (int)(rows < g ? (rows > 0 ? rows : 1) : g);
-}
-
-template <typename T, int VEC, int NV, int TPR, int BT>
-int launch_bwd(const BwdArgs& p, cudaStream_t s) {
-  const int smem = BT / TPR > 1 ? BT * NV * VEC * (int)sizeof(float) : 0;
-  layernorm_bwd_kernel<T, VEC, NV, TPR, BT><<<(unsigned)p.groups, BT, smem, s>>>(p);
+// 1: launched, 0: the row is too long for this shape, -1: an error
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
+  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC) return 0;
+  constexpr int smem = Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG>::kBytes;
+  auto kernel = layernorm_fwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>;
+  if (smem > 40 * 1024)  // with the static arrays, 48 KB would be passed
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+      return cuda_status(e, "layernorm: smem attribute"), -1;
+  share_rows(p, BT / TPR, (int64_t)blocks * sms());
+  kernel<<<(unsigned)p.groups, BT, smem, s>>>(p);
   return 1;
 }
 
-template <typename T, int VEC>
-int dispatch_bwd(const BwdArgs& p, cudaStream_t s) {
-  const int64_t nv = ((int64_t)p.cols + VEC - 1) / VEC;
-  if (nv <= 16) return launch_bwd<T, VEC, 1, 16, 256>(p, s);
-  if (nv <= 32) return launch_bwd<T, VEC, 1, 32, 256>(p, s);
-  if (nv <= 64) return launch_bwd<T, VEC, 1, 64, 256>(p, s);
-  if (nv <= 128) return launch_bwd<T, VEC, 1, 128, 256>(p, s);
-  if (nv <= 256) return launch_bwd<T, VEC, 1, 256, 256>(p, s);
-  if (nv <= 512) return launch_bwd<T, VEC, 2, 256, 256>(p, s);
-  if (nv <= 1024) return launch_bwd<T, VEC, 2, 512, 512>(p, s);
-  return 0;
+// 32 elements per thread in the forward (16 of f32), 256 threads per block and 4 blocks per SM; measured over 32 MiB
+// elements of bf16: 24.7-25 us at 256 to 8192 columns, a copy's time.  Element by element (tensors whose rows lie
+// differently against 16 bytes) a thread takes 8, or 16 of long rows.
+template <typename T, int VEC, bool RAG>
+int dispatch_fwd(FwdArgs& p, cudaStream_t s) {
+  constexpr int NV = VEC == 1 ? 8 : sizeof(T) == 2 ? 32 / VEC : 16 / VEC;
+  int r = launch_fwd<T, VEC, NV, 8, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, NV, 16, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, NV, 32, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, NV, 64, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, NV, 128, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, NV, 256, 256, 3, RAG>(p, 4, s);
+  if (!r) r = launch_fwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, 2, RAG>(p, 2, s);
+  return r;
 }
 
 template <typename T>
-int backward(const BwdArgs& p, cudaStream_t s) {
+int forward(FwdArgs& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.cols % V == 0 && aligned(p.x, p.xs, V, sizeof(T)) && aligned(p.dout, p.dos, V, sizeof(T)) &&
-                   aligned(p.dx, p.dxs, V, sizeof(T));
-  if (!(vec ? dispatch_bwd<T, V>(p, s) : dispatch_bwd<T, 1>(p, s))) {
+  int done;
+  if (p.cols % V == 0 && aligned(p.x, p.xs, V, sizeof(T)) && aligned(p.y, p.ys, V, sizeof(T))) {
+    done = dispatch_fwd<T, V, false>(p, s);
+  } else if (rag_fits<T>(p.x, p.xs, p.y, p.ys)) {
+    p.period = rag_period<T>(p.xs);
+    done = dispatch_fwd<T, V, true>(p, s);
+  } else {
+    done = dispatch_fwd<T, 1, false>(p, s);
+  }
+  if (done < 0) return PDB_ERR_CUDA;
+  if (!done) layernorm_fwd_loop_kernel<T><<<(unsigned)p.rows, kLoopThreads, 0, s>>>(p);
+  return cuda_status(cudaGetLastError(), "layernorm forward launch");
+}
+
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
+  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC) return 0;
+  constexpr int smem = bwd_smem<T, VEC, NV, TPR, BT, STAGES>();
+  auto kernel = layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>;
+  if (smem > 40 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+      return cuda_status(e, "layernorm backward: smem attribute"), -1;
+  share_rows(p, BT / TPR, (int64_t)blocks * sms());
+  kernel<<<(unsigned)p.groups, BT, smem, s>>>(p);
+  return 1;
+}
+
+// 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
+// elements of bf16 with the sums' join: 39-40 us at 128 to 2048 columns, a copy of as many bytes 37.  8192 columns of
+// f32 keep two rows (196 KB for three leave the caches too little: 84 against 76 us).
+template <typename T, int VEC, bool RAG>
+int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
+  constexpr int NV = VEC == 1 ? 4 : 16 / VEC, N = VEC == 1 ? 3 : 2;
+  int r = launch_bwd<T, VEC, NV, 8, 256, 3, RAG>(p, N, s);
+  if (!r) r = launch_bwd<T, VEC, NV, 16, 256, 3, RAG>(p, N, s);
+  if (!r) r = launch_bwd<T, VEC, NV, 32, 256, 3, RAG>(p, N, s);
+  if (!r) r = launch_bwd<T, VEC, NV, 64, 256, 3, RAG>(p, N, s);
+  if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, N, s);
+  if (!r) r = launch_bwd<T, VEC, NV, 256, VEC == 1 ? 256 : 512, 3, RAG>(p, VEC == 1 ? 3 : 1, s);
+  if (!r) r = launch_bwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, sizeof(T) == 4 ? 2 : 3, RAG>(p, 1, s);
+  return r;
+}
+
+template <typename T>
+int backward(BwdArgs& p, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  int done;
+  if (p.cols % V == 0 && aligned(p.x, p.xs, V, sizeof(T)) && aligned(p.dout, p.dos, V, sizeof(T)) &&
+      aligned(p.dx, p.dxs, V, sizeof(T))) {
+    done = dispatch_bwd<T, V, false>(p, s);
+  } else if (rag_fits<T>(p.x, p.xs, p.dout, p.dos) && rag_fits<T>(p.x, p.xs, p.dx, p.dxs)) {
+    p.period = rag_period<T>(p.xs);
+    done = dispatch_bwd<T, V, true>(p, s);
+  } else {
+    done = dispatch_bwd<T, 1, false>(p, s);
+  }
+  if (done < 0) return PDB_ERR_CUDA;
+  if (!done) {
+    p.groups = (int)std::min<int64_t>(p.rows, 4 * sms());
     layernorm_bwd_loop_kernel<T><<<(unsigned)p.rows, kLoopThreads, 0, s>>>(p);
     if (p.partial)
       layernorm_bwd_columns_kernel<T>
@@ -465,17 +793,17 @@ extern "C" int pdb_layernorm_fwd(const pdb_layernorm_fwd_desc* d, void* stream) 
     return set_error(PDB_ERR_SHAPE, "layernorm: rows without columns have no statistics");
   if (d->rows == 0 || d->cols == 0) return PDB_OK;
   if (!d->x || !d->y) return set_error(PDB_ERR_ARG, "null x / y");
-  const FwdArgs p{d->x, d->gamma, d->beta, d->y, d->mean, d->rstd, d->rows, d->x_row_stride, d->y_row_stride,
-                  (int)d->cols, d->param_dtype == PDB_BF16, (float)d->eps, (float)(1.0 / (double)d->cols)};
+  if (!typed(d->x, d->dtype) || !typed(d->y, d->dtype) || !typed(d->gamma, d->param_dtype) || !typed(d->beta, d->param_dtype))
+    return set_error(PDB_ERR_ALIGN, "layernorm: a tensor is not aligned to its type");
+  FwdArgs p{d->x, d->gamma, d->beta, d->y, d->mean, d->rstd, d->rows, d->x_row_stride, d->y_row_stride,
+                  0, (int)d->cols, d->param_dtype == PDB_BF16, param_vec(d->gamma, d->beta), 0, 1, 1, (float)d->eps, (float)(1.0 / (double)d->cols)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return d->dtype == PDB_F32 ? forward<float>(p, s) : forward<__nv_bfloat16>(p, s);
 }
 
 extern "C" size_t pdb_layernorm_bwd_workspace_size(const pdb_layernorm_bwd_desc* d) {
   if (!d || d->rows < 0 || d->cols <= 0 || d->cols > kMaxCols || !d->dgamma) return 0;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  return (size_t)2 * bwd_groups(d->rows, sm_count(dev)) * d->cols * sizeof(float);
+  return (size_t)2 * bwd_groups(d->rows, sms()) * d->cols * sizeof(float);
 }
 
 extern "C" int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream) {
@@ -490,17 +818,28 @@ extern "C" int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream) 
     return set_error(PDB_ERR_ARG, "null x / dout / dx / mean / rstd");
   if (d->dgamma && (!d->workspace || d->workspace_bytes < pdb_layernorm_bwd_workspace_size(d)))
     return set_error(PDB_ERR_ARG, "layernorm backward: workspace too small");
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const BwdArgs p{d->dout, d->x, d->mean, d->rstd, d->gamma, d->dx,
+  if (!typed(d->x, d->dtype) || !typed(d->dout, d->dtype) || !typed(d->dx, d->dtype) || !typed(d->gamma, d->param_dtype) ||
+      !typed(d->dgamma, d->param_dtype) || !typed(d->dbeta, d->param_dtype) || !typed(d->workspace, PDB_F32))
+    return set_error(PDB_ERR_ALIGN, "layernorm backward: a tensor is not aligned to its type");
+  BwdArgs p{d->dout, d->x, d->mean, d->rstd, d->gamma, d->dx,
                   d->dgamma ? static_cast<float*>(d->workspace) : nullptr, d->rows, d->dout_row_stride,
-                  d->x_row_stride, d->dx_row_stride, (int)d->cols, d->param_dtype == PDB_BF16,
-                  bwd_groups(d->rows, sm_count(dev)), (float)(1.0 / (double)d->cols)};
+                  d->x_row_stride, d->dx_row_stride, 0, (int)d->cols, d->param_dtype == PDB_BF16,
+                  param_vec(d->gamma, nullptr), 0, 1, 1, (float)(1.0 / (double)d->cols)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->rows > 0)
     if (int st = d->dtype == PDB_F32 ? backward<float>(p, s) : backward<__nv_bfloat16>(p, s)) return st;
   if (!d->dgamma) return PDB_OK;
-  layernorm_bwd_finish_kernel<<<dim3((unsigned)((d->cols + 31) / 32), 2), 32 * kFinWarps, 0, s>>>(
-      p.partial, d->rows > 0 ? p.groups : 0, p.cols, d->dgamma, d->dbeta, p.param_bf16);
-  return cuda_status(cudaGetLastError(), "layernorm backward finish launch");
+  // its blocks may be scheduled while the pass before drains; they wait for that pass's memory
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((d->cols + 31) / 32), 2);
+  cfg.blockDim = dim3(32 * kFinWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, layernorm_bwd_finish_kernel, (const float*)p.partial,
+                                        d->rows > 0 ? p.groups : 0, p.cols, d->dgamma, d->dbeta, p.param_bf16),
+                     "layernorm backward finish launch");
 }

@@ -21,7 +21,7 @@
 // MN-major (its rows are the contracted index): G^T, x and w enter dw and dx that
 // way, as they lie in memory.
 #include <algorithm>
-#include <mutex>
+#include <cfloat>
 
 #include "common.cuh"
 #include "tma.h"
@@ -32,7 +32,7 @@ namespace {
 constexpr int TM = 256, TN = 256, TK = 64, STAGES = 6, THREADS = 384;
 constexpr int kHalf = 128 * TK * 2;  // one CTA's half of an operand tile, bytes
 constexpr int kSmem = STAGES * 2 * kHalf + 256 + 1024;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 enum Epilogue { kStats = 0, kDlogits = 1, kOut = 2 };
 
@@ -44,11 +44,12 @@ struct Args {
   // kStats, kDlogits: rows are tokens, columns vocabulary entries from col0 on
   const int64_t* target;
   int64_t col0, ignore, vocab;
-  float2* part;   // kStats: (max, sum) per [2 x n tile][m]
+  float2* part;   // kStats: (base, sum) per [2 x n tile][m]
   float* tlogit;  // kStats: the target's logit
   const float* lse;
   const float* dloss;
   int64_t dloss_stride;
+  const float* unit;   // kDlogits: divides dloss; kOut: multiplies the result (null: 1)
   __nv_bfloat16* out;  // kDlogits: G; kOut: the result, or null when it goes to f32
   int64_t ldo;
   float* acc;  // kOut: f32 [splits][m][n]
@@ -77,20 +78,21 @@ __device__ __forceinline__ void tile_at(const Args& p, int tm, int tn, int64_t t
   n0 = (int64_t)((grp & 1) ? tn - 1 - nt : nt) * TN;
 }
 
-// One row's 32 logits of a chunk folded into its running maximum and sum (base 2 exponentials).
-__device__ __forceinline__ void fold(const float (&v)[32], float& m, float& s) {
+// One row's 32 logits of a chunk folded into its running maximum and its sum of 2^(logit log2e - base).  The maximum
+// is kept as the rounded base itself, so its rounding cancels in lse = (base + log2 sum) ln 2.
+__device__ __forceinline__ void fold(const float (&v)[32], float& base, float& s) {
   float c = v[0];
 #pragma unroll
   for (int i = 1; i < 31; i += 2) c = max3(c, v[i], v[i + 1]);
   c = fmaxf(c, v[31]);
-  const float mn = fmaxf(m, c);
-  const float base = mn == -INFINITY ? 0.f : mn * kLog2e;  // nothing but masked columns so far: every term is 0
-  s *= m == -INFINITY ? 0.f : ex2(fmaf(m, kLog2e, -base));
+  const float top = fmaxf(base, c * kLog2e);
+  const float b = top == -INFINITY ? 0.f : top;  // nothing but masked columns so far: every term is 0
+  s *= ex2(base - b);
   float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 32; ++i) a[i & 3] += ex2(fmaf(v[i], kLog2e, -base));
+  for (int i = 0; i < 32; ++i) a[i & 3] += ex2(fmaf(v[i], kLog2e, -b));
   s += (a[0] + a[1]) + (a[2] + a[3]);
-  m = mn;
+  base = top;
 }
 
 template <bool A_MN, bool B_MN, int EPI>
@@ -215,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           skip = tgt == p.ignore;
           if constexpr (EPI == kDlogits) {
             nlse = -p.lse[gm] * kLog2e;
-            up = p.dloss[gm * p.dloss_stride];
+            up = p.dloss[gm * p.dloss_stride] / *p.unit;
             if (!skip && (tgt < 0 || tgt >= p.vocab)) up = NAN;  // no such entry: the gradient says so
           }
           tgt -= p.col0;
@@ -224,6 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (!mbar_wait_cluster(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
       tc_fence_after();
       float mx = -INFINITY, sum = 0.f;
+      const float unit = EPI == kOut && p.unit ? *p.unit : 1.f;
 #pragma unroll 1
       for (int ch = half * (TN / 64); ch < (half + 1) * (TN / 64); ++ch) {
         uint32_t r[32];
@@ -280,6 +283,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               continue;
             }
             C = p.out + gm * p.ldo + c0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= unit;
           }
           uint32_t pk[16];
 #pragma unroll
@@ -308,7 +313,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-// Joins a row's (max, sum) pairs: one warp per row.
+// Joins a row's (base, sum) pairs: one warp per row.
 constexpr int kFinishWarps = 4;
 
 __global__ void __launch_bounds__(32 * kFinishWarps)
@@ -321,27 +326,52 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
   for (int i = lane; i < parts; i += 32) {
     const float2 q = part[(int64_t)i * tokens + row];
     const float mn = fmaxf(m, q.x);
-    if (mn != -INFINITY) s = s * expf(m - mn) + q.y * expf(q.x - mn);
+    if (mn != -INFINITY) s = s * exp2f(m - mn) + q.y * exp2f(q.x - mn);
     m = mn;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float mo = __shfl_xor_sync(0xffffffffu, m, o), so = __shfl_xor_sync(0xffffffffu, s, o);
     const float mn = fmaxf(m, mo);
-    if (mn != -INFINITY) s = s * expf(m - mn) + so * expf(mo - mn);
+    if (mn != -INFINITY) s = s * exp2f(m - mn) + so * exp2f(mo - mn);
     m = mn;
   }
   if (lane == 0) {
-    const float l = m + logf(s);
+    const float l = (m + log2f(s)) * kLn2;
     const int64_t t = target[row];
     if (lse) lse[row] = l;
     if (loss) loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? NAN : l - tlogit[row];
   }
 }
 
+// The unit that dloss is measured in: its largest finite magnitude over the tokens that count (1 if that is 0).  G
+// is rounded to bf16 in this unit.  In dloss's own units the entries of all targets, -(1 - p) dloss with p near 0,
+// would under a mean be one and the same number, whose rounding (up to 2^-9) would not average out but scale the
+// whole gradient; in this unit it is 1, which is exact.
+__global__ void __launch_bounds__(1024)
+    linear_ce_unit_kernel(const float* dloss, int64_t stride, const int64_t* target, int64_t ignore, int64_t tokens, float* unit) {
+  __shared__ float red[32];
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
+    const float a = fabsf(dloss[i * stride]);
+    if (target[i] != ignore && a <= FLT_MAX) m = fmaxf(m, a);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    m = red[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (threadIdx.x == 0) *unit = m > 0.f ? m : 1.f;
+  }
+}
+
 // The f32 shares of a product, added in order and rounded.
 __global__ void __launch_bounds__(256)
-    linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, __nv_bfloat16* out, int64_t ldo) {
+    linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, __nv_bfloat16* out,
+                          int64_t ldo) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // n is a multiple of 8
   if (i >= m * n) return;
   float4 s = *reinterpret_cast<const float4*>(acc + i);
@@ -349,7 +379,8 @@ __global__ void __launch_bounds__(256)
     const float4 q = *reinterpret_cast<const float4*>(acc + (int64_t)k * m * n + i);
     s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
   }
-  uint2 o = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+  const float u = *unit;
+  uint2 o = make_uint2(pack_bf16(s.x * u, s.y * u), pack_bf16(s.z * u, s.w * u));
   *reinterpret_cast<uint2*>(out + (i / n) * ldo + i % n) = o;
 }
 
@@ -432,7 +463,7 @@ void split_k(Args& p, int pairs, int64_t k) {
 struct BwdPlan {
   int64_t piece, pieces;  // vocabulary entries per piece
   int dx_splits, dw_splits;
-  int64_t g, dx_acc, dw_acc, bytes;
+  int64_t g, unit, dx_acc, dw_acc, bytes;
 };
 // G of one piece: at most this many bytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
@@ -451,6 +482,8 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width, int pairs) {
   split_k(a, pairs, tokens);
   b.dw_splits = a.splits;
   int64_t at = up256(tokens * b.piece * 2);
+  b.unit = at;
+  at += kAlign;
   b.dx_acc = at;
   if (b.dx_splits > 1 || b.pieces > 1) at += up256(b.dx_splits * tokens * width * 4);
   b.dw_acc = at;
@@ -459,8 +492,8 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width, int pairs) {
   return b;
 }
 
-void join(const float* acc, int splits, int64_t m, int64_t n, void* out, int64_t ldo, cudaStream_t s) {
-  linear_ce_join_kernel<<<(unsigned)div_up(m * n, 1024), 256, 0, s>>>(acc, splits, m, n,
+void join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, void* out, int64_t ldo, cudaStream_t s) {
+  linear_ce_join_kernel<<<(unsigned)div_up(m * n, 1024), 256, 0, s>>>(acc, splits, m, n, unit,
                                                                        static_cast<__nv_bfloat16*>(out), ldo);
 }
 
@@ -532,6 +565,9 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
   uint8_t* ws = static_cast<uint8_t*>(d->workspace);
   float* dx_acc = reinterpret_cast<float*>(ws + b.dx_acc);
   float* dw_acc = reinterpret_cast<float*>(ws + b.dw_acc);
+  float* unit = reinterpret_cast<float*>(ws + b.unit);
+  linear_ce_unit_kernel<<<1, 1024, 0, s>>>(d->dloss, d->dloss_stride, d->target, d->ignore_index, d->tokens, unit);
+  if (int st = cuda_status(cudaGetLastError(), "linear cross entropy unit launch")) return st;
   const Matrix x{d->x, d->tokens, d->width, d->x_stride};
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, d->vocab - v0);
@@ -551,6 +587,7 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
     p.lse = d->lse;
     p.dloss = d->dloss;
     p.dloss_stride = d->dloss_stride;
+    p.unit = unit;
     p.out = reinterpret_cast<__nv_bfloat16*>(ws);
     p.ldo = b.piece;
     if (int st = gemm<false, false, kDlogits>(x, w, p, s)) return st;
@@ -564,9 +601,10 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
       q.splits = (int)div_up(div_up(q.k, TK), q.kb_split);
       q.out = static_cast<__nv_bfloat16*>(d->dw) + v0 * d->dw_stride;
       q.ldo = d->dw_stride;
+      q.unit = unit;
       if (q.splits > 1) q.acc = dw_acc;
       if (int st = gemm<true, true, kOut>(g, x, q, s)) return st;
-      if (q.acc) join(q.acc, q.splits, q.m, q.n, q.out, q.ldo, s);
+      if (q.acc) join(q.acc, q.splits, q.m, q.n, unit, q.out, q.ldo, s);
     }
     if (d->dx) {
       Args q{};
@@ -580,11 +618,12 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
       q.splits = (int)div_up(nk, q.kb_split);
       q.out = static_cast<__nv_bfloat16*>(d->dx);
       q.ldo = d->dx_stride;
+      q.unit = unit;
       if (b.dx_splits > 1 || b.pieces > 1) q.acc = dx_acc;
       q.add = i > 0;
       if (int st = gemm<false, true, kOut>(g, w, q, s)) return st;
     }
   }
-  if (d->dx && (b.dx_splits > 1 || b.pieces > 1)) join(dx_acc, b.dx_splits, d->tokens, d->width, d->dx, d->dx_stride, s);
+  if (d->dx && (b.dx_splits > 1 || b.pieces > 1)) join(dx_acc, b.dx_splits, d->tokens, d->width, unit, d->dx, d->dx_stride, s);
   return cuda_status(cudaGetLastError(), "linear cross entropy join launch");
 }

@@ -40,22 +40,28 @@ def _rows2d(x: torch.Tensor) -> torch.Tensor:
     return x2
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on_device_of(t: torch.Tensor):
     """The library launches on the current device: make it the tensor's where it is another."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-def _param_dtype(what: str, x: torch.Tensor, cols: int, **vectors) -> torch.dtype:
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current torch stream of the tensor's device, without a stream object in between."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _param_dtype(what: str, x: torch.Tensor, cols: int, gamma, beta) -> torch.dtype:
     """The one dtype of the given per-column vectors (float32, or x's)."""
     ptype = None
-    for nm, t in vectors.items():
+    for nm, t in (("gamma", gamma), ("beta", beta)):
         if t is None:
             continue
-        if t.dtype not in (torch.float32, x.dtype) or t.numel() != cols or t.device != x.device:
+        if (t.dtype != torch.float32 and t.dtype != x.dtype) or t.numel() != cols or t.device != x.device:
             raise ValueError(f"{what}: {nm} must be a CUDA f32 vector of length {cols} (or of x's dtype)")
-        if ptype not in (None, t.dtype):
+        if ptype is not None and ptype != t.dtype:
             raise ValueError(f"{what}: gamma and beta must share one dtype")
         ptype = t.dtype
     return ptype or torch.float32
@@ -99,32 +105,31 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Te
     if x.dtype not in _DTYPES:
         raise TypeError("layernorm: float32 or bfloat16")
     x2 = _rows2d(x)
-    C_ = x2.shape[1]
-    ptype = _param_dtype("layernorm", x, C_, gamma=gamma, beta=beta)
+    R, C_ = x2.shape
+    ptype = _param_dtype("layernorm", x, C_, gamma, beta)
     g = gamma.contiguous() if gamma is not None else None
     b = beta.contiguous() if beta is not None else None
-    y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
+    at_g, at_b = g.data_ptr() if g is not None else None, b.data_ptr() if b is not None else None
     if x.dtype == torch.float32 and ptype == torch.float32 and not return_stats:
-        d = LayerNormDesc(x2.data_ptr(), g.data_ptr() if g is not None else None,
-                          b.data_ptr() if b is not None else None, y.data_ptr(), x2.shape[0], C_,
-                          x2.stride(0) if x2.shape[0] else C_, y.stride(0) if y.shape[0] else C_, float(eps))
+        y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
+        d = LayerNormDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), R, C_, x2.stride(0) if R else C_,
+                          y.stride(0) if R else C_, float(eps))
         with _on_device_of(x):
             check(load().pdb_layernorm_f32(C.byref(d), _stream(x)), "pdb_layernorm_f32")
         return y.view(x.shape)
     x2 = _own_rows(x2)
-    R = x2.shape[0]
-    stats = torch.empty((2, R), dtype=torch.float32, device=x.device) if return_stats else None
-    at = stats.data_ptr() if return_stats else None
-    d = _lib.LayerNormFwdDesc(x2.data_ptr(), g.data_ptr() if g is not None else None,
-                              b.data_ptr() if b is not None else None, y.data_ptr(), at,
-                              at + 4 * R if return_stats else None, R, C_, x2.stride(0), y.stride(0), float(eps),
-                              _DTYPES[x.dtype], _DTYPES[ptype])
-    with _on_device_of(x):
-        check(load().pdb_layernorm_fwd(C.byref(d), _stream(x)), "pdb_layernorm_fwd")
+    y = torch.empty((R, C_), dtype=x.dtype, device=x.device) if out is None else _out_rows("layernorm", out, x2)
+    mean = rstd = at_m = at_r = None
     if return_stats:
-        lead = x.shape[:-1]
-        return y.view(x.shape), stats[0].view(lead), stats[1].view(lead)
-    return y.view(x.shape)
+        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
+        at_m, at_r = mean.data_ptr(), rstd.data_ptr()
+    d = _lib.LayerNormFwdDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), at_m, at_r, R, C_, x2.stride(0), y.stride(0),
+                              eps, _DTYPES[x.dtype], _DTYPES[ptype])
+    with _on_device_of(x):
+        check(load().pdb_layernorm_fwd(C.byref(d), _raw_stream(x)), "pdb_layernorm_fwd")
+    if y.shape != x.shape:
+        y = y.view(x.shape)
+    return (y, mean, rstd) if return_stats else y
 
 
 def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -145,25 +150,24 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
             raise ValueError(f"layernorm_backward: {nm} must be the forward's float32 statistic of {R} rows")
     if dout.device != x.device:
         raise ValueError("layernorm_backward: tensors on different devices")
-    ptype = _param_dtype("layernorm_backward", x, C_, gamma=gamma)
+    ptype = _param_dtype("layernorm_backward", x, C_, gamma, None)
     g = gamma.contiguous() if gamma is not None else None
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = torch.empty((R, C_), dtype=x.dtype, device=x.device)
-    dw = torch.empty((2, C_), dtype=ptype, device=x.device) if weight_grads else None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dgamma = dbeta = None
     d = _lib.LayerNormBwdDesc(do2.data_ptr(), x2.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                               g.data_ptr() if g is not None else None, dx.data_ptr(), None, None, None, 0, R, C_,
                               do2.stride(0), x2.stride(0), C_, _DTYPES[x.dtype], _DTYPES[ptype])
     lib = load()
     with _on_device_of(x):
         if weight_grads:
-            d.dgamma = dw.data_ptr()
-            d.dbeta = d.dgamma + dw.element_size() * C_ if C_ else d.dgamma
+            dgamma, dbeta = torch.empty((2, C_), dtype=ptype, device=x.device).unbind(0)
+            d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
             nbytes = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
-            ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=x.device)
+            ws = torch.empty(nbytes + 16, dtype=torch.uint8, device=x.device)
             d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
-        check(lib.pdb_layernorm_bwd(C.byref(d), _stream(x)), "pdb_layernorm_bwd")
-    dx = dx.view(x.shape)
-    return (dx, dw[0], dw[1]) if weight_grads else (dx, None, None)
+        check(lib.pdb_layernorm_bwd(C.byref(d), _raw_stream(x)), "pdb_layernorm_bwd")
+    return dx, dgamma, dbeta
 
 
 def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -294,36 +298,40 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
     if k is not None and (xs[1].shape[0] != B or xs[1].shape[2:] != (T, D) or k.device != q.device):
         raise ValueError(f"rotary: incompatible q {tuple(q.shape)} and k {tuple(k.shape)}")
     freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
-    if freq.ndim != 1 or len(freq) > _lib.ROTARY_MAX_PAIRS or 2 * len(freq) > D:
+    n = len(freq) if freq.ndim == 1 else -1
+    if n < 0 or n > _lib.ROTARY_MAX_PAIRS or 2 * n > D:
         raise ValueError(f"rotary: inv_freq must be a vector of at most {_lib.ROTARY_MAX_PAIRS} pairs within the head's {D} features")
     if out is None:
         ys = [torch.empty_like(t) for t in xs]
     else:
         outs = (out,) if k is None else tuple(out)
-        if len(outs) != len(ts) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device
-                                       or any(n > 1 and (st == 0 or (i == o.dim() - 1 and st != 1))
-                                              for i, (n, st) in enumerate(zip(o.shape, o.stride())))
-                                       for o, t in zip(outs, ts)):
-            raise ValueError("rotary: out must match the inputs, with unit stride along the features and no broadcast dim")
+        if len(outs) != len(ts):
+            raise ValueError("rotary: out must be one tensor for each input")
+        for o, t in zip(outs, ts):
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+                raise ValueError("rotary: out must have the inputs' shape, dtype and device")
+            if (o.shape[-1] > 1 and o.stride(-1) != 1) or any(m > 1 and st == 0 for m, st in zip(o.shape, o.stride())):
+                raise ValueError("rotary: out must have unit stride along the features and no broadcast dim")
         ys = [_as4d(o, "out") for o in outs]
     d = _lib.RotaryDesc()
     for i, (x, y) in enumerate(zip(xs, ys)):
         d.x[i], d.y[i], d.heads[i] = x.data_ptr(), y.data_ptr(), x.shape[1]
-        d.x_stride[i], d.y_stride[i] = _s3(x), _s3(y)
+        d.x_stride[i][:], d.y_stride[i][:] = x.stride()[:3], y.stride()[:3]
     if positions is not None:
         if positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
             raise TypeError("rotary: positions must be an integer tensor on q's device")
         if positions.dim() not in (1, 2):
             raise ValueError("rotary: positions must be (T,) or (B, T)")
         p = positions.to(torch.int64).expand(B, T)
-        d.positions, d.pos_stride[0], d.pos_stride[1] = p.data_ptr(), p.stride(0), p.stride(1)
-    d.start, d.batch, d.seqlen, d.head_dim, d.rotary_dim = int(start), B, T, D, 2 * len(freq)
-    d.amplitude, d.interleaved, d.inverse, d.dtype = float(amplitude), int(bool(interleaved)), int(bool(inverse)), _DTYPES[q.dtype]
+        d.positions = p.data_ptr()
+        d.pos_stride[:] = p.stride()
+    d.start, d.batch, d.seqlen, d.head_dim, d.rotary_dim = start, B, T, D, 2 * n
+    d.amplitude, d.interleaved, d.inverse, d.dtype = amplitude, bool(interleaved), bool(inverse), _DTYPES[q.dtype]
     C.memmove(d.inv_freq, freq.ctypes.data, freq.nbytes)
     with _on_device_of(q):
-        check(load().pdb_rotary(C.byref(d), _stream(q)), "pdb_rotary")
-    rets = [y.view(t.shape) for y, t in zip(ys, ts)] if out is None else list(outs)
-    return rets[0] if k is None else tuple(rets)
+        check(load().pdb_rotary(C.byref(d), _raw_stream(q)), "pdb_rotary")
+    rets = tuple(y if y.shape == t.shape else y.view(t.shape) for y, t in zip(ys, ts)) if out is None else outs
+    return rets[0] if k is None else rets
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -475,7 +483,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     with _on_device_of(x):
         ws = torch.empty(lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
-        check(lib.pdb_linear_ce_fwd(C.byref(d), _stream(x)), "pdb_linear_ce_fwd")
+        check(lib.pdb_linear_ce_fwd(C.byref(d), _raw_stream(x)), "pdb_linear_ce_fwd")
     lead = x.shape[:-1]
     return (out[0].view(lead), out[1].view(lead)) if return_lse else out[0].view(lead)
 
@@ -512,5 +520,5 @@ def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target:
     with _on_device_of(x):
         ws = torch.empty(lib.pdb_linear_ce_bwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
-        check(lib.pdb_linear_ce_bwd(C.byref(d), _stream(x)), "pdb_linear_ce_bwd")
+        check(lib.pdb_linear_ce_bwd(C.byref(d), _raw_stream(x)), "pdb_linear_ce_bwd")
     return dx.view(x.shape) if need_dx else None, dw

@@ -142,6 +142,52 @@ def case_score_program(T=2048, E=64):
     return (lambda: run.run_t(*ins)), {"source": run.source}
 
 
+def case_norm(direction, dtype, rows=8192, cols=4096):
+    """Layer norm for training: the forward with statistics, or the gradients."""
+    import torch
+
+    from . import kernels
+
+    t = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, dy = (torch.randn((rows, cols), device="cuda", generator=g).to(t) for _ in range(2))
+    gam = 1 + 0.1 * torch.randn(cols, device="cuda", generator=g)
+    bet = 0.1 * torch.randn(cols, device="cuda", generator=g)
+    if direction == "fwd":
+        return (lambda: kernels.layernorm(x, gam, bet, return_stats=True)), {"bytes": 2 * x.numel() * x.element_size()}
+    _, mean, rstd = kernels.layernorm(x, gam, bet, return_stats=True)
+    return (lambda: kernels.layernorm_backward(dy, x, mean, rstd, gam)), {"bytes": 3 * x.numel() * x.element_size()}
+
+
+def case_rotary(B=8, H=32, HK=8, T=4096, D=128):
+    import torch
+
+    from . import kernels
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn((B, H, T, D), device="cuda", generator=g).to(torch.bfloat16)
+    k = torch.randn((B, HK, T, D), device="cuda", generator=g).to(torch.bfloat16)
+    f, _ = kernels.rotary_frequencies(D)
+    out = (torch.empty_like(q), torch.empty_like(k))
+    return (lambda: kernels.rotary(q, k, inv_freq=f, out=out)), {"bytes": 4 * (q.numel() + k.numel())}
+
+
+def case_linear_ce(direction, N=4096, V=65536, D=2048):
+    import torch
+
+    from . import kernels
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn((N, D), device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn((V, D), device="cuda", generator=g) / D ** 0.5).to(torch.bfloat16)
+    t = torch.randint(0, V, (N,), device="cuda", generator=g)
+    if direction == "fwd":
+        return (lambda: kernels.linear_cross_entropy(x, w, t, return_lse=True)), {"TFLOP": 2.0 * N * V * D / 1e12}
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dl = torch.full((N,), 1.0 / N, device="cuda")
+    return (lambda: kernels.linear_cross_entropy_backward(x, w, t, dl, lse)), {"TFLOP": 6.0 * N * V * D / 1e12}
+
+
 CASES = {
     "fwd_config3": lambda: case_fwd(8, 32, 4096, 128),
     "fwd_b2": lambda: case_fwd(2, 32, 4096, 128),
@@ -156,6 +202,13 @@ CASES = {
     "score_program": case_score_program,
     "rowsoftmax_config2": lambda: case_rows("softmax"),
     "layernorm_config2": lambda: case_rows("layernorm"),
+    "norm_fwd_bf16": lambda: case_norm("fwd", "bfloat16"),
+    "norm_bwd_bf16": lambda: case_norm("bwd", "bfloat16"),
+    "norm_bwd_f32": lambda: case_norm("bwd", "float32"),
+    "norm_bwd_heads": lambda: case_norm("bwd", "bfloat16", 262144, 128),
+    "rotary_qk": case_rotary,
+    "linear_ce_fwd": lambda: case_linear_ce("fwd"),
+    "linear_ce_bwd": lambda: case_linear_ce("bwd"),
 }
 
 

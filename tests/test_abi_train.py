@@ -58,6 +58,15 @@ def test_layernorm_refusals():
     d = _norm()
     d.x = None
     assert lib.pdb_layernorm_fwd(C.byref(d), None) == _lib.PDB_ERR_ARG
+    for field in ("x", "y", "gamma", "beta"):
+        d = _norm(dtype=_lib.PDB_BF16, param=_lib.PDB_BF16)
+        setattr(d, field, 17)
+        assert lib.pdb_layernorm_fwd(C.byref(d), None) == _lib.PDB_ERR_ALIGN
+    for field in ("x", "dout", "dx", "gamma", "dgamma", "dbeta", "workspace"):
+        d = _norm_bwd()
+        d.workspace, d.workspace_bytes = 16, 1 << 20
+        setattr(d, field, 17)
+        assert lib.pdb_layernorm_bwd(C.byref(d), None) == _lib.PDB_ERR_ALIGN
     d = _norm(cols=0)
     assert lib.pdb_layernorm_fwd(C.byref(d), None) == _lib.PDB_OK
     d.mean = 16
@@ -67,7 +76,7 @@ def test_layernorm_refusals():
     assert lib.pdb_layernorm_bwd(C.byref(d), None) == _lib.PDB_ERR_ARG
     d = _norm_bwd()
     need = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
-    assert need == 2 * 2 * 8 * 4  # two rows: two partial rows of each gradient
+    assert need == 2 * 10 * 8 * 4  # two rows: at most ten partial rows of each gradient
     d.workspace, d.workspace_bytes = 16, need - 1
     assert lib.pdb_layernorm_bwd(C.byref(d), None) == _lib.PDB_ERR_ARG
     assert b"workspace too small" in lib.pdb_last_error_string()

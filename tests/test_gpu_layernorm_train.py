@@ -95,7 +95,7 @@ def _check_backward(x, dy, mean, rstd, gam, dx, dg, db):
 
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (1, 4096), (300, 64), (1000, 128), (37, 1001), (257, 520), (301, 2048), (70, 4096),
-          (9, 5000), (700, 8192), (5, 8200), (3, 16384), (4, 32768), (2, 40003)]
+          (9, 5000), (64, 1002), (200, 515), (20, 4099), (90, 16), (13, 8191), (700, 8192), (5, 8200), (3, 16384), (4, 32768), (2, 40003)]
 
 
 @pytest.mark.parametrize("R,C", SHAPES)
@@ -130,6 +130,22 @@ def test_without_weights_strided_and_shaped(cuda, t):
         _check_backward(xs, ds, mean, rstd, None, dx, dg, db)
         dx2, dg2, db2 = kernels.layernorm_backward(ds, xs, mean, rstd, weight_grads=False)
         assert dg2 is None and db2 is None and torch.equal(dx, dx2)
+    for xo, do in ((3, 0), (0, 5), (3, 11)):  # rows that lie differently against 16 bytes; the last pair alike
+        xs, ds = x[:, xo:xo + 999], dy[:, do:do + 999]
+        y, mean, rstd = kernels.layernorm(xs, None, None, return_stats=True)
+        _check_forward(xs, None, None, 1e-5, y, mean, rstd)
+        dx, dg, db = kernels.layernorm_backward(ds, xs, mean, rstd)
+        _check_backward(xs, ds, mean, rstd, None, dx, dg, db)
+    for C in (700, 3001, 6000):  # y on other boundaries than x; longer rows, element by element
+        wide, _, g2, b2 = _inputs(cuda, 11, C + 9, T, torch.float32, C)
+        buf = torch.full((11, C + 9), 5.0, device=cuda, dtype=T)
+        out = kernels.layernorm(wide[:, 1:C + 1], g2[:C], b2[:C], out=buf[:, 2:C + 2])
+        _, mean, rstd = kernels.layernorm(wide[:, 1:C + 1], g2[:C], b2[:C], return_stats=True)
+        _check_forward(wide[:, 1:C + 1], g2[:C], b2[:C], 1e-5, out, mean, rstd)
+        assert (buf[:, :2] == 5).all() and (buf[:, C + 2:] == 5).all()
+        xs, ds = wide[:, 1:C + 1], wide[:, 4:C + 4]
+        dx, dg, db = kernels.layernorm_backward(ds, xs, mean, rstd, g2[:C])
+        _check_backward(xs, ds, mean, rstd, g2[:C], dx, dg, db)
     x3, d3 = x.view(3, 20, 1040), dy[:20].expand(3, 20, 1040)
     y, mean, rstd = kernels.layernorm(x3, None, bet, return_stats=True)
     assert y.shape == x3.shape and mean.shape == (3, 20)

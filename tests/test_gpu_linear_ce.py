@@ -253,3 +253,25 @@ def test_gradient_against_differences(cuda):
     G = p * (dl.double().abs() * valid)[:, None]
     size = ((G @ w.double().abs()) * a.double().abs()).sum() + ((G.T @ x.double().abs()) * b.double().abs()).sum()
     assert abs(got - slope) <= (2.0 ** -7 * 1.1 + 100 * h * h) * size
+
+
+@pytest.mark.parametrize("n", [1, 3, 7373])
+def test_a_mean_does_not_scale_the_gradient(cuda, n):
+    """Under a mean, all targets' entries of G are almost the same number; its rounding must not scale the gradient.
+    The regression of dx on its exact value is 1 up to 4 sigma of dx's own rounding, 2^-8 / sqrt(elements) at most,
+    and 1 / vocab from a target's 1 - p, with p near 1 / vocab in every row, rounded to 1."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    g = torch.Generator(device="cpu").manual_seed(11)
+    x = (torch.randn(512, 64, generator=g) * 1e-3).to(torch.bfloat16).to(cuda)
+    w = torch.randn(20000, 64, generator=g).to(torch.bfloat16).to(cuda)
+    t = torch.randint(0, 20000, (512,), generator=g).to(cuda)
+    dl = torch.full((512,), 1.0 / n, device=cuda)
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dx, _ = kernels.linear_cross_entropy_backward(x, w, t, dl, lse, need_dweight=False)
+    p = torch.exp(x.double() @ w.double().T - lse.double()[:, None])
+    ref = (p @ w.double() - w[t].double()) / n
+    slope = (dx.double() * ref).sum() / (ref * ref).sum()
+    assert abs(slope - 1) <= 4 * 2.0 ** -8 / (512 * 64) ** 0.5 + 1 / 20000

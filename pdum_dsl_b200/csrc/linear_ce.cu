@@ -14,14 +14,17 @@
 // the pieces in f32.
 //
 // All of it is bound by the tensor cores: 2 (forward) and 6 (backward) x tokens x
-// vocab x width operations.  One persistent kernel serves the four products: CTA
-// pairs (cta_group::2) on 256 x 256 tiles, operands by TMA into a six-stage ring,
-// two f32 accumulators in TMEM so that a tile's epilogue runs under the next
-// tile's products.  An operand is read K-major (its rows are the tile's rows) or
-// MN-major (its rows are the contracted index): G^T, x and w enter dw and dx that
-// way, as they lie in memory.
+// vocab x width operations.  One persistent kernel serves the four products: tiles of
+// 256 rows on CTA pairs (cta_group::2), or of 128 rows on single CTAs where there are
+// at most that many rows, by up to 256 columns; operands by TMA into a ring, two f32
+// accumulators in TMEM so that a tile's epilogue runs under the next tile's products.
+// An operand is read K-major (its rows are the tile's rows) or MN-major (its rows are
+// the contracted index): G^T, x and w enter dw and dx that way, as they lie in memory.
+// Sixteen warps run the epilogue, 64 columns of 32 rows each, and hand results to TMA
+// stores through shared memory.
 #include <algorithm>
 #include <cfloat>
+#include <utility>
 
 #include "common.cuh"
 #include "tma.h"
@@ -29,42 +32,54 @@
 namespace pdb {
 namespace {
 
-constexpr int TM = 256, TN = 256, TK = 64, STAGES = 6, THREADS = 384;
-constexpr int kHalf = 128 * TK * 2;  // one CTA's half of an operand tile, bytes
-constexpr int kSmem = STAGES * 2 * kHalf + 256 + 1024;
+constexpr int TK = 64, kEpiWarps = 16, THREADS = 128 + 32 * kEpiWarps;
+constexpr int kBox = 64 * 64 * 2;      // an MN-major box: 64 tile rows x 64 contracted rows
+constexpr int kTileA = 128 * TK * 2;   // a CTA's rows of A per stage
+constexpr int kStore = 4096;           // an epilogue warp's staging: 32 rows x 64 bf16 or 32 f32, 128-byte swizzle
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-enum Epilogue { kStats = 0, kDlogits = 1, kOut = 2 };
+enum Epilogue { kStats = 0, kDlogits = 1, kOut = 2, kSum = 3 };  // kOut: bf16, kSum: f32
+
+// CG: CTAs per tile.  Each holds 128 rows of A; B's rows are split between the CTAs of a pair.
+template <int CG, int EPI>
+struct Layout {
+  static constexpr int kTileB = 256 / CG * TK * 2;
+  static constexpr int kStage = kTileA + kTileB;
+  static constexpr int kStaging = EPI == kStats ? 0 : kEpiWarps * kStore;
+  static constexpr int kStages = (227 * 1024 - 1024 - 256 - kStaging) / kStage;
+  static constexpr int kSmem = kStages * kStage + kStaging + 256 + 1024;
+};
 
 struct Args {
   int64_t m, n, k;
+  int tile_n;            // columns per tile, a multiple of 64 (of 32 for kStats), at most 256
   int splits, kb_split;  // shares of the contracted index, and 64-wide blocks in each
   int group;             // m tiles that share a sweep over the n tiles
   int* err;
   // kStats, kDlogits: rows are tokens, columns vocabulary entries from col0 on
   const int64_t* target;
   int64_t col0, ignore, vocab;
-  float2* part;   // kStats: (base, sum) per [2 x n tile][m]
+  float2* part;   // kStats: (base, sum) per [4 x n tile][m]
   float* tlogit;  // kStats: the target's logit
   const float* lse;
   const float* dloss;
   int64_t dloss_stride;
-  const float* unit;   // kDlogits: divides dloss; kOut: multiplies the result (null: 1)
-  __nv_bfloat16* out;  // kDlogits: G; kOut: the result, or null when it goes to f32
-  int64_t ldo;
-  float* acc;  // kOut: f32 [splits][m][n]
-  int add;     // kOut: add to acc
+  float* unit;  // kDlogits: written, the unit that G is measured in; kOut: multiplies the result
+  int add;      // kSum: add to what is there
 };
 
 struct __align__(8) Bars {
-  uint64_t full[STAGES], empty[STAGES];
+  uint64_t full[8], empty[8];
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort;
+  float unit[kEpiWarps];
 };
+static_assert(sizeof(Bars) <= 256, "the barriers' share of shared memory");
 
 // Tile t -> (split, m0, n0): groups of `group` m tiles sweep the n tiles, odd groups backwards, so the tiles
 // in flight share operands in L2.
+template <int TM>
 __device__ __forceinline__ void tile_at(const Args& p, int tm, int tn, int64_t t, int& split, int64_t& m0, int64_t& n0) {
   const int64_t per = (int64_t)tm * tn;
   split = (int)(t / per);
@@ -75,7 +90,7 @@ __device__ __forceinline__ void tile_at(const Args& p, int tm, int tn, int64_t t
   const int rows = min(tm - grp * p.group, p.group);
   const int nt = in / rows;
   m0 = (int64_t)(grp * p.group + in % rows) * TM;
-  n0 = (int64_t)((grp & 1) ? tn - 1 - nt : nt) * TN;
+  n0 = (int64_t)((grp & 1) ? tn - 1 - nt : nt) * p.tile_n;
 }
 
 // One row's 32 logits of a chunk folded into its running maximum and its sum of 2^(logit log2e - base).  The maximum
@@ -88,160 +103,229 @@ __device__ __forceinline__ void fold(const float (&v)[32], float& base, float& s
   const float top = fmaxf(base, c * kLog2e);
   const float b = top == -INFINITY ? 0.f : top;  // nothing but masked columns so far: every term is 0
   s *= ex2(base - b);
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint64_t l2 = f2_pack(kLog2e, kLog2e), nb = f2_pack(-b, -b);
+  uint64_t a0 = f2_pack(0.f, 0.f), a1 = a0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) a[i & 3] += ex2(fmaf(v[i], kLog2e, -b));
-  s += (a[0] + a[1]) + (a[2] + a[3]);
+  for (int i = 0; i < 32; i += 4) {
+    float x, y, z, w;
+    f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), l2, nb), x, y);
+    f2_unpack(f2_fma(f2_pack(v[i + 2], v[i + 3]), l2, nb), z, w);
+    a0 = f2_add(a0, f2_pack(ex2(x), ex2(y)));
+    a1 = f2_add(a1, f2_pack(ex2(z), ex2(w)));
+  }
+  float lo, hi;
+  f2_unpack(f2_add(a0, a1), lo, hi);
+  s += lo + hi;
   base = top;
 }
 
-template <bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+// The unit that dloss is measured in: its largest finite magnitude over the tokens that count (1 if that is 0).  G
+// is rounded to bf16 in this unit.  In dloss's own units the entries of all targets, -(1 - p) dloss with p near 0,
+// would under a mean be one and the same number, whose rounding (up to 2^-9) would not average out but scale the
+// whole gradient; in this unit it is 1, which is exact.  Every CTA finds it for itself, while its first tile's
+// products run.
+__device__ __forceinline__ float find_unit(const Args& p, float* red, int warp, int lane) {
+  float m = 0.f;
+  for (int64_t i = warp * 32 + lane; i < p.m; i += 32 * kEpiWarps) {
+    const float a = fabsf(p.dloss[i * p.dloss_stride]);
+    if (p.target[i] != p.ignore && a <= FLT_MAX) m = fmaxf(m, a);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[warp] = m;
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+#pragma unroll
+  for (int i = 0; i < kEpiWarps; ++i) m = fmaxf(m, red[i]);
+  m = m > 0.f ? m : 1.f;
+  if (blockIdx.x == 0 && warp == 0 && lane == 0) *p.unit = m;
+  return m;
+}
+
+template <int CG>
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, abort, err);
+  else return mbar_wait(bar, parity, abort, err);
+}
+
+template <int CG, bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
     linear_ce_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                          const __grid_constant__ Args p) {
+                          const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ Args p) {
+  using L = Layout<CG, EPI>;
+  constexpr int TM = 128 * CG, STAGES = L::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * kHalf;
-  Bars* bar = reinterpret_cast<Bars*>(sB + STAGES * kHalf);
+  uint8_t* sB = sA + STAGES * kTileA;
+  uint8_t* sC = sB + STAGES * L::kTileB;
+  Bars* bar = reinterpret_cast<Bars*>(sC + L::kStaging);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int unit_id = blockIdx.x / CG, units = gridDim.x / CG;
   const int nk = (int)((p.k + TK - 1) / TK);
-  const int tm = (int)((p.m + TM - 1) / TM), tn = (int)((p.n + TN - 1) / TN);
+  const int tm = (int)((p.m + TM - 1) / TM), tn = (int)((p.n + p.tile_n - 1) / p.tile_n);
   const int64_t num_tiles = (int64_t)tm * tn * p.splits;
 
   if (threadIdx.x == 0) {
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+    if constexpr (EPI != kStats) prefetch_tensormap(&tm_c);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->acc_full[i], 1);
-      mbar_init(&bar->acc_empty[i], 16);  // one arrival per epilogue warp of the pair
+      mbar_init(&bar->acc_empty[i], CG * kEpiWarps);
     }
     bar->abort = 0;
     fence_barrier_init();
   }
   if (warp == 2) {
-    tmem_alloc_pair(&bar->tmem_base, 512);
-    tmem_relinquish_pair();
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(&bar->tmem_base, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&bar->tmem_base, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  cluster_sync_all();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
   tc_fence_after();
+  grid_dep_wait();  // the launch before may still be writing what this one reads
   const uint32_t tmem = bar->tmem_base;
   volatile int* abort = &bar->abort;
 
   if (warp == 0 && lane == 0) {
+    const int b_rows = p.tile_n / CG;  // of B per CTA
+    const uint32_t bytes = CG * (kTileA + b_rows * TK * 2);
     uint32_t g = 0;
     bool ok = true;
-    for (int64_t t = pair; ok && t < num_tiles; t += npairs) {
+    for (int64_t t = unit_id; ok && t < num_tiles; t += units) {
       int split;
       int64_t m0, n0;
-      tile_at(p, tm, tn, t, split, m0, n0);
+      tile_at<TM>(p, tm, tn, t, split, m0, n0);
       const int kb0 = split * p.kb_split, kb1 = min(nk, kb0 + p.kb_split);
-      const int ma = (int)m0 + (int)rank * 128, nb = (int)n0 + (int)rank * 128;
+      const int ma = (int)m0 + (int)rank * 128, nb = (int)n0 + (int)rank * b_rows;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
         const int st = g % STAGES;
-        if (!(ok = mbar_wait_cluster(&bar->empty[st], ((g / STAGES) & 1) ^ 1, abort, p.err))) break;
-        if (rank == 0) mbar_expect_tx(&bar->full[st], 4 * kHalf);
-        const uint32_t full0 = mapa_shared(smem_u32(&bar->full[st]), 0);
-        uint8_t *a = sA + st * kHalf, *b = sB + st * kHalf;
-        if constexpr (A_MN) {  // two boxes of 64 tile rows x 64 contracted rows
-          tma_load_4d_pair(a, &tm_a, full0, ma, kb * TK, 0, 0);
-          tma_load_4d_pair(a + kHalf / 2, &tm_a, full0, ma + 64, kb * TK, 0, 0);
+        if (!(ok = wait_bar<CG>(&bar->empty[st], ((g / STAGES) & 1) ^ 1, abort, p.err))) break;
+        if (rank == 0) mbar_expect_tx(&bar->full[st], bytes);
+        const uint32_t full0 = CG == 2 ? mapa_shared(smem_u32(&bar->full[st]), 0) : 0;
+        auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
+          if constexpr (CG == 2) tma_load_4d_pair(dst, map, full0, c0, c1, 0, 0);
+          else tma_load_4d(dst, map, &bar->full[st], c0, c1, 0, 0);
+        };
+        uint8_t *a = sA + st * kTileA, *b = sB + st * L::kTileB;
+        if constexpr (A_MN) {
+          load(a, &tm_a, ma, kb * TK);
+          load(a + kBox, &tm_a, ma + 64, kb * TK);
         } else {
-          tma_load_4d_pair(a, &tm_a, full0, kb * TK, ma, 0, 0);
+          load(a, &tm_a, kb * TK, ma);
         }
         if constexpr (B_MN) {
-          tma_load_4d_pair(b, &tm_b, full0, nb, kb * TK, 0, 0);
-          tma_load_4d_pair(b + kHalf / 2, &tm_b, full0, nb + 64, kb * TK, 0, 0);
+          for (int r = 0; r < b_rows; r += 64) load(b + r / 64 * kBox, &tm_b, nb + r, kb * TK);
         } else {
-          tma_load_4d_pair(b, &tm_b, full0, kb * TK, nb, 0, 0);
+          load(b, &tm_b, kb * TK, nb);
         }
       }
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
-    constexpr uint32_t idesc = idesc_bf16(TM, TN, A_MN, B_MN);
+    const uint32_t idesc = idesc_bf16(TM, 0, A_MN, B_MN) | ((uint32_t)(p.tile_n >> 3) << 17);
     // K-major: a step of 16 is 32 bytes along the swizzled row; MN-major: 16 rows of 128 bytes, the
-    // second 64 columns in the next box
-    constexpr uint32_t a_step = A_MN ? 2048 : 32, a_lbo = A_MN ? kHalf / 2 : 16;
-    constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? kHalf / 2 : 16;
+    // next 64 columns in the next box
+    constexpr uint32_t a_step = A_MN ? 2048 : 32, a_lbo = A_MN ? kBox : 16;
+    constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? kBox : 16;
     uint32_t g = 0, tt = 0;
     bool ok = true;
-    for (int64_t t = pair; ok && t < num_tiles; t += npairs, ++tt) {
+    for (int64_t t = unit_id; ok && t < num_tiles; t += units, ++tt) {
       const int split = (int)(t / ((int64_t)tm * tn));
       const int kb0 = split * p.kb_split, kb1 = min(nk, kb0 + p.kb_split);
       const int buf = tt & 1;
-      if (!(ok = mbar_wait_cluster(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
+      if (!(ok = wait_bar<CG>(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * TN;
+      const uint32_t acc = tmem + buf * 256;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
         const int st = g % STAGES;
-        if (!(ok = mbar_wait_cluster(&bar->full[st], (g / STAGES) & 1, abort, p.err))) break;
+        if (!(ok = wait_bar<CG>(&bar->full[st], (g / STAGES) & 1, abort, p.err))) break;
         tc_fence_after();
-        const uint32_t a0 = smem_u32(sA + st * kHalf), b0 = smem_u32(sB + st * kHalf);
+        const uint32_t a0 = smem_u32(sA + st * kTileA), b0 = smem_u32(sB + st * L::kTileB);
 #pragma unroll
-        for (int kk = 0; kk < TK / 16; ++kk)
-          mma_ss_pair(acc, sdesc_sw128(a0 + kk * a_step, a_lbo, 1024), sdesc_sw128(b0 + kk * b_step, b_lbo, 1024), idesc,
-                      (kb > kb0 || kk > 0) ? 1u : 0u);
-        const uint32_t e = smem_u32(&bar->empty[st]);
-        tc_commit_pair(e);
-        tc_commit_pair(mapa_shared(e, 1));
+        for (int kk = 0; kk < TK / 16; ++kk) {
+          const uint64_t da = sdesc_sw128(a0 + kk * a_step, a_lbo, 1024), db = sdesc_sw128(b0 + kk * b_step, b_lbo, 1024);
+          if constexpr (CG == 2) mma_ss_pair(acc, da, db, idesc, kb > kb0 || kk > 0);
+          else mma_ss(acc, da, db, idesc, kb > kb0 || kk > 0);
+        }
+        if constexpr (CG == 2) {
+          const uint32_t e = smem_u32(&bar->empty[st]);
+          tc_commit_pair(e);
+          tc_commit_pair(mapa_shared(e, 1));
+        } else {
+          tc_commit(&bar->empty[st]);
+        }
       }
       if (ok) {
-        const uint32_t f = smem_u32(&bar->acc_full[buf]);
-        tc_commit_pair(f);
-        tc_commit_pair(mapa_shared(f, 1));
+        if constexpr (CG == 2) {
+          const uint32_t f = smem_u32(&bar->acc_full[buf]);
+          tc_commit_pair(f);
+          tc_commit_pair(mapa_shared(f, 1));
+        } else {
+          tc_commit(&bar->acc_full[buf]);
+        }
       }
     }
   } else if (warp >= 4) {
-    const int q4 = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quarter, column half
-    const int row = (int)rank * 128 + q4 * 32 + lane;
+    const int e = warp - 4, q4 = warp & 3, cg = e >> 2;  // TMEM lane quarter, group of 64 columns
+    const int row0 = (int)rank * 128 + q4 * 32;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    const uint32_t stage = smem_u32(sC + e * kStore), srow = stage + lane * 128;
+    float unit = 1.f;
+    if constexpr (EPI == kDlogits) unit = find_unit(p, bar->unit, e, lane);
+    if constexpr (EPI == kOut) unit = p.unit ? *p.unit : 1.f;
     uint32_t tt = 0;
-    for (int64_t t = pair; t < num_tiles; t += npairs, ++tt) {
+    for (int64_t t = unit_id; t < num_tiles; t += units, ++tt) {
       int split;
       int64_t m0, n0;
-      tile_at(p, tm, tn, t, split, m0, n0);
+      tile_at<TM>(p, tm, tn, t, split, m0, n0);
       const int buf = tt & 1;
-      const int64_t gm = m0 + row;
+      const int64_t gm = m0 + row0 + lane;
       const bool live = gm < p.m;
       int64_t tgt = -1;
       float nlse = 0.f, up = 0.f;
-      bool skip = false;
-      if constexpr (EPI != kOut) {
+      bool skip = true;
+      if constexpr (EPI == kStats || EPI == kDlogits) {
         if (live) {
           tgt = p.target[gm];
           skip = tgt == p.ignore;
           if constexpr (EPI == kDlogits) {
             nlse = -p.lse[gm] * kLog2e;
-            up = p.dloss[gm * p.dloss_stride] / *p.unit;
+            up = p.dloss[gm * p.dloss_stride] / unit;
             if (!skip && (tgt < 0 || tgt >= p.vocab)) up = NAN;  // no such entry: the gradient says so
           }
           tgt -= p.col0;
         }
       }
-      if (!mbar_wait_cluster(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
+      if (!wait_bar<CG>(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
       tc_fence_after();
-      float mx = -INFINITY, sum = 0.f;
-      const float unit = EPI == kOut && p.unit ? *p.unit : 1.f;
+      float base = -INFINITY, sum = 0.f;
 #pragma unroll 1
-      for (int ch = half * (TN / 64); ch < (half + 1) * (TN / 64); ++ch) {
+      for (int ch = 0; ch < 2; ++ch) {
+        const int c = cg * 64 + ch * 32;  // the tile's column
+        const int64_t c0 = n0 + c;
+        if (c >= p.tile_n || c0 >= p.n) break;  // the whole warp
         uint32_t r[32];
-        __syncwarp();  // rows past the end left the last chunk early
-        tmem_ld32(tmem + lane_off + buf * TN + ch * 32, r);
+        __syncwarp();
+        tmem_ld32(tmem + lane_off + buf * 256 + c, r);
         tmem_wait_ld();
-        const int64_t c0 = n0 + ch * 32;
-        if (!live || c0 >= p.n) continue;
-        const int nv = (int)min((int64_t)32, p.n - c0);
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        const int hit = (int)max((int64_t)-1, min((int64_t)32, tgt - c0));
+        const int hit = tgt - c0 >= 0 && tgt - c0 < 32 ? (int)(tgt - c0) : -1;
         if constexpr (EPI == kStats) {
-          if (hit >= 0 && hit < nv) {
+          const int nv = (int)min((int64_t)32, p.n - c0);
+          if (live && hit >= 0 && hit < nv) {
             float x = v[0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) x = i == hit ? v[i] : x;
@@ -251,130 +335,135 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = i < nv ? v[i] : -INFINITY;
           }
-          fold(v, mx, sum);
-        } else {
-          __nv_bfloat16* C = nullptr;
-          if constexpr (EPI == kDlogits) {
-            C = p.out + gm * p.ldo + c0;
+          fold(v, base, sum);
+        } else if constexpr (EPI == kSum) {
+          // 32 columns fill the staging: 128 bytes a row
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float g = (ex2(fmaf(v[i], kLog2e, nlse)) - (i == hit ? 1.f : 0.f)) * up;
-              v[i] = skip ? 0.f : g;
-            }
-          } else {
-            if (p.acc) {
-              float* dst = p.acc + ((int64_t)split * p.m + gm) * p.n + c0;
-              if ((p.n & 3) == 0 && nv == 32) {
-                float4* d4 = reinterpret_cast<float4*>(dst);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  float4 o = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                  if (p.add) {
-                    const float4 q = d4[i];
-                    o.x += q.x, o.y += q.y, o.z += q.z, o.w += q.w;
-                  }
-                  d4[i] = o;
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (i < nv) dst[i] = p.add ? dst[i] + v[i] : v[i];
-              }
-              continue;
-            }
-            C = p.out + gm * p.ldo + c0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= unit;
+          for (int i = 0; i < 8; ++i) sts128(srow + ((i ^ (lane & 7)) << 4), r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && m0 + row0 < p.m) {
+            if (p.add) tma_reduce_add_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
+            else tma_store_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
+            bulk_commit();
           }
+        } else {
+          if constexpr (EPI == kDlogits) {
+            const uint64_t l2 = f2_pack(kLog2e, kLog2e), nl = f2_pack(nlse, nlse);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x, y;
+              f2_unpack(f2_fma(f2_pack(v[i], v[i + 1]), l2, nl), x, y);
+              v[i] = ex2(x);
+              v[i + 1] = ex2(y);
+            }
+            if (hit >= 0) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = i == hit ? v[i] - 1.f : v[i];
+            }
+          }
+          const float scale = EPI == kDlogits ? up : unit;
+          const uint64_t s2 = f2_pack(scale, scale);
           uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-          if (nv == 32 && (p.ldo & 7) == 0) {
-            uint4* dst = reinterpret_cast<uint4*>(C);
+          for (int i = 0; i < 16; ++i) {
+            float x, y;
+            f2_unpack(f2_mul(f2_pack(v[2 * i], v[2 * i + 1]), s2), x, y);
+            pk[i] = pack_bf16(x, y);
+            if constexpr (EPI == kDlogits) pk[i] = skip ? 0u : pk[i];
+          }
+          if (ch == 0) {
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+          }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < nv) C[i] = __ushort_as_bfloat16((unsigned short)(pk[i >> 1] >> (16 * (i & 1))));
+          for (int i = 0; i < 4; ++i)
+            sts128(srow + (((ch * 4 + i) ^ (lane & 7)) << 4), pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+        }
+      }
+      if constexpr (EPI == kOut || EPI == kDlogits) {
+        // the box is cut at the last row and column by its tensor map
+        if (cg * 64 < p.tile_n && n0 + cg * 64 < p.n && m0 + row0 < p.m) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_4d(&tm_c, stage, (int)n0 + cg * 64, (int)m0 + row0, 0, 0);
+            bulk_commit();
           }
         }
       }
       if constexpr (EPI == kStats)
-        if (live) p.part[((n0 / TN) * 2 + half) * p.m + gm] = make_float2(mx, sum);
-      warp_arrive_cluster_after_tc(mapa_shared(smem_u32(&bar->acc_empty[buf]), 0));
+        if (live) p.part[((n0 / p.tile_n) * 4 + cg) * p.m + gm] = make_float2(base, sum);
+      if constexpr (CG == 2) warp_arrive_cluster_after_tc(mapa_shared(smem_u32(&bar->acc_empty[buf]), 0));
+      else warp_arrive_after_tc(&bar->acc_empty[buf]);
     }
+    if (EPI != kStats && lane == 0) bulk_wait_all();
   }
   tc_fence_before();
-  cluster_sync_all();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
-// Joins a row's (base, sum) pairs: one warp per row.
-constexpr int kFinishWarps = 4;
+// Joins the rows' (base, sum) pairs: a block takes 32 rows (a lane each) and its 32 warps a share of the pairs each.
+constexpr int kFinishWarps = 32;
 
 __global__ void __launch_bounds__(32 * kFinishWarps)
     linear_ce_finish_kernel(const float2* part, int parts, const float* tlogit, const int64_t* target, int64_t tokens,
                             int64_t vocab, int64_t ignore, float* loss, float* lse) {
-  const int64_t row = (int64_t)blockIdx.x * kFinishWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= tokens) return;
-  float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < parts; i += 32) {
-    const float2 q = part[(int64_t)i * tokens + row];
-    const float mn = fmaxf(m, q.x);
-    if (mn != -INFINITY) s = s * exp2f(m - mn) + q.y * exp2f(q.x - mn);
-    m = mn;
+  __shared__ float2 red[kFinishWarps][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  auto join = [](float2& a, float2 b) {
+    const float m = fmaxf(a.x, b.x), z = m == -INFINITY ? 0.f : m;
+    a = make_float2(m, a.y * exp2f(a.x - z) + b.y * exp2f(b.x - z));
+  };
+  grid_dep_wait();
+  float2 s = make_float2(-INFINITY, 0.f);
+  if (row < tokens) {
+    int i = warp;
+    for (; i + 3 * kFinishWarps < parts; i += 4 * kFinishWarps) {
+      float2 q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q[u] = part[(int64_t)(i + u * kFinishWarps) * tokens + row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) join(s, q[u]);
+    }
+    for (; i < parts; i += kFinishWarps) join(s, part[(int64_t)i * tokens + row]);
   }
+  red[warp][lane] = s;
+  __syncthreads();
+  // turned: a warp joins one row's 32 shares
+  s = red[lane][warp];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float mo = __shfl_xor_sync(0xffffffffu, m, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-    const float mn = fmaxf(m, mo);
-    if (mn != -INFINITY) s = s * exp2f(m - mn) + so * exp2f(mo - mn);
-    m = mn;
+    const float2 q = make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o));
+    join(s, q);
   }
-  if (lane == 0) {
-    const float l = (m + log2f(s)) * kLn2;
-    const int64_t t = target[row];
-    if (lse) lse[row] = l;
-    if (loss) loss[row] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? NAN : l - tlogit[row];
-  }
-}
-
-// The unit that dloss is measured in: its largest finite magnitude over the tokens that count (1 if that is 0).  G
-// is rounded to bf16 in this unit.  In dloss's own units the entries of all targets, -(1 - p) dloss with p near 0,
-// would under a mean be one and the same number, whose rounding (up to 2^-9) would not average out but scale the
-// whole gradient; in this unit it is 1, which is exact.
-__global__ void __launch_bounds__(1024)
-    linear_ce_unit_kernel(const float* dloss, int64_t stride, const int64_t* target, int64_t ignore, int64_t tokens, float* unit) {
-  __shared__ float red[32];
-  float m = 0.f;
-  for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
-    const float a = fabsf(dloss[i * stride]);
-    if (target[i] != ignore && a <= FLT_MAX) m = fmaxf(m, a);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    m = red[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (threadIdx.x == 0) *unit = m > 0.f ? m : 1.f;
+  const int64_t r = (int64_t)blockIdx.x * 32 + warp;
+  if (lane == 0 && r < tokens) {
+    const float l = (s.x + log2f(s.y)) * kLn2;
+    const int64_t t = target[r];
+    if (lse) lse[r] = l;
+    if (loss) loss[r] = t == ignore ? 0.f : (t < 0 || t >= vocab) ? NAN : l - tlogit[r];
   }
 }
 
-// The f32 shares of a product, added in order and rounded.
+// The f32 shares of a product, added in order, scaled and rounded.
 __global__ void __launch_bounds__(256)
     linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, __nv_bfloat16* out,
                           int64_t ldo) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // n is a multiple of 8
+  grid_dep_wait();
   if (i >= m * n) return;
   float4 s = *reinterpret_cast<const float4*>(acc + i);
+#pragma unroll 4
   for (int k = 1; k < splits; ++k) {
     const float4 q = *reinterpret_cast<const float4*>(acc + (int64_t)k * m * n + i);
     s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
@@ -385,44 +474,100 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------- host
-int map2d(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, int box_inner, int box_rows) {
-  const uint64_t dims[4] = {(uint64_t)inner, (uint64_t)rows, 1, 1};
-  const uint64_t str[3] = {(uint64_t)ld * 2, (uint64_t)ld * 2, (uint64_t)ld * 2};
-  const uint32_t box[4] = {(uint32_t)box_inner, (uint32_t)box_rows, 1, 1};
-  return encode_tma_4d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 struct Matrix {  // rows x cols as they lie in memory, ld elements apart
   const void* p;
   int64_t rows, cols, ld;
 };
 
-int pair_count() {
+int map2d(CUtensorMap* map, const Matrix& x, int box_inner, int box_rows) {
+  const uint64_t dims[4] = {(uint64_t)x.cols, (uint64_t)x.rows, 1, 1};
+  const uint64_t str[3] = {(uint64_t)x.ld * 2, (uint64_t)x.ld * 2, (uint64_t)x.ld * 2};
+  const uint32_t box[4] = {(uint32_t)box_inner, (uint32_t)box_rows, 1, 1};
+  return encode_tma_4d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x.p, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int sms() {
   int dev = 0;
   cudaGetDevice(&dev);
-  return std::max(1, sm_count(dev) / 2);
+  return std::max(2, sm_count(dev));
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Launched behind the grid before it: set-up overlaps that grid's tail, and every kernel waits before it reads.
+template <typename... Params, typename... Given>
+int launch(void (*kernel)(Params...), int64_t grid, int threads, int smem, int cluster, cudaStream_t s, Given&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, std::forward<Given>(args)...), "linear cross entropy launch");
+}
+
+// Tiles of at most 128 rows run on single CTAs: a pair would spend half of its products on rows that are not there.
+int cta_group(int64_t m) { return m <= 128 ? 1 : 2; }
+
+// The tile's width: of the multiples of `step`, the one whose waves of tiles are least work, the widest of equals
+// (a narrower tile reads A more often; 2 % is allowed for that).
+int tile_width(int64_t m, int64_t n, int splits, int step, int units) {
+  const int64_t tm = div_up(m, 128 * cta_group(m));
+  int best = 256;
+  double least = 0;
+  for (int w = 256; w >= 64; w -= step) {
+    const double work = (double)div_up(tm * div_up(n, w) * splits, units) * (w < 128 ? 128 : w);
+    if (w == 256 || work < 0.98 * least) best = w, least = work;
+  }
+  return best;
 }
 
 // One product: a.m x b.n over k.  K-major operands have k columns, MN-major ones k rows.
-template <bool A_MN, bool B_MN, int EPI>
-int gemm(const Matrix& a, const Matrix& b, Args p, cudaStream_t s) {
+template <int CG, bool A_MN, bool B_MN, int EPI>
+int gemm_on(const Matrix& a, const Matrix& b, const CUtensorMap& tc, Args p, cudaStream_t s) {
+  using L = Layout<CG, EPI>;
+  p.tile_n = tile_width(p.m, p.n, p.splits, EPI == kStats && !B_MN ? 32 : 64 * CG, sms() / CG);
   CUtensorMap ta, tb;
-  if (int st = map2d(&ta, a.p, a.cols, a.rows, a.ld, 64, A_MN ? 64 : 128)) return st;
-  if (int st = map2d(&tb, b.p, b.cols, b.rows, b.ld, 64, B_MN ? 64 : 128)) return st;
+  if (int st = map2d(&ta, a, 64, A_MN ? 64 : 128)) return st;
+  if (int st = map2d(&tb, b, 64, B_MN ? 64 : p.tile_n / CG)) return st;
   p.err = device_error_flag();
-  auto kernel = linear_ce_gemm_kernel<A_MN, B_MN, EPI>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
+  p.group = 8;
+  auto kernel = linear_ce_gemm_kernel<CG, A_MN, B_MN, EPI>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem))
     return cuda_status(e, "linear cross entropy: smem attribute");
-  const int64_t tiles = ((p.m + TM - 1) / TM) * ((p.n + TN - 1) / TN) * p.splits;
-  const int64_t pairs = std::min<int64_t>(tiles, pair_count());
-  kernel<<<(unsigned)(2 * pairs), THREADS, kSmem, s>>>(ta, tb, p);
-  return cuda_status(cudaGetLastError(), "linear cross entropy launch");
+  const int64_t tiles = div_up(p.m, 128 * CG) * div_up(p.n, p.tile_n) * p.splits;
+  return launch(kernel, CG * std::min<int64_t>(tiles, sms() / CG), THREADS, L::kSmem, CG, s, ta, tb, tc, p);
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+int gemm(const Matrix& a, const Matrix& b, const CUtensorMap& tc, const Args& p, cudaStream_t s) {
+  return cta_group(p.m) == 1 ? gemm_on<1, A_MN, B_MN, EPI>(a, b, tc, p, s) : gemm_on<2, A_MN, B_MN, EPI>(a, b, tc, p, s);
+}
+
+// ... whose result goes to bf16, or to f32 shares [splits][m][n] when acc is given.
+template <bool A_MN, bool B_MN>
+int gemm_out(const Matrix& a, const Matrix& b, const Matrix& out, float* acc, const Args& p, cudaStream_t s) {
+  CUtensorMap tc;
+  if (!acc) {
+    if (int st = map2d(&tc, out, 64, 32)) return st;
+    return gemm<A_MN, B_MN, kOut>(a, b, tc, p, s);
+  }
+  const uint64_t dims[4] = {(uint64_t)p.n, (uint64_t)p.m, (uint64_t)p.splits, 1};
+  const uint64_t str[3] = {(uint64_t)p.n * 4, (uint64_t)(p.m * p.n) * 4, (uint64_t)(p.m * p.n) * 4};
+  const uint32_t box[4] = {32, 32, 1, 1};
+  if (int st = encode_tma_4d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, acc, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
+  return gemm<A_MN, B_MN, kSum>(a, b, tc, p, s);
 }
 
 constexpr int64_t kAlign = 256;
 int64_t up256(int64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
-int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // Sizes up to here keep every product below within 2^62.
 constexpr int64_t kMaxTokens = 1 << 24, kMaxVocab = 1 << 24, kMaxWidth = 1 << 16;
 
@@ -441,21 +586,23 @@ int check(int64_t tokens, int64_t vocab, int64_t width, int64_t x_stride, int64_
 
 struct FwdPlan {
   int parts;
-  int64_t part, tlogit, bytes;  // byte offsets
+  int64_t tlogit, bytes;  // byte offset of the targets' logits
 };
 FwdPlan plan_fwd(int64_t tokens, int64_t vocab) {
   FwdPlan f{};
-  f.parts = (int)(2 * div_up(vocab, TN));
+  const int w = tile_width(tokens, vocab, 1, 32, sms() / cta_group(tokens));
+  f.parts = (int)(4 * div_up(vocab, w));
   f.tlogit = up256((int64_t)f.parts * tokens * 8);
   f.bytes = f.tlogit + up256(tokens * 4);
   return f;
 }
 
-// Shares of the contracted index for a product that has fewer tiles than there are CTA pairs: each
+// Shares of the contracted index for a product that has fewer tiles than there are CTAs or pairs of them: each
 // share at least 8 blocks of 64.
-void split_k(Args& p, int pairs, int64_t k) {
-  const int64_t tiles = div_up(p.m, TM) * div_up(p.n, TN), nk = div_up(k, TK);
-  int64_t s = std::max<int64_t>(1, std::min(pairs / tiles, nk / 8));
+void split_k(Args& p, int64_t k) {
+  const int cg = cta_group(p.m);
+  const int64_t tiles = div_up(p.m, 128 * cg) * div_up(p.n, 256), nk = div_up(k, TK);
+  int64_t s = std::max<int64_t>(1, std::min(sms() / cg / tiles, nk / 8));
   p.kb_split = (int)div_up(nk, s);
   p.splits = (int)div_up(nk, p.kb_split);
 }
@@ -463,23 +610,23 @@ void split_k(Args& p, int pairs, int64_t k) {
 struct BwdPlan {
   int64_t piece, pieces;  // vocabulary entries per piece
   int dx_splits, dw_splits;
-  int64_t g, unit, dx_acc, dw_acc, bytes;
+  int64_t unit, dx_acc, dw_acc, bytes;
 };
 // G of one piece: at most this many bytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 
-BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width, int pairs) {
+BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   BwdPlan b{};
-  const int64_t most = std::max<int64_t>(TN, kPieceBytes / (2 * std::max<int64_t>(tokens, 1)) / TN * TN);
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * std::max<int64_t>(tokens, 1)) / 256 * 256);
   b.pieces = div_up(vocab, most);
-  b.piece = std::min(div_up(div_up(vocab, b.pieces), TN) * TN, div_up(vocab, 8) * 8);
+  b.piece = std::min(div_up(div_up(vocab, b.pieces), 256) * 256, div_up(vocab, 8) * 8);
   b.pieces = div_up(vocab, b.piece);
   Args a{};
   a.m = tokens, a.n = width;
-  split_k(a, pairs, std::min(b.piece, vocab));
+  split_k(a, std::min(b.piece, vocab));
   b.dx_splits = a.splits;
   a.m = std::min(b.piece, vocab);
-  split_k(a, pairs, tokens);
+  split_k(a, tokens);
   b.dw_splits = a.splits;
   int64_t at = up256(tokens * b.piece * 2);
   b.unit = at;
@@ -492,9 +639,9 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width, int pairs) {
   return b;
 }
 
-void join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, void* out, int64_t ldo, cudaStream_t s) {
-  linear_ce_join_kernel<<<(unsigned)div_up(m * n, 1024), 256, 0, s>>>(acc, splits, m, n, unit,
-                                                                       static_cast<__nv_bfloat16*>(out), ldo);
+int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, void* out, int64_t ldo, cudaStream_t s) {
+  return launch(linear_ce_join_kernel, div_up(m * n, 1024), 256, 0, 1, s, acc, splits, m, n, unit,
+                static_cast<__nv_bfloat16*>(out), ldo);
 }
 
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -526,22 +673,20 @@ extern "C" int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream) 
   p.k = d->width;
   p.splits = 1;
   p.kb_split = (int)div_up(d->width, TK);
-  p.group = 8;
   p.target = d->target;
   p.ignore = d->ignore_index;
   p.vocab = d->vocab;
-  p.part = reinterpret_cast<float2*>(ws + f.part);
+  p.part = reinterpret_cast<float2*>(ws);
   p.tlogit = reinterpret_cast<float*>(ws + f.tlogit);
   const Matrix x{d->x, d->tokens, d->width, d->x_stride}, w{d->w, d->vocab, d->width, d->w_stride};
-  if (int st = gemm<false, false, kStats>(x, w, p, s)) return st;
-  linear_ce_finish_kernel<<<(unsigned)div_up(d->tokens, kFinishWarps), 32 * kFinishWarps, 0, s>>>(
-      p.part, f.parts, p.tlogit, d->target, d->tokens, d->vocab, d->ignore_index, d->loss, d->lse);
-  return cuda_status(cudaGetLastError(), "linear cross entropy finish launch");
+  if (int st = gemm<false, false, kStats>(x, w, CUtensorMap{}, p, s)) return st;
+  return launch(linear_ce_finish_kernel, div_up(d->tokens, 32), 32 * kFinishWarps, 0, 1, s, p.part, f.parts, p.tlogit,
+                d->target, d->tokens, d->vocab, d->ignore_index, d->loss, d->lse);
 }
 
 extern "C" size_t pdb_linear_ce_bwd_workspace_size(const pdb_linear_ce_bwd_desc* d) {
   if (!d || check(d->tokens, d->vocab, d->width, d->x_stride, d->w_stride, d->dtype) != PDB_OK || d->tokens == 0) return 0;
-  return (size_t)plan_bwd(d->tokens, d->vocab, d->width, pair_count()).bytes;
+  return (size_t)plan_bwd(d->tokens, d->vocab, d->width).bytes;
 }
 
 extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) {
@@ -559,22 +704,19 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
   }
   if (!d->x || !d->w || !d->target || !d->lse || !d->dloss)
     return set_error(PDB_ERR_ARG, "linear cross entropy: null x / w / target / lse / dloss");
-  const BwdPlan b = plan_bwd(d->tokens, d->vocab, d->width, pair_count());
+  const BwdPlan b = plan_bwd(d->tokens, d->vocab, d->width);
   if (!d->workspace || d->workspace_bytes < (size_t)b.bytes || !a16(d->workspace))
     return set_error(PDB_ERR_ARG, "linear cross entropy: workspace too small or not 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(d->workspace);
   float* dx_acc = reinterpret_cast<float*>(ws + b.dx_acc);
   float* dw_acc = reinterpret_cast<float*>(ws + b.dw_acc);
   float* unit = reinterpret_cast<float*>(ws + b.unit);
-  linear_ce_unit_kernel<<<1, 1024, 0, s>>>(d->dloss, d->dloss_stride, d->target, d->ignore_index, d->tokens, unit);
-  if (int st = cuda_status(cudaGetLastError(), "linear cross entropy unit launch")) return st;
   const Matrix x{d->x, d->tokens, d->width, d->x_stride};
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, d->vocab - v0);
     const Matrix w{static_cast<const __nv_bfloat16*>(d->w) + v0 * d->w_stride, nv, d->width, d->w_stride};
     const Matrix g{ws, d->tokens, nv, b.piece};
     Args p{};
-    p.group = 8;
     p.m = d->tokens;
     p.n = nv;
     p.k = d->width;
@@ -588,42 +730,38 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
     p.dloss = d->dloss;
     p.dloss_stride = d->dloss_stride;
     p.unit = unit;
-    p.out = reinterpret_cast<__nv_bfloat16*>(ws);
-    p.ldo = b.piece;
-    if (int st = gemm<false, false, kDlogits>(x, w, p, s)) return st;
+    CUtensorMap tc;
+    if (int st = map2d(&tc, g, 64, 32)) return st;
+    if (int st = gemm<false, false, kDlogits>(x, w, tc, p, s)) return st;
     if (d->dw) {
       Args q{};
-      q.group = 8;
       q.m = nv;
       q.n = d->width;
       q.k = d->tokens;
       q.kb_split = (int)div_up(div_up(q.k, TK), b.dw_splits);
       q.splits = (int)div_up(div_up(q.k, TK), q.kb_split);
-      q.out = static_cast<__nv_bfloat16*>(d->dw) + v0 * d->dw_stride;
-      q.ldo = d->dw_stride;
       q.unit = unit;
-      if (q.splits > 1) q.acc = dw_acc;
-      if (int st = gemm<true, true, kOut>(g, x, q, s)) return st;
-      if (q.acc) join(q.acc, q.splits, q.m, q.n, unit, q.out, q.ldo, s);
+      const Matrix dw{static_cast<__nv_bfloat16*>(d->dw) + v0 * d->dw_stride, nv, d->width, d->dw_stride};
+      float* acc = b.dw_splits > 1 ? dw_acc : nullptr;
+      if (int st = gemm_out<true, true>(g, x, dw, acc, q, s)) return st;
+      if (acc)
+        if (int st = join(acc, q.splits, q.m, q.n, unit, const_cast<void*>(dw.p), dw.ld, s)) return st;
     }
     if (d->dx) {
       Args q{};
-      q.group = 8;
       q.m = d->tokens;
       q.n = d->width;
       q.k = nv;
-      // every piece takes the same number of shares, so that each share has its own sum
-      const int64_t nk = div_up(nv, TK);
-      q.kb_split = (int)div_up(nk, b.dx_splits);
-      q.splits = (int)div_up(nk, q.kb_split);
-      q.out = static_cast<__nv_bfloat16*>(d->dx);
-      q.ldo = d->dx_stride;
+      // every piece takes at most the first one's number of shares, and adds to their sums
+      q.kb_split = (int)div_up(div_up(nv, TK), b.dx_splits);
+      q.splits = (int)div_up(div_up(nv, TK), q.kb_split);
       q.unit = unit;
-      if (b.dx_splits > 1 || b.pieces > 1) q.acc = dx_acc;
       q.add = i > 0;
-      if (int st = gemm<false, true, kOut>(g, w, q, s)) return st;
+      const Matrix dx{d->dx, d->tokens, d->width, d->dx_stride};
+      if (int st = gemm_out<false, true>(g, w, dx, b.dx_splits > 1 || b.pieces > 1 ? dx_acc : nullptr, q, s)) return st;
     }
   }
-  if (d->dx && (b.dx_splits > 1 || b.pieces > 1)) join(dx_acc, b.dx_splits, d->tokens, d->width, unit, d->dx, d->dx_stride, s);
-  return cuda_status(cudaGetLastError(), "linear cross entropy join launch");
+  if (d->dx && (b.dx_splits > 1 || b.pieces > 1))
+    return join(dx_acc, b.dx_splits, d->tokens, d->width, unit, d->dx, d->dx_stride, s);
+  return PDB_OK;
 }

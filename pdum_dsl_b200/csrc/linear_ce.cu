@@ -516,15 +516,17 @@ int launch(void (*kernel)(Params...), int64_t grid, int threads, int smem, int c
 // Tiles of at most 128 rows run on single CTAs: a pair would spend half of its products on rows that are not there.
 int cta_group(int64_t m) { return m <= 128 ? 1 : 2; }
 
-// The tile's width: of the multiples of `step`, the one whose waves of tiles are least work, the widest of equals
-// (a narrower tile reads A more often; 2 % is allowed for that).
+// The tile's width: of the multiples of `step`, the one whose waves of tiles load least, since operand rows into shared
+// memory (the tile's rows and its columns) are what a step costs: at 1024 x 50176 x 1024, 17 waves of 160 columns took
+// 105 us where 11 waves of 256 take 84.
 int tile_width(int64_t m, int64_t n, int splits, int step, int units) {
-  const int64_t tm = div_up(m, 128 * cta_group(m));
+  const int rows = 128 * cta_group(m);
+  const int64_t tm = div_up(m, rows);
   int best = 256;
-  double least = 0;
+  int64_t least = 0;
   for (int w = 256; w >= 64; w -= step) {
-    const double work = (double)div_up(tm * div_up(n, w) * splits, units) * (w < 128 ? 128 : w);
-    if (w == 256 || work < 0.98 * least) best = w, least = work;
+    const int64_t work = div_up(tm * div_up(n, w) * splits, units) * (rows + w);
+    if (w == 256 || work < least) best = w, least = work;
   }
   return best;
 }
@@ -619,7 +621,8 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   BwdPlan b{};
   const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * std::max<int64_t>(tokens, 1)) / 256 * 256);
   b.pieces = div_up(vocab, most);
-  b.piece = std::min(div_up(div_up(vocab, b.pieces), 256) * 256, div_up(vocab, 8) * 8);
+  // rows of G on 128-byte lines: with 50024 columns, 1021 x 50021 x 1000 took 94 us for dx
+  b.piece = std::min(div_up(div_up(vocab, b.pieces), 256) * 256, div_up(vocab, 64) * 64);
   b.pieces = div_up(vocab, b.piece);
   Args a{};
   a.m = tokens, a.n = width;

@@ -16,7 +16,8 @@
 //
 // HBM-bound: every element is read and written once.  A thread holds the cos and
 // sin of one 16-byte group of pairs and turns that group in several heads of its
-// position, so the angles cost little.
+// position, so the angles cost little; the loads of four heads are in flight before
+// the first is turned, and the turns run on two pairs per instruction.
 #include <cmath>
 
 #include "common.cuh"
@@ -34,10 +35,12 @@ struct Args {
   const int64_t* pos;
   int64_t ps[2], start;
   int64_t batch, seqlen;
-  int half;        // pairs
-  int units;       // groups of VEC pairs (halves) or VEC / 2 pairs (interleaved), then of VEC features that pass
+  int half;       // pairs
+  int units;      // groups of VEC pairs (halves) or VEC / 2 pairs (interleaved), then of VEC features that pass
   int rot_units;
-  int chunk, chunks;  // heads per thread, and how many such shares
+  int per_block;  // positions that a block's threads cover
+  int chunk;      // heads per thread
+  int shares0;    // shares of x[0]'s heads; x[1]'s follow
   float amplitude;
   uint64_t turns[PDB_ROTARY_MAX_PAIRS];  // per position, in 2^-64 of a turn
 };
@@ -51,24 +54,76 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void from_f32(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 
+// VEC elements as f32 and back, two at a time where there are two.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Pack<T, VEC>& u, float (&f)[VEC]) {
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {  // a bf16 is the upper half of its f32
+      f[2 * j] = __uint_as_float(w[j] << 16);
+      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = to_f32(u.v[j]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void narrow(const float (&f)[VEC], Pack<T, VEC>& u) {
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) w[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) from_f32(u.v[j], f[j]);
+  }
+}
+// (a, c) -> (a cs - c sn, c cs + a sn) for N pairs
+template <int N>
+__device__ __forceinline__ void turn_pairs(float (&a)[N], float (&c)[N], const float (&cs)[N], const float (&sn)[N]) {
+  if constexpr (N == 1) {
+    const float t = a[0] * cs[0] - c[0] * sn[0];
+    c[0] = c[0] * cs[0] + a[0] * sn[0];
+    a[0] = t;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const uint64_t x = f2_pack(a[j], a[j + 1]), y = f2_pack(c[j], c[j + 1]), u = f2_pack(cs[j], cs[j + 1]);
+      f2_unpack(f2_fma(x, u, f2_mul(y, f2_pack(-sn[j], -sn[j + 1]))), a[j], a[j + 1]);
+      f2_unpack(f2_fma(y, u, f2_mul(x, f2_pack(sn[j], sn[j + 1]))), c[j], c[j + 1]);
+    }
+  }
+}
+
 // INTER: a group is VEC features, VEC / 2 pairs (one pair of two accesses where no address is even).
 // Else a group is VEC pairs, VEC features from each half.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args p) {
   using P = Pack<T, VEC>;
-  constexpr int NP = INTER ? (VEC > 1 ? VEC / 2 : 1) : VEC;
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int unit = (int)(i % p.units);
-  const int64_t rest = i / p.units;
-  const int share = (int)(rest % p.chunks);
-  const int64_t bt = rest / p.chunks;
-  const int64_t b = bt / p.seqlen, t = bt - b * p.seqlen;
-  if (b >= p.batch) return;
-  const int h0 = share * p.chunk, total = p.heads[0] + p.heads[1];
-  const int h1 = h0 + p.chunk < total ? h0 + p.chunk : total;
+  constexpr int NP = INTER ? (VEC > 1 ? VEC / 2 : 1) : VEC, FLIGHT = 4;
+  // the second access of a group, where it has one: the other half's, or the other feature of a lone pair
+  constexpr bool TWO = !INTER || VEC == 1;
+  const int span = p.units < kThreads ? p.units : kThreads;
+  const int unit = blockIdx.z * kThreads + (int)threadIdx.x % span, at = (int)threadIdx.x / span;
+  const int64_t bt = (int64_t)blockIdx.x * p.per_block + at;
+  if (at >= p.per_block || unit >= p.units || bt >= p.batch * p.seqlen) return;
+  int64_t b, t;
+  if ((uint64_t)bt <= 0xffffffffu && (uint64_t)p.seqlen <= 0xffffffffu) {
+    b = (uint32_t)bt / (uint32_t)p.seqlen;
+    t = (uint32_t)bt % (uint32_t)p.seqlen;
+  } else {
+    b = bt / p.seqlen;
+    t = bt % p.seqlen;
+  }
+  // this block's share of the heads of one of the tensors
+  const int w = blockIdx.y >= p.shares0;
+  const int h0 = (blockIdx.y - (w ? p.shares0 : 0)) * p.chunk, n = min(p.chunk, p.heads[w] - h0);
   const bool turn = unit < p.rot_units;
   const int j0 = unit * NP;
   const int64_t f0 = turn ? (INTER ? 2 * j0 : j0) : (int64_t)2 * p.half + (unit - p.rot_units) * VEC;
+  const int other = INTER ? 1 : p.half;
   float cs[NP], sn[NP];
   if (turn) {
     const uint64_t pos = (uint64_t)(p.pos ? p.pos[b * p.ps[0] + t * p.ps[1]] : p.start + t);
@@ -81,36 +136,41 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       cs[j] *= p.amplitude;
     }
   }
-  for (int h = h0; h < h1; ++h) {
-    const int w = h >= p.heads[0];
-    const int64_t hh = w ? h - p.heads[0] : h;
-    const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + hh * p.xs[w][1] + t * p.xs[w][2] + f0;
-    T* y = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + hh * p.ys[w][1] + t * p.ys[w][2] + f0;
-    P u = *reinterpret_cast<const P*>(x);
-    if (turn) {
-      if constexpr (INTER && VEC == 1) {
-        const float a = to_f32(u.v[0]), c = to_f32(x[1]);
-        from_f32(u.v[0], a * cs[0] - c * sn[0]);
-        from_f32(y[1], c * cs[0] + a * sn[0]);
-      } else if constexpr (INTER) {
+  const int64_t xh = p.xs[w][1], yh = p.ys[w][1];
+  const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + h0 * xh + t * p.xs[w][2] + f0;
+  T* y = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + h0 * yh + t * p.ys[w][2] + f0;
+  for (int h = 0; h < n; h += FLIGHT) {
+    P u[FLIGHT], v[FLIGHT];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          const float a = to_f32(u.v[2 * j]), c = to_f32(u.v[2 * j + 1]);
-          from_f32(u.v[2 * j], a * cs[j] - c * sn[j]);
-          from_f32(u.v[2 * j + 1], c * cs[j] + a * sn[j]);
-        }
-      } else {
-        P v = *reinterpret_cast<const P*>(x + p.half);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          const float a = to_f32(u.v[j]), c = to_f32(v.v[j]);
-          from_f32(u.v[j], a * cs[j] - c * sn[j]);
-          from_f32(v.v[j], c * cs[j] + a * sn[j]);
-        }
-        *reinterpret_cast<P*>(y + p.half) = v;
-      }
+    for (int i = 0; i < FLIGHT; ++i, x += xh) {
+      if (h + i >= n) break;
+      u[i] = *reinterpret_cast<const P*>(x);
+      if (TWO && turn) v[i] = *reinterpret_cast<const P*>(x + other);
     }
-    *reinterpret_cast<P*>(y) = u;
+#pragma unroll
+    for (int i = 0; i < FLIGHT; ++i, y += yh) {
+      if (h + i >= n) break;
+      if (turn) {
+        float f[VEC];
+        widen<T, VEC>(u[i], f);
+        if constexpr (TWO) {
+          float g[VEC];
+          widen<T, VEC>(v[i], g);
+          turn_pairs<NP>(f, g, cs, sn);
+          narrow<T, VEC>(g, v[i]);
+          *reinterpret_cast<P*>(y + other) = v[i];
+        } else {
+          float a[NP], c[NP];
+#pragma unroll
+          for (int j = 0; j < NP; ++j) a[j] = f[2 * j], c[j] = f[2 * j + 1];
+          turn_pairs<NP>(a, c, cs, sn);
+#pragma unroll
+          for (int j = 0; j < NP; ++j) f[2 * j] = a[j], f[2 * j + 1] = c[j];
+        }
+        narrow<T, VEC>(f, u[i]);
+      }
+      *reinterpret_cast<P*>(y) = u[i];
+    }
   }
 }
 
@@ -124,19 +184,23 @@ int launch(Args& p, const pdb_rotary_desc& d, cudaStream_t s) {
   if (p.units == 0) return PDB_OK;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int total = p.heads[0] + p.heads[1];
-  const int64_t points = p.batch * p.seqlen * p.units;
-  // heads per thread: 8 where that leaves every SM four blocks, fewer otherwise
-  const int64_t want = (int64_t)sm_count(dev) * 4 * kThreads;
-  p.chunk = 8;
-  while (p.chunk > 1 && points * ((total + p.chunk - 1) / p.chunk) < want) p.chunk >>= 1;
-  p.chunks = (total + p.chunk - 1) / p.chunk;
-  const int64_t blocks = (points * p.chunks + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return set_error(PDB_ERR_SHAPE, "rotary: too many heads and positions for one launch");
+  const int span = p.units < kThreads ? p.units : kThreads;
+  p.per_block = kThreads / span;
+  const int64_t points = p.batch * p.seqlen;
+  const int64_t bx = (points + p.per_block - 1) / p.per_block, bz = (p.units + kThreads - 1) / kThreads;
+  if (bx > 0x7fffffffLL) return set_error(PDB_ERR_SHAPE, "rotary: too many positions for one launch");
+  // heads per thread: 8 (16 of narrow groups, whose angles weigh more) where that leaves every SM four blocks, fewer
+  // otherwise
+  auto shares = [&](int n) { return (n + p.chunk - 1) / p.chunk; };
+  p.chunk = VEC * sizeof(T) >= 8 ? 8 : 16;
+  while (p.chunk > 1 && bx * bz * (shares(p.heads[0]) + shares(p.heads[1])) < (int64_t)sm_count(dev) * 4) p.chunk >>= 1;
+  while (shares(p.heads[0]) + shares(p.heads[1]) > 65535) p.chunk *= 2;
+  p.shares0 = shares(p.heads[0]);
+  const dim3 grid((unsigned)bx, (unsigned)(p.shares0 + shares(p.heads[1])), (unsigned)bz);
   if (inter)
-    rotary_kernel<T, VEC, true><<<(unsigned)blocks, kThreads, 0, s>>>(p);
+    rotary_kernel<T, VEC, true><<<grid, kThreads, 0, s>>>(p);
   else
-    rotary_kernel<T, VEC, false><<<(unsigned)blocks, kThreads, 0, s>>>(p);
+    rotary_kernel<T, VEC, false><<<grid, kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError(), "rotary launch");
 }
 

@@ -172,7 +172,6 @@ def test_linear_cross_entropy_workspaces():
     """The gradient's workspace is one piece of G (at most 512 MiB, or 256 columns) and f32 sums of dx, where they are
     shared or in pieces; the largest sizes stay within 64 bits."""
     lib = _lib.load()
-    al = lambda n: (n + 255) // 256 * 256
 
     def need(tokens, vocab, width):
         kw = dict(tokens=tokens, vocab=vocab, width=width, x_stride=width, w_stride=width)
@@ -182,7 +181,7 @@ def test_linear_cross_entropy_workspaces():
     assert need(8192, 128000, 4096) == 8192 * 32000 * 2 + 256 + 4 * 8192 * 4096  # four pieces of 32000
     assert need(8192, 32000, 4096) == 8192 * 32000 * 2 + 256  # one
     assert need(1 << 24, 1 << 24, 1 << 16) == (1 << 24) * 256 * 2 + 256 + 4 * (1 << 40)
-    assert need(1, 1, 8) == al(2 * 8) + 256
+    assert need(1, 1, 8) == 256 + 256
 
 
 def test_host_tensors_are_refused():

@@ -8,6 +8,7 @@ entry point raises ``BackendUnavailable``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libpdb_sm100.so"
@@ -333,6 +334,10 @@ class RotaryDesc(C.Structure):
         ("dtype", C.c_int32),
         ("reserved", C.c_int32),
     ]
+
+
+# RotaryDesc as one struct record, field for field (the nested arrays flattened)
+ROTARY_PACK = struct.Struct(f"4Q14qQ7qd{8 * ROTARY_MAX_PAIRS}s4i")
 
 
 class LinearCeFwdDesc(C.Structure):

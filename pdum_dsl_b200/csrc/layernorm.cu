@@ -740,8 +740,9 @@ int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
-// elements of bf16 with the sums' join: 39-40 us at 128 to 2048 columns, a copy of as many bytes 37.  8192 columns of
-// f32 keep two rows (196 KB for three leave the caches too little: 84 against 76 us).
+// elements of bf16 with the sums' join: 38-40 us at 128 to 4096 columns, a copy of as many bytes 37; 51 us at 8192,
+// where an SM has one row at a time.  Blocks of 512 threads on f32 keep two rows (three, 196 KB, leave the caches too
+// little: 83 against 74 us at 8192 columns).
 template <typename T, int VEC, bool RAG>
 int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
   constexpr int NV = VEC == 1 ? 4 : 16 / VEC, N = VEC == 1 ? 3 : 2;
@@ -750,8 +751,9 @@ int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
   if (!r) r = launch_bwd<T, VEC, NV, 32, 256, 3, RAG>(p, N, s);
   if (!r) r = launch_bwd<T, VEC, NV, 64, 256, 3, RAG>(p, N, s);
   if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, N, s);
-  if (!r) r = launch_bwd<T, VEC, NV, 256, VEC == 1 ? 256 : 512, 3, RAG>(p, VEC == 1 ? 3 : 1, s);
-  if (!r) r = launch_bwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, sizeof(T) == 4 ? 2 : 3, RAG>(p, 1, s);
+  constexpr int S = sizeof(T) == 4 ? 2 : 3;
+  if (!r) r = launch_bwd<T, VEC, NV, 256, VEC == 1 ? 256 : 512, S, RAG>(p, VEC == 1 ? 3 : 1, s);
+  if (!r) r = launch_bwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, S, RAG>(p, 1, s);
   return r;
 }
 

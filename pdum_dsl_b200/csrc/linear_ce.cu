@@ -427,15 +427,17 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
   grid_dep_wait();
   float2 s = make_float2(-INFINITY, 0.f);
   if (row < tokens) {
-    int i = warp;
-    for (; i + 3 * kFinishWarps < parts; i += 4 * kFinishWarps) {
-      float2 q[4];
+    constexpr int FLIGHT = 8;  // loads before the first is joined
+    for (int i = warp; i < parts; i += FLIGHT * kFinishWarps) {
+      float2 q[FLIGHT];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) q[u] = part[(int64_t)(i + u * kFinishWarps) * tokens + row];
+      for (int u = 0; u < FLIGHT; ++u) {
+        const int k = i + u * kFinishWarps;
+        q[u] = k < parts ? part[(int64_t)k * tokens + row] : make_float2(-INFINITY, 0.f);
+      }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) join(s, q[u]);
+      for (int u = 0; u < FLIGHT; ++u) join(s, q[u]);
     }
-    for (; i < parts; i += kFinishWarps) join(s, part[(int64_t)i * tokens + row]);
   }
   red[warp][lane] = s;
   __syncthreads();

@@ -118,10 +118,11 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Te
             check(load().pdb_layernorm_f32(C.byref(d), _stream(x)), "pdb_layernorm_f32")
         return y.view(x.shape)
     x2 = _own_rows(x2)
-    y = torch.empty((R, C_), dtype=x.dtype, device=x.device) if out is None else _out_rows("layernorm", out, x2)
+    y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
     mean = rstd = at_m = at_r = None
     if return_stats:
-        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
         at_m, at_r = mean.data_ptr(), rstd.data_ptr()
     d = _lib.LayerNormFwdDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), at_m, at_r, R, C_, x2.stride(0), y.stride(0),
                               eps, _DTYPES[x.dtype], _DTYPES[ptype])
@@ -153,7 +154,7 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
     ptype = _param_dtype("layernorm_backward", x, C_, gamma, None)
     g = gamma.contiguous() if gamma is not None else None
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x2)
     dgamma = dbeta = None
     d = _lib.LayerNormBwdDesc(do2.data_ptr(), x2.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                               g.data_ptr() if g is not None else None, dx.data_ptr(), None, None, None, 0, R, C_,
@@ -161,13 +162,14 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
     lib = load()
     with _on_device_of(x):
         if weight_grads:
-            dgamma, dbeta = torch.empty((2, C_), dtype=ptype, device=x.device).unbind(0)
+            dgamma = x.new_empty((C_,), dtype=ptype)
+            dbeta = torch.empty_like(dgamma)
             d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
             nbytes = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
-            ws = torch.empty(nbytes + 16, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(nbytes + 16, dtype=torch.uint8)
             d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
         check(lib.pdb_layernorm_bwd(C.byref(d), _raw_stream(x)), "pdb_layernorm_bwd")
-    return dx, dgamma, dbeta
+    return dx if dx.shape == x.shape else dx.view(x.shape), dgamma, dbeta
 
 
 def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -313,21 +315,22 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
             if (o.shape[-1] > 1 and o.stride(-1) != 1) or any(m > 1 and st == 0 for m, st in zip(o.shape, o.stride())):
                 raise ValueError("rotary: out must have unit stride along the features and no broadcast dim")
         ys = [_as4d(o, "out") for o in outs]
-    d = _lib.RotaryDesc()
-    for i, (x, y) in enumerate(zip(xs, ys)):
-        d.x[i], d.y[i], d.heads[i] = x.data_ptr(), y.data_ptr(), x.shape[1]
-        d.x_stride[i][:], d.y_stride[i][:] = x.stride()[:3], y.stride()[:3]
+    at_p, ps = 0, (0, 0)
     if positions is not None:
         if positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
             raise TypeError("rotary: positions must be an integer tensor on q's device")
         if positions.dim() not in (1, 2):
             raise ValueError("rotary: positions must be (T,) or (B, T)")
-        p = positions.to(torch.int64).expand(B, T)
-        d.positions = p.data_ptr()
-        d.pos_stride[:] = p.stride()
-    d.start, d.batch, d.seqlen, d.head_dim, d.rotary_dim = start, B, T, D, 2 * n
-    d.amplitude, d.interleaved, d.inverse, d.dtype = amplitude, bool(interleaved), bool(inverse), _DTYPES[q.dtype]
-    C.memmove(d.inv_freq, freq.ctypes.data, freq.nbytes)
+        p = positions if positions.dtype == torch.int64 else positions.to(torch.int64)
+        if p.shape != (B, T):
+            p = p.expand(B, T)
+        at_p, ps = p.data_ptr(), p.stride()
+    # one packed record: a third of the time of setting the descriptor's fields one by one
+    x0, y0, x1, y1 = xs[0], ys[0], xs[-1], ys[-1]
+    d = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(
+        x0.data_ptr(), x1.data_ptr(), y0.data_ptr(), y1.data_ptr(), x0.shape[1], 0 if k is None else x1.shape[1],
+        *x0.stride()[:3], *x1.stride()[:3], *y0.stride()[:3], *y1.stride()[:3], at_p, *ps, start, B, T, D, 2 * n,
+        amplitude, freq.tobytes(), bool(interleaved), bool(inverse), _DTYPES[q.dtype], 0))
     with _on_device_of(q):
         check(load().pdb_rotary(C.byref(d), _raw_stream(q)), "pdb_rotary")
     rets = tuple(y if y.shape == t.shape else y.view(t.shape) for y, t in zip(ys, ts)) if out is None else outs
@@ -442,7 +445,7 @@ def pointwise(x: torch.Tensor, program, out: torch.Tensor | None = None) -> torc
     return y
 
 
-def _head_operand(name: str, t: torch.Tensor) -> torch.Tensor:
+def _head_operand(t: torch.Tensor) -> torch.Tensor:
     """A 2-D bf16 matrix as the tensor maps take it: 16-byte aligned rows with unit stride, laid out anew otherwise."""
     R, W = t.shape
     ok = t.data_ptr() % 16 == 0 and (W <= 1 or t.stride(1) == 1) and (R <= 1 or (t.stride(0) >= W and t.stride(0) % 8 == 0))
@@ -463,7 +466,9 @@ def _head_args(what: str, x, weight, target):
         raise TypeError(f"{what}: target must be int64")
     if weight.device != x.device or target.device != x.device:
         raise ValueError(f"{what}: tensors on different devices")
-    return _head_operand("x", x.reshape(-1, x.shape[-1])), _head_operand("weight", weight), target.reshape(-1).contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    t = target if target.dim() == 1 else target.reshape(-1)
+    return _head_operand(x2), _head_operand(weight), t.contiguous()
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
@@ -475,17 +480,16 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     another index outside the vocabulary; with ``return_lse`` (loss, lse), which the backward takes."""
     x2, w, t = _head_args("linear_cross_entropy", x, weight, target)
     N, W = x2.shape
-    out = torch.empty((2 if return_lse else 1, N), dtype=torch.float32, device=x.device)
-    at = out.data_ptr()
-    d = _lib.LinearCeFwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), at, at + 4 * N if return_lse else None, None, 0,
+    loss = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    lse = torch.empty_like(loss)
+    d = _lib.LinearCeFwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), None, 0,
                              N, w.shape[0], W, _head_stride(x2), _head_stride(w), int(ignore_index), _lib.PDB_BF16, 0)
     lib = load()
     with _on_device_of(x):
-        ws = torch.empty(lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.pdb_linear_ce_fwd(C.byref(d), _raw_stream(x)), "pdb_linear_ce_fwd")
-    lead = x.shape[:-1]
-    return (out[0].view(lead), out[1].view(lead)) if return_lse else out[0].view(lead)
+    return (loss, lse) if return_lse else loss
 
 
 def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, dloss: torch.Tensor,
@@ -511,14 +515,14 @@ def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target:
         g, gs = dloss, 0
     else:
         g, gs = dloss.expand(target.shape).reshape(-1).contiguous(), 1
-    dx = torch.empty((N, W), dtype=torch.bfloat16, device=x.device) if need_dx else None
-    dw = torch.empty((V, W), dtype=torch.bfloat16, device=x.device) if need_dweight else None
+    dx = x.new_empty((N, W)) if need_dx else None
+    dw = x.new_empty((V, W)) if need_dweight else None
     d = _lib.LinearCeBwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), lse.data_ptr(), g.data_ptr(),
                              dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dweight else None, None, 0,
                              N, V, W, _head_stride(x2), _head_stride(w), W, W, gs, int(ignore_index), _lib.PDB_BF16, 0)
     lib = load()
     with _on_device_of(x):
-        ws = torch.empty(lib.pdb_linear_ce_bwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(lib.pdb_linear_ce_bwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
         check(lib.pdb_linear_ce_bwd(C.byref(d), _raw_stream(x)), "pdb_linear_ce_bwd")
     return dx.view(x.shape) if need_dx else None, dw

@@ -94,6 +94,21 @@ def _rot(**kw):
     return d
 
 
+def test_rotary_record_is_the_descriptor():
+    """The packed record fills every field of the descriptor in order."""
+    freq = np.arange(64, dtype=np.float64)
+    assert _lib.ROTARY_PACK.size == C.sizeof(_lib.RotaryDesc)
+    d = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(*range(1, 5), *range(5, 19), 19, *range(20, 27), 27.5,
+                                                               freq.tobytes(), 1, 2, 3, 4))
+    assert list(d.x) == [1, 2] and list(d.y) == [3, 4] and list(d.heads) == [5, 6]
+    assert [list(s) for s in d.x_stride] == [[7, 8, 9], [10, 11, 12]]
+    assert [list(s) for s in d.y_stride] == [[13, 14, 15], [16, 17, 18]]
+    assert (d.positions, list(d.pos_stride), d.start) == (19, [20, 21], 22)
+    assert (d.batch, d.seqlen, d.head_dim, d.rotary_dim, d.amplitude) == (23, 24, 25, 26, 27.5)
+    assert list(d.inv_freq) == [*freq] + [0.0] * 64
+    assert (d.interleaved, d.inverse, d.dtype, d.reserved) == (1, 2, 3, 4)
+
+
 def test_rotary_refusals():
     lib = _lib.load()
     assert lib.pdb_rotary(None, None) == _lib.PDB_ERR_ARG

@@ -8,10 +8,12 @@
 //
 // Forward: one product whose epilogue reduces each row of a tile to a running
 // maximum and a sum of exponentials (32 bits), and a small kernel that joins the
-// tiles' pairs.  Backward: per piece of the vocabulary, the product again with an
-// epilogue that turns logits into G (bf16, the operand type of the two products
-// that follow), then dw of the piece, complete in one product, and dx, summed over
-// the pieces in f32.
+// tiles' pairs.  Backward: the tokens that are ignored are left out first (their rows
+// of x are not even read by the products, whatever they hold), by a kernel that packs
+// the others' rows and counts them; the products take the count from memory.  Then,
+// per piece of the vocabulary, the product again with an epilogue that turns logits
+// into G (bf16, the operand type of the two products that follow), dw of the piece,
+// complete in one product, and dx, summed over the pieces in f32.
 //
 // All of it is bound by the tensor cores: 2 (forward) and 6 (backward) x tokens x
 // vocab x width operations.  One persistent kernel serves the four products: tiles of
@@ -56,16 +58,21 @@ struct Args {
   int splits, kb_split;  // shares of the contracted index, and 64-wide blocks in each
   int group;             // m tiles that share a sweep over the n tiles
   int* err;
-  // kStats, kDlogits: rows are tokens, columns vocabulary entries from col0 on
+  // The tokens that count, found on the device: state[0] of them; state[1]: their rows of x are packed, under tm_x.
+  const int* state;      // null: all of them, unpacked
+  int dyn;               // 1: m, 2: k is their number
+  const int* token_of;   // kOut: the row of the result that each packed row goes to
+  __nv_bfloat16* out;    // ... and the result
+  int64_t ldo;
+  // kStats, kDlogits: rows are (packed) tokens, columns vocabulary entries from col0 on
   const int64_t* target;
-  int64_t col0, ignore, vocab;
-  float2* part;   // kStats: (base, sum) per [4 x n tile][m]
-  float* tlogit;  // kStats: the target's logit
-  const float* lse;
+  int64_t col0, vocab;
+  float2* part;        // kStats: (base, sum) per [4 x n tile][m]
+  float* tlogit;       // kStats: the target's logit
+  const float* lse;    // kDlogits
   const float* dloss;
-  int64_t dloss_stride;
-  float* unit;  // kDlogits: written, the unit that G is measured in; kOut: multiplies the result
-  int add;      // kSum: add to what is there
+  const float* unit;   // kDlogits: the unit that G is measured in; kOut: multiplies the result
+  int add;             // kSum: add to what is there
 };
 
 struct __align__(8) Bars {
@@ -73,7 +80,6 @@ struct __align__(8) Bars {
   uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort;
-  float unit[kEpiWarps];
 };
 static_assert(sizeof(Bars) <= 256, "the barriers' share of shared memory");
 
@@ -119,28 +125,6 @@ __device__ __forceinline__ void fold(const float (&v)[32], float& base, float& s
   base = top;
 }
 
-// The unit that dloss is measured in: its largest finite magnitude over the tokens that count (1 if that is 0).  G
-// is rounded to bf16 in this unit.  In dloss's own units the entries of all targets, -(1 - p) dloss with p near 0,
-// would under a mean be one and the same number, whose rounding (up to 2^-9) would not average out but scale the
-// whole gradient; in this unit it is 1, which is exact.  Every CTA finds it for itself, while its first tile's
-// products run.
-__device__ __forceinline__ float find_unit(const Args& p, float* red, int warp, int lane) {
-  float m = 0.f;
-  for (int64_t i = warp * 32 + lane; i < p.m; i += 32 * kEpiWarps) {
-    const float a = fabsf(p.dloss[i * p.dloss_stride]);
-    if (p.target[i] != p.ignore && a <= FLT_MAX) m = fmaxf(m, a);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
-#pragma unroll
-  for (int i = 0; i < kEpiWarps; ++i) m = fmaxf(m, red[i]);
-  m = m > 0.f ? m : 1.f;
-  if (blockIdx.x == 0 && warp == 0 && lane == 0) *p.unit = m;
-  return m;
-}
-
 template <int CG>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
   if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, abort, err);
@@ -150,7 +134,8 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 template <int CG, bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
     linear_ce_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                          const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ Args p) {
+                          const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ CUtensorMap tm_x,
+                          const __grid_constant__ Args p) {
   using L = Layout<CG, EPI>;
   constexpr int TM = 128 * CG, STAGES = L::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -162,10 +147,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const int unit_id = blockIdx.x / CG, units = gridDim.x / CG;
-  const int nk = (int)((p.k + TK - 1) / TK);
-  const int tm = (int)((p.m + TM - 1) / TM), tn = (int)((p.n + p.tile_n - 1) / p.tile_n);
-  const int64_t num_tiles = (int64_t)tm * tn * p.splits;
-
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tm_a);
     prefetch_tensormap(&tm_b);
@@ -197,9 +178,22 @@ __global__ void __launch_bounds__(THREADS, 1)
   grid_dep_wait();  // the launch before may still be writing what this one reads
   const uint32_t tmem = bar->tmem_base;
   volatile int* abort = &bar->abort;
+  int64_t m = p.m, k = p.k;
+  bool packed = false, scatter = false;
+  if (EPI != kStats && p.state) {
+    const int count = p.state[0];
+    packed = p.state[1] != 0;
+    scatter = p.dyn == 1 && count < m;
+    (p.dyn == 1 ? m : k) = count;
+  }
+  const int nk = (int)((k + TK - 1) / TK), kb_split = p.dyn == 2 ? (nk + p.splits - 1) / p.splits : p.kb_split;
+  const int tm = (int)((m + TM - 1) / TM), tn = (int)((p.n + p.tile_n - 1) / p.tile_n);
+  const int64_t num_tiles = (int64_t)tm * tn * p.splits;
 
   if (warp == 0 && lane == 0) {
     const int b_rows = p.tile_n / CG;  // of B per CTA
+    const CUtensorMap* map_a = EPI == kDlogits && packed ? &tm_x : &tm_a;
+    const CUtensorMap* map_b = A_MN && packed ? &tm_x : &tm_b;
     const uint32_t bytes = CG * (kTileA + b_rows * TK * 2);
     uint32_t g = 0;
     bool ok = true;
@@ -207,7 +201,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int split;
       int64_t m0, n0;
       tile_at<TM>(p, tm, tn, t, split, m0, n0);
-      const int kb0 = split * p.kb_split, kb1 = min(nk, kb0 + p.kb_split);
+      const int kb0 = split * kb_split, kb1 = min(nk, kb0 + kb_split);
       const int ma = (int)m0 + (int)rank * 128, nb = (int)n0 + (int)rank * b_rows;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
         const int st = g % STAGES;
@@ -220,15 +214,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         uint8_t *a = sA + st * kTileA, *b = sB + st * L::kTileB;
         if constexpr (A_MN) {
-          load(a, &tm_a, ma, kb * TK);
-          load(a + kBox, &tm_a, ma + 64, kb * TK);
+          load(a, map_a, ma, kb * TK);
+          load(a + kBox, map_a, ma + 64, kb * TK);
         } else {
-          load(a, &tm_a, kb * TK, ma);
+          load(a, map_a, kb * TK, ma);
         }
         if constexpr (B_MN) {
-          for (int r = 0; r < b_rows; r += 64) load(b + r / 64 * kBox, &tm_b, nb + r, kb * TK);
+          for (int r = 0; r < b_rows; r += 64) load(b + r / 64 * kBox, map_b, nb + r, kb * TK);
         } else {
-          load(b, &tm_b, kb * TK, nb);
+          load(b, map_b, kb * TK, nb);
         }
       }
     }
@@ -242,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     for (int64_t t = unit_id; ok && t < num_tiles; t += units, ++tt) {
       const int split = (int)(t / ((int64_t)tm * tn));
-      const int kb0 = split * p.kb_split, kb1 = min(nk, kb0 + p.kb_split);
+      const int kb0 = split * kb_split, kb1 = min(nk, kb0 + kb_split);
       const int buf = tt & 1;
       if (!(ok = wait_bar<CG>(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
       tc_fence_after();
@@ -282,8 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const uint32_t stage = smem_u32(sC + e * kStore), srow = stage + lane * 128;
     float unit = 1.f;
-    if constexpr (EPI == kDlogits) unit = find_unit(p, bar->unit, e, lane);
-    if constexpr (EPI == kOut) unit = p.unit ? *p.unit : 1.f;
+    if constexpr (EPI == kDlogits || EPI == kOut) unit = *p.unit;
     uint32_t tt = 0;
     for (int64_t t = unit_id; t < num_tiles; t += units, ++tt) {
       int split;
@@ -291,18 +284,17 @@ __global__ void __launch_bounds__(THREADS, 1)
       tile_at<TM>(p, tm, tn, t, split, m0, n0);
       const int buf = tt & 1;
       const int64_t gm = m0 + row0 + lane;
-      const bool live = gm < p.m;
+      const bool live = gm < m;
+      const bool none = split * kb_split >= nk;  // a share of the contracted index without any of it
       int64_t tgt = -1;
       float nlse = 0.f, up = 0.f;
-      bool skip = true;
       if constexpr (EPI == kStats || EPI == kDlogits) {
         if (live) {
           tgt = p.target[gm];
-          skip = tgt == p.ignore;
           if constexpr (EPI == kDlogits) {
             nlse = -p.lse[gm] * kLog2e;
-            up = p.dloss[gm * p.dloss_stride] / unit;
-            if (!skip && (tgt < 0 || tgt >= p.vocab)) up = NAN;  // no such entry: the gradient says so
+            up = p.dloss[gm] / unit;
+            if (tgt < 0 || tgt >= p.vocab) up = NAN;  // no such entry: the gradient says so
           }
           tgt -= p.col0;
         }
@@ -319,6 +311,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         tmem_ld32(tmem + lane_off + buf * 256 + c, r);
         tmem_wait_ld();
+        if ((EPI == kOut || EPI == kSum) && none) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -344,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int i = 0; i < 8; ++i) sts128(srow + ((i ^ (lane & 7)) << 4), r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && m0 + row0 < p.m) {
+          if (lane == 0 && m0 + row0 < m) {
             if (p.add) tma_reduce_add_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
             else tma_store_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
             bulk_commit();
@@ -372,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             float x, y;
             f2_unpack(f2_mul(f2_pack(v[2 * i], v[2 * i + 1]), s2), x, y);
             pk[i] = pack_bf16(x, y);
-            if constexpr (EPI == kDlogits) pk[i] = skip ? 0u : pk[i];
+            if constexpr (EPI == kDlogits) pk[i] = live ? pk[i] : 0u;
           }
           if (ch == 0) {
             if (lane == 0) bulk_wait_read_all();
@@ -385,17 +381,32 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if constexpr (EPI == kOut || EPI == kDlogits) {
         // the box is cut at the last row and column by its tensor map
-        if (cg * 64 < p.tile_n && n0 + cg * 64 < p.n && m0 + row0 < p.m) {
+        // (rows of G behind the last token are 0 up to the end of a block of 64, which dw sums over)
+        const int64_t rows = EPI == kDlogits ? min(p.m, (m + TK - 1) / TK * TK) : m;
+        if (cg * 64 < p.tile_n && n0 + cg * 64 < p.n && m0 + row0 < rows) {
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
+          if (EPI == kOut && !A_MN && scatter) {  // eight lanes per row, four rows at a time, each to its token's row
+            const int64_t col = n0 + cg * 64 + (lane & 7) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              const int64_t row = m0 + row0 + r;
+              uint4 q;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                           : "r"(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4))
+                           : "memory");
+              if (row < m && col < p.n) *reinterpret_cast<uint4*>(p.out + p.token_of[row] * p.ldo + col) = q;
+            }
+          } else if (lane == 0) {
             tma_store_4d(&tm_c, stage, (int)n0 + cg * 64, (int)m0 + row0, 0, 0);
             bulk_commit();
           }
         }
       }
       if constexpr (EPI == kStats)
-        if (live) p.part[((n0 / p.tile_n) * 4 + cg) * p.m + gm] = make_float2(base, sum);
+        if (live) p.part[((n0 / p.tile_n) * 4 + cg) * m + gm] = make_float2(base, sum);
       if constexpr (CG == 2) warp_arrive_cluster_after_tc(mapa_shared(smem_u32(&bar->acc_empty[buf]), 0));
       else warp_arrive_after_tc(&bar->acc_empty[buf]);
     }
@@ -457,13 +468,13 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
   }
 }
 
-// The f32 shares of a product, added in order, scaled and rounded.
+// The f32 shares of a product, added in order, scaled and rounded; packed rows go to their tokens' rows.
 __global__ void __launch_bounds__(256)
-    linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, __nv_bfloat16* out,
-                          int64_t ldo) {
+    linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state,
+                          const int* token_of, __nv_bfloat16* out, int64_t ldo) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // n is a multiple of 8
   grid_dep_wait();
-  if (i >= m * n) return;
+  if (i >= (state ? *state : m) * n) return;
   float4 s = *reinterpret_cast<const float4*>(acc + i);
 #pragma unroll 4
   for (int k = 1; k < splits; ++k) {
@@ -472,7 +483,122 @@ __global__ void __launch_bounds__(256)
   }
   const float u = *unit;
   uint2 o = make_uint2(pack_bf16(s.x * u, s.y * u), pack_bf16(s.z * u, s.w * u));
-  *reinterpret_cast<uint2*>(out + (i / n) * ldo + i % n) = o;
+  const int64_t row = i / n;
+  *reinterpret_cast<uint2*>(out + (token_of ? token_of[row] : row) * ldo + i % n) = o;
+}
+
+// Packs the tokens that count, in their order: their rows of x (when a token is ignored, or `pack`: rows that do not
+// start on 128-byte lines cost the products a quarter more reads), targets, lse and dloss; and writes their number, the
+// rows of dx that stay 0, and the unit of dloss.
+//
+// The unit is dloss's largest finite magnitude over those tokens (1 if that is 0).  G is rounded to bf16 in this unit.
+// In dloss's own units the entries of all targets, -(1 - p) dloss with p near 0, would under a mean be one and the same
+// number, whose rounding (up to 2^-9) would not average out but scale the whole gradient; in this unit it is 1, which
+// is exact.
+//
+// A block packs `rows` tokens; for its place it counts the tokens before them itself, so one launch is enough.
+struct Pack {
+  const __nv_bfloat16* x;
+  const int64_t* target;
+  const float* lse;
+  const float* dloss;
+  int64_t tokens, width, ldx, dloss_stride, ignore;
+  int rows, pack;
+  __nv_bfloat16* xp;  // [tokens][ldp]
+  int64_t ldp;
+  int64_t* targetp;
+  float* lsep;
+  float* dlossp;
+  int* token_of;
+  int* state;
+  float* unit;
+  __nv_bfloat16* dx;  // nullable
+  int64_t lddx;
+};
+
+constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32;
+
+__global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack p) {
+  __shared__ int before_s[kPackWarps], total_s[kPackWarps], place[kPackThreads];
+  __shared__ float max_s[kPackWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t first = (int64_t)blockIdx.x * p.rows, last = min(p.tokens, first + p.rows);
+  grid_dep_wait();
+  int before = 0, total = 0;
+  float top = 0.f;
+  constexpr int FLIGHT = 16;  // loads before the first is looked at: the count is all latency
+  for (int i = tid; i < (int)p.tokens; i += FLIGHT * kPackThreads) {
+    int64_t t[FLIGHT];
+    float a[FLIGHT];
+#pragma unroll
+    for (int u = 0; u < FLIGHT; ++u) {
+      const int n = i + u * kPackThreads;
+      t[u] = n < (int)p.tokens ? p.target[n] : p.ignore;
+      a[u] = n < (int)p.tokens && blockIdx.x == 0 ? fabsf(p.dloss[n * p.dloss_stride]) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < FLIGHT; ++u) {
+      const bool counts = t[u] != p.ignore;
+      before += counts && i + u * kPackThreads < first;
+      total += counts;
+      if (counts && a[u] <= FLT_MAX) top = fmaxf(top, a[u]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if (lane == 0) before_s[warp] = before, total_s[warp] = total, max_s[warp] = top;
+  __syncthreads();
+  before = total = 0;
+  for (int i = 0; i < kPackWarps; ++i) before += before_s[i], total += total_s[i], top = fmaxf(top, max_s[i]);
+  const bool pack = p.pack || total < p.tokens;
+  if (blockIdx.x == 0 && tid == 0) {
+    p.state[0] = total;
+    p.state[1] = pack;
+    *p.unit = top > 0.f ? top : 1.f;
+  }
+  const int64_t vecs = p.width / 8;
+  for (int64_t c = first; c < last; c += kPackThreads) {
+    const int64_t n = c + tid;
+    const bool counts = n < last && p.target[n] != p.ignore;
+    const uint32_t votes = __ballot_sync(0xffffffffu, counts);
+    __syncthreads();
+    if (lane == 0) before_s[warp] = __popc(votes);
+    __syncthreads();
+    int at = before + __popc(votes & ((1u << lane) - 1u)), all = 0;
+    for (int i = 0; i < kPackWarps; ++i) {
+      at += i < warp ? before_s[i] : 0;
+      all += before_s[i];
+    }
+    before += all;
+    place[tid] = counts ? at : -1;
+    if (counts) {
+      p.targetp[at] = p.target[n];
+      p.lsep[at] = p.lse[n];
+      p.dlossp[at] = p.dloss[n * p.dloss_stride];
+      p.token_of[at] = (int)n;
+    }
+    __syncthreads();
+    if (!pack) continue;
+    const int64_t here = min((int64_t)kPackThreads, last - c);
+    for (int64_t e = tid; e < here * vecs; e += kPackThreads) {
+      const int r = (int)(e / vecs);
+      const int64_t col = (e - r * vecs) * 8;
+      if (place[r] >= 0)
+        *reinterpret_cast<uint4*>(p.xp + place[r] * p.ldp + col) = *reinterpret_cast<const uint4*>(p.x + (c + r) * p.ldx + col);
+      else if (p.dx)
+        *reinterpret_cast<uint4*>(p.dx + (c + r) * p.lddx + col) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  // the rest of the last block of 64 rows that dw sums over: G is 0 there, and x must not be infinite
+  if (pack && blockIdx.x == gridDim.x - 1) {
+    const int64_t rest = min(p.tokens, (int64_t)(total + TK - 1) / TK * TK) - total;
+    for (int64_t e = tid; e < rest * vecs; e += kPackThreads)
+      *reinterpret_cast<uint4*>(p.xp + (total + e / vecs) * p.ldp + e % vecs * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // ------------------------------------------------------------------- host
@@ -533,12 +659,15 @@ int tile_width(int64_t m, int64_t n, int splits, int step, int units) {
   return best;
 }
 
-// One product: a.m x b.n over k.  K-major operands have k columns, MN-major ones k rows.
+// One product: a.m x b.n over k.  K-major operands have k columns, MN-major ones k rows.  xp: the packed rows of x
+// (A of G, B of dw), where the product has a choice.
 template <int CG, bool A_MN, bool B_MN, int EPI>
-int gemm_on(const Matrix& a, const Matrix& b, const CUtensorMap& tc, Args p, cudaStream_t s) {
+int gemm_on(const Matrix& a, const Matrix& b, const CUtensorMap& tc, const Matrix& xp, Args p, cudaStream_t s) {
   using L = Layout<CG, EPI>;
   p.tile_n = tile_width(p.m, p.n, p.splits, EPI == kStats && !B_MN ? 32 : 64 * CG, sms() / CG);
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, tx{};
+  if (xp.p)
+    if (int st = map2d(&tx, xp, 64, A_MN ? 64 : 128)) return st;
   if (int st = map2d(&ta, a, 64, A_MN ? 64 : 128)) return st;
   if (int st = map2d(&tb, b, 64, B_MN ? 64 : p.tile_n / CG)) return st;
   p.err = device_error_flag();
@@ -547,27 +676,30 @@ int gemm_on(const Matrix& a, const Matrix& b, const CUtensorMap& tc, Args p, cud
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem))
     return cuda_status(e, "linear cross entropy: smem attribute");
   const int64_t tiles = div_up(p.m, 128 * CG) * div_up(p.n, p.tile_n) * p.splits;
-  return launch(kernel, CG * std::min<int64_t>(tiles, sms() / CG), THREADS, L::kSmem, CG, s, ta, tb, tc, p);
+  return launch(kernel, CG * std::min<int64_t>(tiles, sms() / CG), THREADS, L::kSmem, CG, s, ta, tb, tc, tx, p);
 }
 
 template <bool A_MN, bool B_MN, int EPI>
-int gemm(const Matrix& a, const Matrix& b, const CUtensorMap& tc, const Args& p, cudaStream_t s) {
-  return cta_group(p.m) == 1 ? gemm_on<1, A_MN, B_MN, EPI>(a, b, tc, p, s) : gemm_on<2, A_MN, B_MN, EPI>(a, b, tc, p, s);
+int gemm(const Matrix& a, const Matrix& b, const CUtensorMap& tc, const Matrix& xp, const Args& p, cudaStream_t s) {
+  return cta_group(p.m) == 1 ? gemm_on<1, A_MN, B_MN, EPI>(a, b, tc, xp, p, s)
+                             : gemm_on<2, A_MN, B_MN, EPI>(a, b, tc, xp, p, s);
 }
 
 // ... whose result goes to bf16, or to f32 shares [splits][m][n] when acc is given.
 template <bool A_MN, bool B_MN>
-int gemm_out(const Matrix& a, const Matrix& b, const Matrix& out, float* acc, const Args& p, cudaStream_t s) {
+int gemm_out(const Matrix& a, const Matrix& b, const Matrix& out, float* acc, const Matrix& xp, Args p, cudaStream_t s) {
   CUtensorMap tc;
   if (!acc) {
     if (int st = map2d(&tc, out, 64, 32)) return st;
-    return gemm<A_MN, B_MN, kOut>(a, b, tc, p, s);
+    p.out = static_cast<__nv_bfloat16*>(const_cast<void*>(out.p));
+    p.ldo = out.ld;
+    return gemm<A_MN, B_MN, kOut>(a, b, tc, xp, p, s);
   }
   const uint64_t dims[4] = {(uint64_t)p.n, (uint64_t)p.m, (uint64_t)p.splits, 1};
   const uint64_t str[3] = {(uint64_t)p.n * 4, (uint64_t)(p.m * p.n) * 4, (uint64_t)(p.m * p.n) * 4};
   const uint32_t box[4] = {32, 32, 1, 1};
   if (int st = encode_tma_4d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, acc, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return st;
-  return gemm<A_MN, B_MN, kSum>(a, b, tc, p, s);
+  return gemm<A_MN, B_MN, kSum>(a, b, tc, xp, p, s);
 }
 
 constexpr int64_t kAlign = 256;
@@ -614,7 +746,8 @@ void split_k(Args& p, int64_t k) {
 struct BwdPlan {
   int64_t piece, pieces;  // vocabulary entries per piece
   int dx_splits, dw_splits;
-  int64_t unit, dx_acc, dw_acc, bytes;
+  int64_t ldp;            // row distance of the packed x
+  int64_t state, unit, xp, target, lse, dloss, token_of, dx_acc, dw_acc, bytes;
 };
 // G of one piece: at most this many bytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
@@ -634,8 +767,19 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   split_k(a, tokens);
   b.dw_splits = a.splits;
   int64_t at = up256(tokens * b.piece * 2);
-  b.unit = at;
-  at += kAlign;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up256(bytes);
+    return here;
+  };
+  b.ldp = div_up(width, 64) * 64;
+  b.state = take(2 * sizeof(int));
+  b.unit = take(sizeof(float));
+  b.xp = take(tokens * b.ldp * 2);
+  b.target = take(tokens * 8);
+  b.lse = take(tokens * 4);
+  b.dloss = take(tokens * 4);
+  b.token_of = take(tokens * 4);
   b.dx_acc = at;
   if (b.dx_splits > 1 || b.pieces > 1) at += up256(b.dx_splits * tokens * width * 4);
   b.dw_acc = at;
@@ -644,8 +788,9 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   return b;
 }
 
-int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, void* out, int64_t ldo, cudaStream_t s) {
-  return launch(linear_ce_join_kernel, div_up(m * n, 1024), 256, 0, 1, s, acc, splits, m, n, unit,
+int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state, const int* token_of,
+         void* out, int64_t ldo, cudaStream_t s) {
+  return launch(linear_ce_join_kernel, div_up(m * n, 1024), 256, 0, 1, s, acc, splits, m, n, unit, state, token_of,
                 static_cast<__nv_bfloat16*>(out), ldo);
 }
 
@@ -667,6 +812,8 @@ extern "C" int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream) 
   if (d->tokens == 0) return PDB_OK;
   if (!d->x || !d->w || !d->target || (!d->loss && !d->lse))
     return set_error(PDB_ERR_ARG, "linear cross entropy: null x / w / target, or neither loss nor lse");
+  if (!a16(d->x) || !a16(d->w))
+    return set_error(PDB_ERR_ALIGN, "linear cross entropy: x and w must be 16-byte aligned");
   const FwdPlan f = plan_fwd(d->tokens, d->vocab);
   if (!d->workspace || d->workspace_bytes < (size_t)f.bytes || !a16(d->workspace))
     return set_error(PDB_ERR_ARG, "linear cross entropy: workspace too small or not 16-byte aligned");
@@ -679,12 +826,11 @@ extern "C" int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream) 
   p.splits = 1;
   p.kb_split = (int)div_up(d->width, TK);
   p.target = d->target;
-  p.ignore = d->ignore_index;
   p.vocab = d->vocab;
   p.part = reinterpret_cast<float2*>(ws);
   p.tlogit = reinterpret_cast<float*>(ws + f.tlogit);
   const Matrix x{d->x, d->tokens, d->width, d->x_stride}, w{d->w, d->vocab, d->width, d->w_stride};
-  if (int st = gemm<false, false, kStats>(x, w, CUtensorMap{}, p, s)) return st;
+  if (int st = gemm<false, false, kStats>(x, w, CUtensorMap{}, Matrix{}, p, s)) return st;
   return launch(linear_ce_finish_kernel, div_up(d->tokens, 32), 32 * kFinishWarps, 0, 1, s, p.part, f.parts, p.tlogit,
                 d->target, d->tokens, d->vocab, d->ignore_index, d->loss, d->lse);
 }
@@ -709,6 +855,8 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
   }
   if (!d->x || !d->w || !d->target || !d->lse || !d->dloss)
     return set_error(PDB_ERR_ARG, "linear cross entropy: null x / w / target / lse / dloss");
+  if (!a16(d->x) || !a16(d->w))
+    return set_error(PDB_ERR_ALIGN, "linear cross entropy: x and w must be 16-byte aligned");
   const BwdPlan b = plan_bwd(d->tokens, d->vocab, d->width);
   if (!d->workspace || d->workspace_bytes < (size_t)b.bytes || !a16(d->workspace))
     return set_error(PDB_ERR_ARG, "linear cross entropy: workspace too small or not 16-byte aligned");
@@ -716,7 +864,32 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
   float* dx_acc = reinterpret_cast<float*>(ws + b.dx_acc);
   float* dw_acc = reinterpret_cast<float*>(ws + b.dw_acc);
   float* unit = reinterpret_cast<float*>(ws + b.unit);
-  const Matrix x{d->x, d->tokens, d->width, d->x_stride};
+  int* state = reinterpret_cast<int*>(ws + b.state);
+  int* token_of = reinterpret_cast<int*>(ws + b.token_of);
+  const Matrix x{d->x, d->tokens, d->width, d->x_stride}, xp{ws + b.xp, d->tokens, d->width, b.ldp};
+  Pack k{};
+  k.x = static_cast<const __nv_bfloat16*>(d->x);
+  k.target = d->target;
+  k.lse = d->lse;
+  k.dloss = d->dloss;
+  k.tokens = d->tokens;
+  k.width = d->width;
+  k.ldx = d->x_stride;
+  k.dloss_stride = d->dloss_stride;
+  k.ignore = d->ignore_index;
+  k.rows = (int)div_up(d->tokens, 2 * sms());
+  k.pack = d->width % 64 != 0;
+  k.xp = reinterpret_cast<__nv_bfloat16*>(ws + b.xp);
+  k.ldp = b.ldp;
+  k.targetp = reinterpret_cast<int64_t*>(ws + b.target);
+  k.lsep = reinterpret_cast<float*>(ws + b.lse);
+  k.dlossp = reinterpret_cast<float*>(ws + b.dloss);
+  k.token_of = token_of;
+  k.state = state;
+  k.unit = unit;
+  k.dx = static_cast<__nv_bfloat16*>(d->dx);
+  k.lddx = d->dx_stride;
+  if (int st = launch(linear_ce_pack_kernel, div_up(d->tokens, k.rows), kPackThreads, 0, 1, s, k)) return st;
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, d->vocab - v0);
     const Matrix w{static_cast<const __nv_bfloat16*>(d->w) + v0 * d->w_stride, nv, d->width, d->w_stride};
@@ -727,30 +900,31 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
     p.k = d->width;
     p.splits = 1;
     p.kb_split = (int)div_up(d->width, TK);
-    p.target = d->target;
+    p.state = state;
+    p.dyn = 1;
+    p.target = k.targetp;
     p.col0 = v0;
-    p.ignore = d->ignore_index;
     p.vocab = d->vocab;
-    p.lse = d->lse;
-    p.dloss = d->dloss;
-    p.dloss_stride = d->dloss_stride;
+    p.lse = k.lsep;
+    p.dloss = k.dlossp;
     p.unit = unit;
     CUtensorMap tc;
     if (int st = map2d(&tc, g, 64, 32)) return st;
-    if (int st = gemm<false, false, kDlogits>(x, w, tc, p, s)) return st;
+    if (int st = gemm<false, false, kDlogits>(x, w, tc, xp, p, s)) return st;
     if (d->dw) {
       Args q{};
       q.m = nv;
       q.n = d->width;
       q.k = d->tokens;
-      q.kb_split = (int)div_up(div_up(q.k, TK), b.dw_splits);
-      q.splits = (int)div_up(div_up(q.k, TK), q.kb_split);
+      q.splits = b.dw_splits;
+      q.state = state;
+      q.dyn = 2;
       q.unit = unit;
       const Matrix dw{static_cast<__nv_bfloat16*>(d->dw) + v0 * d->dw_stride, nv, d->width, d->dw_stride};
       float* acc = b.dw_splits > 1 ? dw_acc : nullptr;
-      if (int st = gemm_out<true, true>(g, x, dw, acc, q, s)) return st;
+      if (int st = gemm_out<true, true>(g, x, dw, acc, xp, q, s)) return st;
       if (acc)
-        if (int st = join(acc, q.splits, q.m, q.n, unit, const_cast<void*>(dw.p), dw.ld, s)) return st;
+        if (int st = join(acc, q.splits, q.m, q.n, unit, nullptr, nullptr, const_cast<void*>(dw.p), dw.ld, s)) return st;
     }
     if (d->dx) {
       Args q{};
@@ -760,13 +934,16 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
       // every piece takes at most the first one's number of shares, and adds to their sums
       q.kb_split = (int)div_up(div_up(nv, TK), b.dx_splits);
       q.splits = (int)div_up(div_up(nv, TK), q.kb_split);
+      q.state = state;
+      q.dyn = 1;
+      q.token_of = token_of;
       q.unit = unit;
       q.add = i > 0;
       const Matrix dx{d->dx, d->tokens, d->width, d->dx_stride};
-      if (int st = gemm_out<false, true>(g, w, dx, b.dx_splits > 1 || b.pieces > 1 ? dx_acc : nullptr, q, s)) return st;
+      if (int st = gemm_out<false, true>(g, w, dx, b.dx_splits > 1 || b.pieces > 1 ? dx_acc : nullptr, Matrix{}, q, s)) return st;
     }
   }
   if (d->dx && (b.dx_splits > 1 || b.pieces > 1))
-    return join(dx_acc, b.dx_splits, d->tokens, d->width, unit, d->dx, d->dx_stride, s);
+    return join(dx_acc, b.dx_splits, d->tokens, d->width, unit, state, token_of, d->dx, d->dx_stride, s);
   return PDB_OK;
 }

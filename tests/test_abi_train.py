@@ -162,7 +162,9 @@ def test_linear_cross_entropy_refusals():
                 assert size(C.byref(d)) == 0
     assert lib.pdb_linear_ce_fwd(C.byref(_ce(loss=None, lse=None)), None) == _lib.PDB_ERR_ARG
     assert lib.pdb_linear_ce_bwd(C.byref(_ce_bwd(dx=None, dw=None)), None) == _lib.PDB_ERR_ARG
-    for kw in ({"dx": 8}, {"dw": 8}, {"dx_stride": 68}, {"dw_stride": 56}):
+    for kw in ({"x": 8}, {"w": 40}):
+        assert lib.pdb_linear_ce_fwd(C.byref(_ce(**kw)), None) == _lib.PDB_ERR_ALIGN, kw
+    for kw in ({"x": 8}, {"w": 40}, {"dx": 8}, {"dw": 8}, {"dx_stride": 68}, {"dw_stride": 56}):
         assert lib.pdb_linear_ce_bwd(C.byref(_ce_bwd(**kw)), None) == _lib.PDB_ERR_ALIGN, kw
     for d, run, size in ((_ce(), lib.pdb_linear_ce_fwd, lib.pdb_linear_ce_fwd_workspace_size),
                          (_ce_bwd(), lib.pdb_linear_ce_bwd, lib.pdb_linear_ce_bwd_workspace_size)):
@@ -187,16 +189,20 @@ def test_linear_cross_entropy_workspaces():
     """The gradient's workspace is one piece of G (at most 512 MiB, or 256 columns) and f32 sums of dx, where they are
     shared or in pieces; the largest sizes stay within 64 bits."""
     lib = _lib.load()
+    al = lambda n: (n + 255) // 256 * 256
 
     def need(tokens, vocab, width):
         kw = dict(tokens=tokens, vocab=vocab, width=width, x_stride=width, w_stride=width)
         assert lib.pdb_linear_ce_fwd_workspace_size(C.byref(_ce(**kw))) >= 8 * 4 * -(-vocab // 256) * tokens
         return lib.pdb_linear_ce_bwd_workspace_size(C.byref(_ce_bwd(dx_stride=width, dw_stride=width, **kw)))
 
-    assert need(8192, 128000, 4096) == 8192 * 32000 * 2 + 256 + 4 * 8192 * 4096  # four pieces of 32000
-    assert need(8192, 32000, 4096) == 8192 * 32000 * 2 + 256  # one
-    assert need(1 << 24, 1 << 24, 1 << 16) == (1 << 24) * 256 * 2 + 256 + 4 * (1 << 40)
-    assert need(1, 1, 8) == 256 + 256
+    def rows(tokens, width):  # the packed tokens: rows of x, target, lse, dloss and index, behind count and unit
+        return 512 + al(tokens * ((width + 63) // 64) * 128) + al(tokens * 8) + 3 * al(tokens * 4)
+
+    assert need(8192, 128000, 4096) == 8192 * 32000 * 2 + rows(8192, 4096) + 4 * 8192 * 4096  # four pieces of 32000
+    assert need(8192, 32000, 4096) == 8192 * 32000 * 2 + rows(8192, 4096)  # one
+    assert need(1 << 24, 1 << 24, 1 << 16) == (1 << 24) * 256 * 2 + rows(1 << 24, 1 << 16) + 4 * (1 << 40)
+    assert need(1, 1, 8) == 256 + 512 + 5 * 256
 
 
 def test_host_tensors_are_refused():

@@ -162,8 +162,8 @@ def test_nothing_to_do(cuda):
     assert (dx == 0).all() and (dw == 0).all()
     x[3] = float("inf")  # in an ignored row: no gradient still
     _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
-    dx, _ = kernels.linear_cross_entropy_backward(x, w, t, dl, lse, need_dweight=False)
-    assert (dx == 0).all()
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    assert (dx == 0).all() and (dw == 0).all()
     none = x[:0]
     loss, lse = kernels.linear_cross_entropy(none, w, t[:0], return_lse=True)
     dx, dw = kernels.linear_cross_entropy_backward(none, w, t[:0], dl[:0], lse)
@@ -275,3 +275,39 @@ def test_a_mean_does_not_scale_the_gradient(cuda, n):
     ref = (p @ w.double() - w[t].double()) / n
     slope = (dx.double() * ref).sum() / (ref * ref).sum()
     assert abs(slope - 1) <= 4 * 2.0 ** -8 / (512 * 64) ** 0.5 + 1 / 20000
+
+
+@pytest.mark.parametrize("N,V,W,count", [(300, 700, 72, 1), (300, 700, 72, 33), (300, 700, 72, 64), (300, 700, 72, 299),
+                                         (513, 20000, 256, 255), (2000, 300, 64, 129), (700, 40000, 40, 350), (40, 700, 64, 7)])
+def test_ignored_tokens_hold_anything(cuda, N, V, W, count):
+    """Infinities and NaN in the rows, lse and dloss of ignored tokens (a padded batch) reach no gradient, for counts that
+    end inside and on the products' blocks; the gradients are those of the remaining tokens alone."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, N, V, W, N + count, ignored=0.0)
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    keep = torch.zeros(N, dtype=torch.bool, device=cuda)
+    keep[torch.randperm(N, generator=torch.Generator().manual_seed(count))[:count].to(cuda)] = True
+    t = torch.where(keep, t, IGN)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    _check_backward(x, w, t, dl, lse, dx, dw)
+    x2, lse2, dl2 = x.clone(), lse.clone(), dl.clone()
+    for value in (float("nan"), float("inf"), -float("inf")):
+        x2[~keep], lse2[~keep], dl2[~keep] = value, value, value
+        dx2, dw2 = kernels.linear_cross_entropy_backward(x2, w, t, dl2, lse2)
+        assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
+    loss = kernels.linear_cross_entropy(x2, w, t)
+    assert (loss[~keep] == 0).all() and loss.isfinite().all()
+    kernels.check_device_errors()
+
+
+def test_ignored_tokens_over_several_pieces(cuda):
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 8200, 70001, 24, 12, ignored=0.4)
+    _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+    kernels.check_device_errors()
+    _check_backward(x, w, t, dl, lse, dx, dw)

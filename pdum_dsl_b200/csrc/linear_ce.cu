@@ -84,19 +84,18 @@ struct __align__(8) Bars {
 static_assert(sizeof(Bars) <= 256, "the barriers' share of shared memory");
 
 // Tile t -> (split, m0, n0): groups of `group` m tiles sweep the n tiles, odd groups backwards, so the tiles
-// in flight share operands in L2.
+// in flight share operands in L2.  In 32 bits: every epilogue warp does this for every tile.
 template <int TM>
-__device__ __forceinline__ void tile_at(const Args& p, int tm, int tn, int64_t t, int& split, int64_t& m0, int64_t& n0) {
-  const int64_t per = (int64_t)tm * tn;
+__device__ __forceinline__ void tile_at(const Args& p, uint32_t tm, uint32_t tn, uint32_t t, int& split, int& m0, int& n0) {
+  const uint32_t per = tm * tn;
   split = (int)(t / per);
-  const int64_t r = t - split * per;
-  const int64_t gsz = (int64_t)p.group * tn;
-  const int grp = (int)(r / gsz);
-  const int in = (int)(r - grp * gsz);
-  const int rows = min(tm - grp * p.group, p.group);
-  const int nt = in / rows;
-  m0 = (int64_t)(grp * p.group + in % rows) * TM;
-  n0 = (int64_t)((grp & 1) ? tn - 1 - nt : nt) * p.tile_n;
+  const uint32_t r = t - split * per;
+  const uint32_t gsz = p.group * tn;
+  const uint32_t grp = r / gsz, in = r - grp * gsz;
+  const uint32_t rows = min(tm - grp * p.group, (uint32_t)p.group);
+  const uint32_t nt = in / rows;
+  m0 = (int)(grp * p.group + in - nt * rows) * TM;
+  n0 = (int)((grp & 1) ? tn - 1 - nt : nt) * p.tile_n;
 }
 
 // One row's 32 logits of a chunk folded into its running maximum and its sum of 2^(logit log2e - base).  The maximum
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   const int nk = (int)((k + TK - 1) / TK), kb_split = p.dyn == 2 ? (nk + p.splits - 1) / p.splits : p.kb_split;
   const int tm = (int)((m + TM - 1) / TM), tn = (int)((p.n + p.tile_n - 1) / p.tile_n);
-  const int64_t num_tiles = (int64_t)tm * tn * p.splits;
+  const int num_tiles = tm * tn * p.splits;  // the host saw to it that they are fewer than 2^31
 
   if (warp == 0 && lane == 0) {
     const int b_rows = p.tile_n / CG;  // of B per CTA
@@ -197,12 +196,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t bytes = CG * (kTileA + b_rows * TK * 2);
     uint32_t g = 0;
     bool ok = true;
-    for (int64_t t = unit_id; ok && t < num_tiles; t += units) {
-      int split;
-      int64_t m0, n0;
+    for (int t = unit_id; ok && t < num_tiles; t += units) {
+      int split, m0, n0;
       tile_at<TM>(p, tm, tn, t, split, m0, n0);
       const int kb0 = split * kb_split, kb1 = min(nk, kb0 + kb_split);
-      const int ma = (int)m0 + (int)rank * 128, nb = (int)n0 + (int)rank * b_rows;
+      const int ma = m0 + (int)rank * 128, nb = n0 + (int)rank * b_rows;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
         const int st = g % STAGES;
         if (!(ok = wait_bar<CG>(&bar->empty[st], ((g / STAGES) & 1) ^ 1, abort, p.err))) break;
@@ -234,8 +232,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? kBox : 16;
     uint32_t g = 0, tt = 0;
     bool ok = true;
-    for (int64_t t = unit_id; ok && t < num_tiles; t += units, ++tt) {
-      const int split = (int)(t / ((int64_t)tm * tn));
+    for (int t = unit_id; ok && t < num_tiles; t += units, ++tt) {
+      const int split = (int)((uint32_t)t / (uint32_t)(tm * tn));
       const int kb0 = split * kb_split, kb1 = min(nk, kb0 + kb_split);
       const int buf = tt & 1;
       if (!(ok = wait_bar<CG>(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
@@ -277,35 +275,41 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t stage = smem_u32(sC + e * kStore), srow = stage + lane * 128;
     float unit = 1.f;
     if constexpr (EPI == kDlogits || EPI == kOut) unit = *p.unit;
+    // a row's target, lse and dloss, read while the tile before is worked on
+    int64_t next_target = -1;
+    float next_lse = 0.f, next_dloss = 0.f;
+    auto look = [&](int t) {
+      if constexpr (EPI == kStats || EPI == kDlogits) {
+        if (t >= num_tiles) return;
+        int split, m0, n0;
+        tile_at<TM>(p, tm, tn, t, split, m0, n0);
+        const int row = m0 + row0 + lane;
+        if (row >= m) return;
+        next_target = p.target[row];
+        if constexpr (EPI == kDlogits) next_lse = p.lse[row], next_dloss = p.dloss[row];
+      }
+    };
+    look(unit_id);
     uint32_t tt = 0;
-    for (int64_t t = unit_id; t < num_tiles; t += units, ++tt) {
-      int split;
-      int64_t m0, n0;
+    for (int t = unit_id; t < num_tiles; t += units, ++tt) {
+      int split, m0, n0;
       tile_at<TM>(p, tm, tn, t, split, m0, n0);
       const int buf = tt & 1;
-      const int64_t gm = m0 + row0 + lane;
+      const int64_t gm = m0 + row0 + lane;  // rows and columns are below 2^25
       const bool live = gm < m;
       const bool none = split * kb_split >= nk;  // a share of the contracted index without any of it
-      int64_t tgt = -1;
-      float nlse = 0.f, up = 0.f;
-      if constexpr (EPI == kStats || EPI == kDlogits) {
-        if (live) {
-          tgt = p.target[gm];
-          if constexpr (EPI == kDlogits) {
-            nlse = -p.lse[gm] * kLog2e;
-            up = p.dloss[gm] / unit;
-            if (tgt < 0 || tgt >= p.vocab) up = NAN;  // no such entry: the gradient says so
-          }
-          tgt -= p.col0;
-        }
-      }
+      const int64_t tgt = live ? next_target - p.col0 : -1;
+      const float nlse = -next_lse * kLog2e;
+      float up = next_dloss / unit;
+      if (next_target < 0 || next_target >= p.vocab) up = NAN;  // no such entry: the gradient says so
+      look(t + units);
       if (!wait_bar<CG>(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
       tc_fence_after();
       float base = -INFINITY, sum = 0.f;
 #pragma unroll 1
       for (int ch = 0; ch < 2; ++ch) {
         const int c = cg * 64 + ch * 32;  // the tile's column
-        const int64_t c0 = n0 + c;
+        const int c0 = n0 + c;
         if (c >= p.tile_n || c0 >= p.n) break;  // the whole warp
         uint32_t r[32];
         __syncwarp();
@@ -341,8 +345,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && m0 + row0 < m) {
-            if (p.add) tma_reduce_add_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
-            else tma_store_4d(&tm_c, stage, (int)c0, (int)m0 + row0, split, 0);
+            if (p.add) tma_reduce_add_4d(&tm_c, stage, c0, m0 + row0, split, 0);
+            else tma_store_4d(&tm_c, stage, c0, m0 + row0, split, 0);
             bulk_commit();
           }
         } else {
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (row < m && col < p.n) *reinterpret_cast<uint4*>(p.out + p.token_of[row] * p.ldo + col) = q;
             }
           } else if (lane == 0) {
-            tma_store_4d(&tm_c, stage, (int)n0 + cg * 64, (int)m0 + row0, 0, 0);
+            tma_store_4d(&tm_c, stage, n0 + cg * 64, m0 + row0, 0, 0);
             bulk_commit();
           }
         }
@@ -468,19 +472,44 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
   }
 }
 
-// The f32 shares of a product, added in order, scaled and rounded; packed rows go to their tokens' rows.
-__global__ void __launch_bounds__(256)
+// The f32 shares of a product, added in a fixed order, scaled and rounded; packed rows go to their tokens' rows.
+// GROUPS threads share an element's shares (one after another, 135 shares of a small product took 38 us).
+constexpr int kJoinThreads = 256;
+
+template <int GROUPS>
+__global__ void __launch_bounds__(kJoinThreads)
     linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state,
                           const int* token_of, __nv_bfloat16* out, int64_t ldo) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // n is a multiple of 8
+  constexpr int EACH = kJoinThreads / GROUPS, FLIGHT = 8;
+  __shared__ float4 red[GROUPS][EACH];
+  const int group = threadIdx.x / EACH, l = threadIdx.x % EACH;
+  const int64_t i = ((int64_t)blockIdx.x * EACH + l) * 4;  // n is a multiple of 8
   grid_dep_wait();
-  if (i >= (state ? *state : m) * n) return;
-  float4 s = *reinterpret_cast<const float4*>(acc + i);
-#pragma unroll 4
-  for (int k = 1; k < splits; ++k) {
-    const float4 q = *reinterpret_cast<const float4*>(acc + (int64_t)k * m * n + i);
-    s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+  const bool live = i < (state ? *state : m) * n;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    for (int k = group; k < splits; k += FLIGHT * GROUPS) {
+      float4 q[FLIGHT];
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u) {
+        const int at = k + u * GROUPS;
+        q[u] = at < splits ? *reinterpret_cast<const float4*>(acc + (int64_t)at * m * n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u) s.x += q[u].x, s.y += q[u].y, s.z += q[u].z, s.w += q[u].w;
+    }
   }
+  if constexpr (GROUPS > 1) {
+    red[group][l] = s;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) {
+      const float4 q = red[g][l];
+      s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+    }
+  }
+  if (!live) return;
   const float u = *unit;
   uint2 o = make_uint2(pack_bf16(s.x * u, s.y * u), pack_bf16(s.z * u, s.w * u));
   const int64_t row = i / n;
@@ -641,8 +670,12 @@ int launch(void (*kernel)(Params...), int64_t grid, int threads, int smem, int c
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, std::forward<Given>(args)...), "linear cross entropy launch");
 }
 
-// Tiles of at most 128 rows run on single CTAs: a pair would spend half of its products on rows that are not there.
-int cta_group(int64_t m) { return m <= 128 ? 1 : 2; }
+// A pair's tile has 256 rows: where they end in an odd block of 128, and few come before it, single CTAs waste less than
+// they lose by reading B alone (300 x 32000 x 2048: 49 us against 60 on pairs; 640: 73 against 83; 256: 56 against 53).
+int cta_group(int64_t m) {
+  const int64_t blocks = div_up(m, 128);
+  return blocks % 2 == 1 && blocks <= 7 ? 1 : 2;
+}
 
 // The tile's width: of the multiples of `step`, the one whose waves of tiles load least, since operand rows into shared
 // memory (the tile's rows and its columns) are what a step costs: at 1024 x 50176 x 1024, 17 waves of 160 columns took
@@ -676,6 +709,7 @@ int gemm_on(const Matrix& a, const Matrix& b, const CUtensorMap& tc, const Matri
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem))
     return cuda_status(e, "linear cross entropy: smem attribute");
   const int64_t tiles = div_up(p.m, 128 * CG) * div_up(p.n, p.tile_n) * p.splits;
+  if (tiles > 0x3fffffffLL) return set_error(PDB_ERR_SHAPE, "linear cross entropy: too many tiles");
   return launch(kernel, CG * std::min<int64_t>(tiles, sms() / CG), THREADS, L::kSmem, CG, s, ta, tb, tc, tx, p);
 }
 
@@ -790,8 +824,11 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
 
 int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state, const int* token_of,
          void* out, int64_t ldo, cudaStream_t s) {
-  return launch(linear_ce_join_kernel, div_up(m * n, 1024), 256, 0, 1, s, acc, splits, m, n, unit, state, token_of,
-                static_cast<__nv_bfloat16*>(out), ldo);
+  auto on = [&](auto kernel, int groups) {
+    return launch(kernel, div_up(m * n, 4 * kJoinThreads / groups), kJoinThreads, 0, 1, s, acc, splits, m, n, unit, state,
+                  token_of, static_cast<__nv_bfloat16*>(out), ldo);
+  };
+  return splits > 8 ? on(linear_ce_join_kernel<16>, 16) : on(linear_ce_join_kernel<1>, 1);
 }
 
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -275,15 +275,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t stage = smem_u32(sC + e * kStore), srow = stage + lane * 128;
     float unit = 1.f;
     if constexpr (EPI == kDlogits || EPI == kOut) unit = *p.unit;
-    // a row's target, lse and dloss, read while the tile before is worked on
+    // the next tile's place and its rows' targets, lse and dloss, found while the tile before is worked on
+    int next_split = 0, next_m0 = 0, next_n0 = 0;
     int64_t next_target = -1;
     float next_lse = 0.f, next_dloss = 0.f;
     auto look = [&](int t) {
+      if (t >= num_tiles) return;
+      tile_at<TM>(p, tm, tn, t, next_split, next_m0, next_n0);
       if constexpr (EPI == kStats || EPI == kDlogits) {
-        if (t >= num_tiles) return;
-        int split, m0, n0;
-        tile_at<TM>(p, tm, tn, t, split, m0, n0);
-        const int row = m0 + row0 + lane;
+        const int row = next_m0 + row0 + lane;
         if (row >= m) return;
         next_target = p.target[row];
         if constexpr (EPI == kDlogits) next_lse = p.lse[row], next_dloss = p.dloss[row];
@@ -292,8 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     look(unit_id);
     uint32_t tt = 0;
     for (int t = unit_id; t < num_tiles; t += units, ++tt) {
-      int split, m0, n0;
-      tile_at<TM>(p, tm, tn, t, split, m0, n0);
+      const int split = next_split, m0 = next_m0, n0 = next_n0;
       const int buf = tt & 1;
       const int64_t gm = m0 + row0 + lane;  // rows and columns are below 2^25
       const bool live = gm < m;

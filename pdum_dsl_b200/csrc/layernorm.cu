@@ -112,6 +112,29 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int slot, int
   }
 }
 
+// ... and over the CL blocks of a cluster that share a row: each leaves its sums in every block's shared memory.  The
+// buffers alternate as above: one is written again only after the barrier of the sum between.
+template <int CL, int N>
+__device__ __forceinline__ void cluster_sum(float (&v)[N], float* sums, int rank, int& phase) {
+  if constexpr (CL > 1) {
+    float* buf = sums + phase * CL * N;
+    phase ^= 1;
+    if (threadIdx.x < CL) {
+      const uint32_t dst = mapa_shared(smem_u32(buf + rank * N), threadIdx.x);
+#pragma unroll
+      for (int n = 0; n < N; ++n) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4 * n), "f"(v[n]) : "memory");
+    }
+    cluster_sync_all();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < CL; ++c) s += buf[c * N + n];
+      v[n] = s;
+    }
+  }
+}
+
 // The N elements that a thread holds of a row as N / 2 pairs, so that the arithmetic
 // runs on two elements per instruction (with scalar arithmetic both directions were
 // bound by instructions, not by memory: 33 per element in the backward pass).
@@ -136,10 +159,73 @@ __device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, VEC> (&raw)[NV]
     }
   }
 }
-// first: the column of the thread's first element; the vectors lie `step` columns apart.  RAG: a vector may begin
-// before the row or end behind it.
+// Where a ragged row begins and ends within its 16-byte vectors: `shift` elements of the first one lie before the row,
+// `tail` elements of the last one (its number `tail_i` of thread `tail_l`) are the row's.  All alike for the rows of a
+// block, so what is done about them branches with the block; only two threads of a row hold such vectors.
+template <int VEC>
+struct Edges {
+  int shift, tail;
+  bool head;    // this thread's first vector begins before the row
+  int tail_at;  // the number of this thread's vector that the row ends in (-1: none, or at its end)
+  uint32_t keep[VEC >= 4 ? 4 : 1];  // the first vector's bits that are the row's
+};
+
+template <typename T, int VEC, int NV, int TPR>
+__device__ __forceinline__ Edges<VEC> find_edges(int shift, int cols, int l, int rank) {
+  Edges<VEC> e;
+  const int last = (cols + shift - 1) / VEC, mine = rank * NV * TPR + l;  // vectors of the row, of this thread
+  e.shift = shift;
+  e.tail = cols + shift - last * VEC;
+  e.head = mine == 0 && shift > 0;
+  e.tail_at = e.tail < VEC && last >= mine && (last - mine) % TPR == 0 && (last - mine) / TPR < NV ? (last - mine) / TPR : -1;
+  constexpr int per = 4 / sizeof(T);  // elements per word
+#pragma unroll
+  for (int w = 0; w < 4 && VEC >= 4; ++w) {
+    const int dead = shift - w * per;  // of this word's elements
+    e.keep[w] = !e.head || dead <= 0 ? ~0u : dead >= per ? 0u : 0xffff0000u;
+  }
+  return e;
+}
+
+// The part of an edge vector that is the row's, in as few aligned stores as it has binary digits.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_edge(T* at, const Pack<T, VEC>& o, bool head, bool tail, const Edges<VEC>& e) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&o);
+  if (head && tail) {  // a row within one vector
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (j >= e.shift && j < e.tail) at[j] = o.v[j];
+  } else if (sizeof(T) == 4) {
+    if (head) {
+      if (e.shift & 1) at[e.shift] = e.shift == 1 ? o.v[1] : o.v[VEC - 1];
+      if (e.shift <= 2) *reinterpret_cast<uint2*>(at + 2) = make_uint2(w[2], w[3]);
+    } else {
+      if (e.tail >= 2) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+      if (e.tail & 1) at[e.tail - 1] = e.tail == 1 ? o.v[0] : o.v[2 % VEC];
+    }
+  } else {
+    uint32_t* at32 = reinterpret_cast<uint32_t*>(at);
+    if (head) {
+      const int odd = e.shift >> 1, first = (e.shift + 1) >> 1;  // the half dead word, the first word that lives
+      const uint32_t half = odd == 0 ? w[0] : odd == 1 ? w[1] : odd == 2 ? w[2] : w[3];
+      if (e.shift & 1) reinterpret_cast<uint16_t*>(at)[e.shift] = (uint16_t)(half >> 16);
+      if (first == 1) at32[1] = w[1];
+      if (first == 3) at32[3] = w[3];
+      if (first <= 2) *reinterpret_cast<uint2*>(at32 + 2) = make_uint2(w[2], w[3]);
+    } else {
+      const int odd = e.tail >> 1;
+      const uint32_t half = odd == 0 ? w[0] : odd == 1 ? w[1] : odd == 2 ? w[2] : w[3];
+      if (e.tail >= 4) *reinterpret_cast<uint2*>(at32) = make_uint2(w[0], w[1]);
+      if (e.tail & 2) at32[e.tail >= 4 ? 2 : 0] = e.tail >= 4 ? w[2] : w[0];
+      if (e.tail & 1) reinterpret_cast<uint16_t*>(at)[e.tail - 1] = (uint16_t)half;
+    }
+  }
+}
+
+// first: the column of the thread's first element; the vectors lie `step` columns apart.
 template <typename T, int VEC, int NV, bool RAG>
-__device__ __forceinline__ void store_pairs(T* row, int first, int step, int cols, const uint64_t (&v)[NV * VEC / 2]) {
+__device__ __forceinline__ void store_pairs(T* row, int first, int step, int cols, const uint64_t (&v)[NV * VEC / 2],
+                                            const Edges<VEC>& edges) {
   Pack<T, VEC> o[NV];
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -162,12 +248,12 @@ __device__ __forceinline__ void store_pairs(T* row, int first, int step, int col
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = first + i * step;
-    if (RAG ? c >= 0 && c + VEC <= cols : c < cols) {
-      *reinterpret_cast<Pack<T, VEC>*>(row + c) = o[i];
-    } else if (RAG) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (c + j >= 0 && c + j < cols) row[c + j] = o[i].v[j];
+    if constexpr (RAG) {
+      const bool head = i == 0 && edges.head, tail = i == edges.tail_at;
+      if (head || tail) store_edge<T, VEC>(row + c, o[i], head, tail, edges);
+      else if (c < cols) *reinterpret_cast<Pack<T, VEC>*>(row + c) = o[i];
+    } else {
+      if (c < cols) *reinterpret_cast<Pack<T, VEC>*>(row + c) = o[i];
     }
   }
 }
@@ -221,8 +307,8 @@ __device__ __forceinline__ void copy_wait() {
 // `period` apart start equally far (`shift` elements) behind a 16-byte boundary, and a
 // block takes rows of one such class only: its threads own aligned vectors, the first
 // one beginning `shift` elements before the row, and the columns of a thread stay the
-// same from row to row.  (Element by element, 32768 rows of 1001 bf16 took 70 us in
-// the backward pass, and this way 45.)
+// same from row to row.  (Element by element, 32768 rows of 1001 bf16 took 76 us in
+// the backward pass, and this way 50.)
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, int NT, bool RAG>
 struct Rows {
   // cp.async moves 4 bytes at least; smaller elements come one row ahead through registers
@@ -275,7 +361,7 @@ struct Rows {
   }
   // The oldest row's elements as f32 pairs (0 outside the row), and the next fetch.  A slot is filled again a row
   // after it was read.
-  __device__ __forceinline__ void take(uint64_t (&v)[NT][NV * VEC / 2]) {
+  __device__ __forceinline__ void take(uint64_t (&v)[NT][NV * VEC / 2], const Edges<VEC>& edges) {
     if constexpr (kAsync) copy_wait<STAGES - 2>();
     P c[NT][NV];
 #pragma unroll
@@ -283,12 +369,11 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < NV; ++i) c[n][i] = kAsync ? slots[((tail * NT + n) * NV + i) * BT + threadIdx.x] : reg[n][i];
     tail = tail + 1 == STAGES ? 0 : tail + 1;
-    if (RAG && first_col < 0) {  // the end of the row before
+    if constexpr (RAG) {  // without the end of the row before
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (first_col + j < 0) from_f32(c[n][0].v[j], 0.f);
+        for (int w = 0; w < 4; ++w) reinterpret_cast<uint32_t*>(&c[n][0])[w] &= edges.keep[w];
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) unpack(c[n], v[n]);
@@ -303,9 +388,9 @@ struct Rows {
 struct Run {
   int cls, period;
   int64_t first, last;
-  __device__ __forceinline__ Run(int64_t rows, int period_, int classes, int64_t chunk) : period(period_) {
-    cls = blockIdx.x % classes;
-    first = blockIdx.x / classes * chunk;
+  __device__ __forceinline__ Run(int64_t rows, int period_, int classes, int64_t chunk, int block) : period(period_) {
+    cls = block % classes;
+    first = block / classes * chunk;
     last = min((rows - cls + period - 1) / period, first + chunk);
   }
   __device__ __forceinline__ int64_t row(int64_t j) const { return cls + period * j; }
@@ -321,13 +406,14 @@ __device__ __forceinline__ int row_shift(const void* p, int64_t stride, int cls)
 // ---------------------------------------------------------------- forward
 // A block takes a run of rows; scale and shift stay in registers.
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
-__global__ void __launch_bounds__(BT) layernorm_fwd_kernel(const FwdArgs p) {
+__global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
   __shared__ float red[RPB * 2 * NW];
   extern __shared__ __align__(16) uint8_t dyn[];
   const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
-  const Run run(p.rows, p.period, p.classes, p.chunk);
-  const int first_col = l * VEC - row_shift<T, RAG>(p.x, p.xs, run.cls);
+  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x);
+  const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = l * VEC - shift;
+  const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, 0);
   Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG> rows;
   rows.first_col = first_col;
   rows.cols = p.cols;
@@ -340,7 +426,7 @@ __global__ void __launch_bounds__(BT) layernorm_fwd_kernel(const FwdArgs p) {
   for (int64_t j0 = run.first; j0 < run.last; j0 += RPB) {
     if (TPR >= 32 && j0 + slot >= run.last) break;  // whole warps (and whole barrier groups) leave together
     uint64_t v[1][N2];
-    rows.take(v);
+    rows.take(v, edges);
     uint64_t a = f2_pack(0.f, 0.f);
 #pragma unroll
     for (int e = 0; e < N2; ++e) a = f2_add(a, v[0][e]);
@@ -362,16 +448,17 @@ __global__ void __launch_bounds__(BT) layernorm_fwd_kernel(const FwdArgs p) {
           const uint64_t d = f2_pack(c < p.cols ? lo : 0.f, c + TPR < p.cols ? hi : 0.f);
           a = f2_fma(d, d, a);
         }
-      } else if (RAG && (c < 0 || c + VEC > p.cols)) {
-#pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          float lo, hi;
-          f2_unpack(v[0][(i * VEC + j) / 2], lo, hi);
-          const uint64_t d = f2_pack(c + j >= 0 && c + j < p.cols ? lo : 0.f, c + j + 1 >= 0 && c + j + 1 < p.cols ? hi : 0.f);
-          a = f2_fma(d, d, a);
-        }
       } else {
         uint64_t q = f2_pack(0.f, 0.f);
+        if (RAG && ((i == 0 && edges.head) || i == edges.tail_at)) {
+          const int from = i == 0 && edges.head ? edges.shift : 0, to = i == edges.tail_at ? edges.tail : VEC;
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            float lo, hi;
+            f2_unpack(v[0][(i * VEC + j) / 2], lo, hi);
+            v[0][(i * VEC + j) / 2] = f2_pack(j >= from && j < to ? lo : 0.f, j + 1 >= from && j + 1 < to ? hi : 0.f);
+          }
+        }
 #pragma unroll
         for (int j = i * VEC / 2; j < (i + 1) * VEC / 2; ++j) q = f2_fma(v[0][j], v[0][j], q);
         if (c < p.cols) a = f2_add(a, q);
@@ -389,7 +476,7 @@ __global__ void __launch_bounds__(BT) layernorm_fwd_kernel(const FwdArgs p) {
       const uint64_t r2 = f2_pack(rstd, rstd);
 #pragma unroll
       for (int e = 0; e < N2; ++e) v[0][e] = f2_fma(f2_mul(v[0][e], r2), g[e], b[e]);
-      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.y) + row * p.ys, first_col, TPR * VEC, p.cols, v[0]);
+      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.y) + row * p.ys, first_col, TPR * VEC, p.cols, v[0], edges);
     }
   }
   rows.drain();
@@ -453,15 +540,17 @@ constexpr int bwd_smem() {
 
 // A block takes a run of rows and keeps, per thread, the sums of dy z and dy over its
 // rows for the columns that the thread owns; the row slots of the block are added in
-// shared memory at the end, one partial row per block.
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+// shared memory at the end, one partial row per block.  CL blocks share longer rows.
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL>
 __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernorm_bwd_kernel(const BwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
-  __shared__ float red[RPB * 2 * NW * 2];
+  __shared__ float red[RPB * 2 * NW * 2], sums[2 * CL * 2];
   extern __shared__ __align__(16) uint8_t dyn[];
-  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
-  const Run run(p.rows, p.period, p.classes, p.chunk);
-  const int first_col = l * VEC - row_shift<T, RAG>(p.x, p.xs, run.cls);
+  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR, rank = CL > 1 ? (int)cluster_rank() : 0;
+  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x / CL);
+  const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = (rank * NV * TPR + l) * VEC - shift;
+  const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, rank);
+  if constexpr (CL > 1) cluster_sync_all();  // every block of the cluster is there
   Rows<T, VEC, NV, TPR, BT, STAGES, 2, RAG> rows;
   rows.first_col = first_col;
   rows.cols = p.cols;
@@ -482,7 +571,7 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
   };
   float mean_w = stat(p.mean, run.first), rstd_w = stat(p.rstd, run.first);
   float mean_n = stat(p.mean, run.first + W * RPB), rstd_n = stat(p.rstd, run.first + W * RPB);
-  int phase = 0, it = 0;
+  int phase = 0, cluster_phase = 0, it = 0;
   for (int64_t j0 = run.first; j0 < run.last; j0 += RPB, ++it) {
     if (TPR >= 32 && j0 + slot >= run.last) break;
     if (it == W) {
@@ -492,7 +581,7 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
     }
     const float mean = __shfl_sync(0xffffffffu, mean_w, it, W), rstd = __shfl_sync(0xffffffffu, rstd_w, it, W);
     uint64_t v[2][N2];
-    rows.take(v);
+    rows.take(v, edges);
     auto &z = v[0], &dz = v[1];
     // z as one fused step: the rounding of mean * rstd is of the size of mean's own
     const uint64_t r2 = f2_pack(rstd, rstd), mr2 = f2_pack(-mean * rstd, -mean * rstd);
@@ -508,18 +597,20 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
     }
     float s[2] = {f2_total(s0), f2_total(s1)};
     row_sum<TPR, 2>(s, red, slot, phase);
+    cluster_sum<CL>(s, sums, rank, cluster_phase);
     const float k0 = -s[0] * p.inv_cols * rstd, k1 = -s[1] * p.inv_cols * rstd;
     const uint64_t k02 = f2_pack(k0, k0), k12 = f2_pack(k1, k1);
 #pragma unroll
     for (int e = 0; e < N2; ++e) dz[e] = f2_fma(z[e], k12, f2_fma(dz[e], r2, k02));
     if (j0 + slot < run.last)
-      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.dx) + run.row(j0 + slot) * p.dxs, first_col, TPR * VEC, p.cols, dz);
+      store_pairs<T, VEC, NV, RAG>(static_cast<T*>(p.dx) + run.row(j0 + slot) * p.dxs, first_col, TPR * VEC, p.cols, dz,
+                                   edges);
   }
   rows.drain();
   if (!p.partial) return;
   const int64_t half = (int64_t)p.groups * p.cols;
-  float* out = p.partial + (int64_t)blockIdx.x * p.cols;
-  float* sums = reinterpret_cast<float*>(dyn);  // [RPB][TPR * NV * VEC]
+  float* out = p.partial + (int64_t)(blockIdx.x / CL) * p.cols;
+  float* columns = reinterpret_cast<float*>(dyn);  // [RPB][TPR * NV * VEC]
   constexpr int WIDTH = TPR * NV * VEC;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -537,13 +628,13 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
 #pragma unroll
       for (int e = 0; e < NV * VEC; ++e) {
         const int c = first_col + e / VEC * TPR * VEC + e % VEC;
-        if (c >= 0) sums[slot * WIDTH + c] = f[e];
+        if (c >= 0) columns[slot * WIDTH + c] = f[e];
       }
       __syncthreads();
       for (int c = threadIdx.x; c < p.cols; c += BT) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < RPB; ++r) s += sums[r * WIDTH + c];
+        for (int r = 0; r < RPB; ++r) s += columns[r * WIDTH + c];
         out[which * half + c] = s;
       }
     }
@@ -679,18 +770,34 @@ int rag_period(int64_t stride) {
   return p;
 }
 
+// p.groups clusters of CL blocks
+template <typename Args>
+int launch(void (*kernel)(Args), const Args& p, int threads, int smem, int cl, cudaStream_t s) {
+  if (smem > 40 * 1024)  // with the static arrays, 48 KB would be passed
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+      return cuda_status(e, "layernorm: smem attribute"), -1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.groups * cl));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cl;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = cl > 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p)) return cuda_status(e, "layernorm launch"), -1;
+  return 1;
+}
+
 // 1: launched, 0: the row is too long for this shape, -1: an error
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
   if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC) return 0;
-  constexpr int smem = Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG>::kBytes;
-  auto kernel = layernorm_fwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>;
-  if (smem > 40 * 1024)  // with the static arrays, 48 KB would be passed
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-      return cuda_status(e, "layernorm: smem attribute"), -1;
   share_rows(p, BT / TPR, (int64_t)blocks * sms());
-  kernel<<<(unsigned)p.groups, BT, smem, s>>>(p);
-  return 1;
+  return launch(layernorm_fwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>, p, BT,
+                Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG>::kBytes, 1, s);
 }
 
 // 32 elements per thread in the forward (16 of f32), 256 threads per block and 4 blocks per SM; measured over 32 MiB
@@ -726,17 +833,12 @@ int forward(FwdArgs& p, cudaStream_t s) {
   return cuda_status(cudaGetLastError(), "layernorm forward launch");
 }
 
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL = 1>
 int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
-  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC) return 0;
-  constexpr int smem = bwd_smem<T, VEC, NV, TPR, BT, STAGES>();
-  auto kernel = layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>;
-  if (smem > 40 * 1024)
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-      return cuda_status(e, "layernorm backward: smem attribute"), -1;
-  share_rows(p, BT / TPR, (int64_t)blocks * sms());
-  kernel<<<(unsigned)p.groups, BT, smem, s>>>(p);
-  return 1;
+  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC * CL) return 0;
+  share_rows(p, BT / TPR, (int64_t)blocks * sms() / CL);
+  return launch(layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>, p, BT,
+                bwd_smem<T, VEC, NV, TPR, BT, STAGES>(), CL, s);
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
@@ -754,6 +856,10 @@ int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
   constexpr int S = sizeof(T) == 4 ? 2 : 3;
   if (!r) r = launch_bwd<T, VEC, NV, 256, VEC == 1 ? 256 : 512, S, RAG>(p, VEC == 1 ? 3 : 1, s);
   if (!r) r = launch_bwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, S, RAG>(p, 1, s);
+  if constexpr (VEC > 1) {
+    if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 2>(p, 1, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 4>(p, 1, s);
+  }
   return r;
 }
 

@@ -38,12 +38,27 @@ struct Args {
   int half;       // pairs
   int units;      // groups of VEC pairs (halves) or VEC / 2 pairs (interleaved), then of VEC features that pass
   int rot_units;
+  int64_t pass0;  // the first feature of the groups that pass
   int per_block;  // positions that a block's threads cover
   int chunk;      // heads per thread
   int shares0;    // shares of x[0]'s heads; x[1]'s follow
   float amplitude;
-  uint64_t turns[PDB_ROTARY_MAX_PAIRS];  // per position, in 2^-64 of a turn
+  alignas(16) uint64_t turns[PDB_ROTARY_MAX_PAIRS];  // per position, in 2^-64 of a turn
 };
+
+// N entries of the table.  Through the constant port, lanes that want different entries are served one after another,
+// which narrow groups (up to 32 different entries in a warp) take by a generic load instead.
+template <int N>
+__device__ __forceinline__ void load_turns(const uint64_t* at, uint64_t (&v)[N]) {
+  if constexpr (N == 1) {
+    asm("ld.b64 %0, [%1];" : "=l"(v[0]) : "l"(at));
+  } else if constexpr (N == 2) {
+    asm("ld.v2.b64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "l"(at));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = at[j];
+  }
+}
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
@@ -97,8 +112,8 @@ __device__ __forceinline__ void turn_pairs(float (&a)[N], float (&c)[N], const f
   }
 }
 
-// INTER: a group is VEC features, VEC / 2 pairs (one pair of two accesses where no address is even).
-// Else a group is VEC pairs, VEC features from each half.
+// INTER: a group is VEC features, VEC / 2 pairs (one pair of two accesses where no address is even); the last group that
+// turns may reach into the features that pass.  Else a group is VEC pairs, VEC features from each half.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args p) {
   using P = Pack<T, VEC>;
@@ -107,10 +122,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   constexpr bool TWO = !INTER || VEC == 1;
   const int span = p.units < kThreads ? p.units : kThreads;
   const int unit = blockIdx.z * kThreads + (int)threadIdx.x % span, at = (int)threadIdx.x / span;
-  const int64_t bt = (int64_t)blockIdx.x * p.per_block + at;
-  if (at >= p.per_block || unit >= p.units || bt >= p.batch * p.seqlen) return;
+  const int64_t bt = (int64_t)blockIdx.x * p.per_block + at, points = p.batch * p.seqlen;
+  if (at >= p.per_block || unit >= p.units || bt >= points) return;
   int64_t b, t;
-  if ((uint64_t)bt <= 0xffffffffu && (uint64_t)p.seqlen <= 0xffffffffu) {
+  if ((uint64_t)points <= 0xffffffffu) {
     b = (uint32_t)bt / (uint32_t)p.seqlen;
     t = (uint32_t)bt % (uint32_t)p.seqlen;
   } else {
@@ -122,15 +137,17 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int h0 = (blockIdx.y - (w ? p.shares0 : 0)) * p.chunk, n = min(p.chunk, p.heads[w] - h0);
   const bool turn = unit < p.rot_units;
   const int j0 = unit * NP;
-  const int64_t f0 = turn ? (INTER ? 2 * j0 : j0) : (int64_t)2 * p.half + (unit - p.rot_units) * VEC;
+  const int64_t f0 = turn ? (INTER ? 2 * j0 : j0) : p.pass0 + (int64_t)(unit - p.rot_units) * VEC;
   const int other = INTER ? 1 : p.half;
   float cs[NP], sn[NP];
   if (turn) {
     const uint64_t pos = (uint64_t)(p.pos ? p.pos[b * p.ps[0] + t * p.ps[1]] : p.start + t);
+    uint64_t turns[NP];
+    load_turns<NP>(p.turns + j0, turns);
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       // the signed top 32 bits: half turns in units of 2^-31
-      const int frac = (int)((pos * p.turns[j0 + j] + 0x80000000ull) >> 32);
+      const int frac = (int)((pos * turns[j] + 0x80000000ull) >> 32);
       sincospif((float)frac * 4.656612873077393e-10f, &sn[j], &cs[j]);
       sn[j] *= p.amplitude;
       cs[j] *= p.amplitude;
@@ -158,50 +175,61 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
           widen<T, VEC>(v[i], g);
           turn_pairs<NP>(f, g, cs, sn);
           narrow<T, VEC>(g, v[i]);
+          narrow<T, VEC>(f, u[i]);
           *reinterpret_cast<P*>(y + other) = v[i];
         } else {
+          const P as_it_was = u[i];
           float a[NP], c[NP];
 #pragma unroll
           for (int j = 0; j < NP; ++j) a[j] = f[2 * j], c[j] = f[2 * j + 1];
           turn_pairs<NP>(a, c, cs, sn);
 #pragma unroll
           for (int j = 0; j < NP; ++j) f[2 * j] = a[j], f[2 * j + 1] = c[j];
+          narrow<T, VEC>(f, u[i]);
+          if (j0 + NP > p.half) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+              if (j0 + j >= p.half) u[i].v[2 * j] = as_it_was.v[2 * j], u[i].v[2 * j + 1] = as_it_was.v[2 * j + 1];
+          }
         }
-        narrow<T, VEC>(f, u[i]);
       }
       *reinterpret_cast<P*>(y) = u[i];
     }
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool INTER>
 int launch(Args& p, const pdb_rotary_desc& d, cudaStream_t s) {
-  const bool inter = d.interleaved != 0;
-  p.rot_units = inter && VEC > 1 ? (int)(d.rotary_dim / VEC) : p.half / VEC;
+  constexpr int NP = INTER ? (VEC > 1 ? VEC / 2 : 1) : VEC, G = INTER ? 2 * NP : VEC;
+  p.rot_units = INTER ? (p.half + NP - 1) / NP : p.half / VEC;
+  p.pass0 = INTER ? (int64_t)p.rot_units * G : 2 * (int64_t)p.half;
   // in place there is nothing to do for the features that pass through
   const bool copy = (p.heads[0] && p.x[0] != p.y[0]) || (p.heads[1] && p.x[1] != p.y[1]);
-  p.units = p.rot_units + (copy ? (int)((d.head_dim - d.rotary_dim) / VEC) : 0);
+  p.units = p.rot_units + (copy ? (int)((d.head_dim - p.pass0) / VEC) : 0);
   if (p.units == 0) return PDB_OK;
   int dev = 0;
   cudaGetDevice(&dev);
   const int span = p.units < kThreads ? p.units : kThreads;
   p.per_block = kThreads / span;
-  const int64_t points = p.batch * p.seqlen;
-  const int64_t bx = (points + p.per_block - 1) / p.per_block, bz = (p.units + kThreads - 1) / kThreads;
-  if (bx > 0x7fffffffLL) return set_error(PDB_ERR_SHAPE, "rotary: too many positions for one launch");
+  const int64_t points = p.batch * p.seqlen, least = (int64_t)sm_count(dev) * 4;  // four blocks per SM
+  const int64_t bx = (points + p.per_block - 1) / p.per_block;
+  const int64_t bz = (p.units + kThreads - 1) / kThreads;
   // heads per thread: 8 (16 of narrow groups, whose angles weigh more) where that leaves every SM four blocks, fewer
   // otherwise
   auto shares = [&](int n) { return (n + p.chunk - 1) / p.chunk; };
   p.chunk = VEC * sizeof(T) >= 8 ? 8 : 16;
-  while (p.chunk > 1 && bx * bz * (shares(p.heads[0]) + shares(p.heads[1])) < (int64_t)sm_count(dev) * 4) p.chunk >>= 1;
+  while (p.chunk > 1 && bx * bz * (shares(p.heads[0]) + shares(p.heads[1])) < least) p.chunk >>= 1;
   while (shares(p.heads[0]) + shares(p.heads[1]) > 65535) p.chunk *= 2;
   p.shares0 = shares(p.heads[0]);
+  if (bx > 0x7fffffffLL) return set_error(PDB_ERR_SHAPE, "rotary: too many positions for one launch");
   const dim3 grid((unsigned)bx, (unsigned)(p.shares0 + shares(p.heads[1])), (unsigned)bz);
-  if (inter)
-    rotary_kernel<T, VEC, true><<<grid, kThreads, 0, s>>>(p);
-  else
-    rotary_kernel<T, VEC, false><<<grid, kThreads, 0, s>>>(p);
+  rotary_kernel<T, VEC, INTER><<<grid, kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError(), "rotary launch");
+}
+
+template <typename T, int VEC>
+int launch(Args& p, const pdb_rotary_desc& d, cudaStream_t s) {
+  return d.interleaved ? launch<T, VEC, true>(p, d, s) : launch<T, VEC, false>(p, d, s);
 }
 
 }  // namespace
@@ -232,8 +260,12 @@ extern "C" int pdb_rotary(const pdb_rotary_desc* d, void* stream) {
   auto fit = [&](int64_t elements) {
     while (vec > 1 && elements % vec != 0) vec >>= 1;
   };
-  fit(inter ? d->rotary_dim : p.half);
-  fit(d->head_dim - d->rotary_dim);
+  if (inter) {
+    fit(d->head_dim);
+  } else {
+    fit(p.half);
+    fit(d->head_dim - d->rotary_dim);
+  }
   for (int w = 0; w < 2; ++w) {
     p.heads[w] = (int)d->heads[w];
     if (d->heads[w] == 0) continue;

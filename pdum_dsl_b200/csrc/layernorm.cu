@@ -879,10 +879,10 @@ int backward(BwdArgs& p, cudaStream_t s) {
   if (done < 0) return PDB_ERR_CUDA;
   if (!done) {
     p.groups = (int)std::min<int64_t>(p.rows, 4 * sms());
-    layernorm_bwd_loop_kernel<T><<<(unsigned)p.rows, kLoopThreads, 0, s>>>(p);
-    if (p.partial)
+    if (p.partial)  // first: dx may lie where x or dout does
       layernorm_bwd_columns_kernel<T>
           <<<dim3((unsigned)((p.cols + kColThreads - 1) / kColThreads), (unsigned)p.groups), kColThreads, 0, s>>>(p);
+    layernorm_bwd_loop_kernel<T><<<(unsigned)p.rows, kLoopThreads, 0, s>>>(p);
   }
   return cuda_status(cudaGetLastError(), "layernorm backward launch");
 }

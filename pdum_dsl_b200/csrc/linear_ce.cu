@@ -38,6 +38,7 @@ constexpr int TK = 64, kEpiWarps = 16, THREADS = 128 + 32 * kEpiWarps;
 constexpr int kBox = 64 * 64 * 2;      // an MN-major box: 64 tile rows x 64 contracted rows
 constexpr int kTileA = 128 * TK * 2;   // a CTA's rows of A per stage
 constexpr int kStore = 4096;           // an epilogue warp's staging: 32 rows x 64 bf16 or 32 f32, 128-byte swizzle
+                                       // (kStats: 128 rows' (base, sum) of three of the four groups of columns)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 enum Epilogue { kStats = 0, kDlogits = 1, kOut = 2, kSum = 3 };  // kOut: bf16, kSum: f32
@@ -47,7 +48,7 @@ template <int CG, int EPI>
 struct Layout {
   static constexpr int kTileB = 256 / CG * TK * 2;
   static constexpr int kStage = kTileA + kTileB;
-  static constexpr int kStaging = EPI == kStats ? 0 : kEpiWarps * kStore;
+  static constexpr int kStaging = EPI == kStats ? 3 * 128 * 8 + 1024 : kEpiWarps * kStore;
   static constexpr int kStages = (227 * 1024 - 1024 - 256 - kStaging) / kStage;
   static constexpr int kSmem = kStages * kStage + kStaging + 256 + 1024;
 };
@@ -67,7 +68,7 @@ struct Args {
   // kStats, kDlogits: rows are (packed) tokens, columns vocabulary entries from col0 on
   const int64_t* target;
   int64_t col0, vocab;
-  float2* part;        // kStats: (base, sum) per [4 x n tile][m]
+  float2* part;        // kStats: (base, sum) per [n tile][m]
   float* tlogit;       // kStats: the target's logit
   const float* lse;    // kDlogits
   const float* dloss;
@@ -78,6 +79,7 @@ struct Args {
 struct __align__(8) Bars {
   uint64_t full[8], empty[8];
   uint64_t acc_full[2], acc_empty[2];
+  uint64_t left[4], taken[4];  // kStats, per 32 rows
   uint32_t tmem_base;
   int abort;
 };
@@ -124,6 +126,12 @@ __device__ __forceinline__ void fold(const float (&v)[32], float& base, float& s
   base = top;
 }
 
+// Two (base, sum) pairs into one.
+__device__ __forceinline__ void join_sums(float2& a, float2 b) {
+  const float m = fmaxf(a.x, b.x), z = m == -INFINITY ? 0.f : m;
+  a = make_float2(m, a.y * exp2f(a.x - z) + b.y * exp2f(b.x - z));
+}
+
 template <int CG>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
   if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, abort, err);
@@ -157,6 +165,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->acc_full[i], 1);
       mbar_init(&bar->acc_empty[i], CG * kEpiWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bar->left[i], 3);
+      mbar_init(&bar->taken[i], 1);
     }
     bar->abort = 0;
     fence_barrier_init();
@@ -223,6 +235,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           load(b, map_b, kb * TK, nb);
         }
       }
+    }
+    // given up: this thread's copies in flight arrive first (a pair's are counted at rank 0, and its CTAs leave together)
+    if (!ok && rank == 0) {
+      int never = 0;
+      for (uint32_t i = g > STAGES ? g - STAGES : 0; i < g; ++i)
+        mbar_wait(&bar->full[i % STAGES], (i / STAGES) & 1, &never, nullptr, 10000000ull);
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
     const uint32_t idesc = idesc_bf16(TM, 0, A_MN, B_MN) | ((uint32_t)(p.tile_n >> 3) << 17);
@@ -408,10 +426,26 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
-      if constexpr (EPI == kStats)
-        if (live) p.part[((n0 / p.tile_n) * 4 + cg) * m + gm] = make_float2(base, sum);
       if constexpr (CG == 2) warp_arrive_cluster_after_tc(mapa_shared(smem_u32(&bar->acc_empty[buf]), 0));
       else warp_arrive_after_tc(&bar->acc_empty[buf]);
+      if constexpr (EPI == kStats) {
+        // the four warps with these rows join their columns: three leave theirs in shared memory for the first
+        float2* mine = reinterpret_cast<float2*>(sC) + q4 * 32 + lane;
+        if (cg > 0) {
+          if (tt > 0 && !mbar_wait(&bar->taken[q4], (tt - 1) & 1, abort, p.err)) break;
+          mine[(cg - 1) * 128] = make_float2(base, sum);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar->left[q4]);
+        } else {
+          if (!mbar_wait(&bar->left[q4], tt & 1, abort, p.err)) break;
+          float2 j = make_float2(base, sum);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) join_sums(j, mine[i * 128]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar->taken[q4]);
+          if (live) p.part[(int64_t)(n0 / p.tile_n) * m + gm] = j;
+        }
+      }
     }
     if (EPI != kStats && lane == 0) bulk_wait_all();
   }
@@ -434,10 +468,6 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
   __shared__ float2 red[kFinishWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * 32 + lane;
-  auto join = [](float2& a, float2 b) {
-    const float m = fmaxf(a.x, b.x), z = m == -INFINITY ? 0.f : m;
-    a = make_float2(m, a.y * exp2f(a.x - z) + b.y * exp2f(b.x - z));
-  };
   grid_dep_wait();
   float2 s = make_float2(-INFINITY, 0.f);
   if (row < tokens) {
@@ -450,7 +480,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
         q[u] = k < parts ? part[(int64_t)k * tokens + row] : make_float2(-INFINITY, 0.f);
       }
 #pragma unroll
-      for (int u = 0; u < FLIGHT; ++u) join(s, q[u]);
+      for (int u = 0; u < FLIGHT; ++u) join_sums(s, q[u]);
     }
   }
   red[warp][lane] = s;
@@ -460,7 +490,7 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float2 q = make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o));
-    join(s, q);
+    join_sums(s, q);
   }
   const int64_t r = (int64_t)blockIdx.x * 32 + warp;
   if (lane == 0 && r < tokens) {
@@ -760,7 +790,7 @@ struct FwdPlan {
 FwdPlan plan_fwd(int64_t tokens, int64_t vocab) {
   FwdPlan f{};
   const int w = tile_width(tokens, vocab, 1, 32, sms() / cta_group(tokens));
-  f.parts = (int)(4 * div_up(vocab, w));
+  f.parts = (int)div_up(vocab, w);
   f.tlogit = up256((int64_t)f.parts * tokens * 8);
   f.bytes = f.tlogit + up256(tokens * 4);
   return f;

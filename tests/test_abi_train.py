@@ -193,7 +193,7 @@ def test_linear_cross_entropy_workspaces():
 
     def need(tokens, vocab, width):
         kw = dict(tokens=tokens, vocab=vocab, width=width, x_stride=width, w_stride=width)
-        assert lib.pdb_linear_ce_fwd_workspace_size(C.byref(_ce(**kw))) >= 8 * 4 * -(-vocab // 256) * tokens
+        assert lib.pdb_linear_ce_fwd_workspace_size(C.byref(_ce(**kw))) >= 8 * -(-vocab // 256) * tokens
         return lib.pdb_linear_ce_bwd_workspace_size(C.byref(_ce_bwd(dx_stride=width, dw_stride=width, **kw)))
 
     def rows(tokens, width):  # the packed tokens: rows of x, target, lse, dloss and index, behind count and unit

@@ -252,3 +252,33 @@ def test_gradient_against_differences(cuda):
     # the difference is off by h^2/6 times a third derivative of order |terms|; the gradients by ~100 u
     size = ((dx.double() * v).abs().sum() + (dg.double() * p).abs().sum() + (db.double() * q).abs().sum()).item()
     assert abs(got.item() - slope) <= (200 * U + 10 * h * h) * size
+
+
+@pytest.mark.parametrize("C", [96, 1001, 9000, 50000])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_in_place(cuda, C, t):
+    """y over x; through the C ABI also dx over dout and over x, whichever kernels the width takes."""
+    import ctypes as CT
+
+    import torch
+
+    from pdum_dsl_b200 import _lib, kernels
+
+    x, dy, gam, bet = _inputs(cuda, 40, C, _types()[t], torch.float32, C)
+    y, mean, rstd = kernels.layernorm(x, gam, bet, return_stats=True)
+    z = x.clone()
+    kernels.layernorm(z, gam, bet, out=z)
+    assert torch.equal(z, kernels.layernorm(x, gam, bet))
+    want = kernels.layernorm_backward(dy, x, mean, rstd, gam)
+    lib = _lib.load()
+    for over in ("dout", "x"):
+        a, b = dy.clone(), x.clone()
+        dx = a if over == "dout" else b
+        dw = torch.empty(2, C, device=cuda)
+        d = _lib.LayerNormBwdDesc(a.data_ptr(), b.data_ptr(), mean.data_ptr(), rstd.data_ptr(), gam.data_ptr(), dx.data_ptr(),
+                                  dw[0].data_ptr(), dw[1].data_ptr(), None, 0, 40, C, C, C, C,
+                                  _lib.PDB_BF16 if t == "bf16" else _lib.PDB_F32, _lib.PDB_F32)
+        ws = torch.empty(lib.pdb_layernorm_bwd_workspace_size(CT.byref(d)), dtype=torch.uint8, device=cuda)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(lib.pdb_layernorm_bwd(CT.byref(d), torch.cuda.current_stream().cuda_stream), "pdb_layernorm_bwd")
+        assert torch.equal(dx, want[0]) and torch.equal(dw[0], want[1]) and torch.equal(dw[1], want[2])

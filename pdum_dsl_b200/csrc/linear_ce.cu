@@ -132,6 +132,18 @@ __device__ __forceinline__ void join_sums(float2& a, float2 b) {
   a = make_float2(m, a.y * exp2f(a.x - z) + b.y * exp2f(b.x - z));
 }
 
+// The products issued so far arrive on this barrier (of both CTAs of a pair) when they are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    tc_commit(bar);
+}
+
 template <int CG>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
   if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, abort, err);
@@ -248,7 +260,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     // next 64 columns in the next box
     constexpr uint32_t a_step = A_MN ? 2048 : 32, a_lbo = A_MN ? kBox : 16;
     constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? kBox : 16;
-    uint32_t g = 0, tt = 0;
+    // The loop is kept short: its scheduler also serves epilogue warps, and a block's four products are over in 512 cycles.
+    // A descriptor's start address counts 16 bytes, so a stage and a step are additions to its low word.
+    const uint64_t da0 = sdesc_sw128(smem_u32(sA), a_lbo, 1024), db0 = sdesc_sw128(smem_u32(sB), b_lbo, 1024);
+    uint32_t st = 0, parity = 0, tt = 0;
     bool ok = true;
     for (int t = unit_id; ok && t < num_tiles; t += units, ++tt) {
       const int split = (int)((uint32_t)t / (uint32_t)(tm * tn));
@@ -257,34 +272,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!(ok = wait_bar<CG>(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256;
-      for (int kb = kb0; kb < kb1; ++kb, ++g) {
-        const int st = g % STAGES;
-        if (!(ok = wait_bar<CG>(&bar->full[st], (g / STAGES) & 1, abort, p.err))) break;
+      uint32_t more = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = wait_bar<CG>(&bar->full[st], parity, abort, p.err))) break;
         tc_fence_after();
-        const uint32_t a0 = smem_u32(sA + st * kTileA), b0 = smem_u32(sB + st * L::kTileB);
+        const uint64_t da = da0 + st * (kTileA >> 4), db = db0 + st * (L::kTileB >> 4);
 #pragma unroll
         for (int kk = 0; kk < TK / 16; ++kk) {
-          const uint64_t da = sdesc_sw128(a0 + kk * a_step, a_lbo, 1024), db = sdesc_sw128(b0 + kk * b_step, b_lbo, 1024);
-          if constexpr (CG == 2) mma_ss_pair(acc, da, db, idesc, kb > kb0 || kk > 0);
-          else mma_ss(acc, da, db, idesc, kb > kb0 || kk > 0);
+          if constexpr (CG == 2) mma_ss_pair(acc, da + (kk * a_step >> 4), db + (kk * b_step >> 4), idesc, more | kk);
+          else mma_ss(acc, da + (kk * a_step >> 4), db + (kk * b_step >> 4), idesc, more | kk);
         }
-        if constexpr (CG == 2) {
-          const uint32_t e = smem_u32(&bar->empty[st]);
-          tc_commit_pair(e);
-          tc_commit_pair(mapa_shared(e, 1));
-        } else {
-          tc_commit(&bar->empty[st]);
-        }
+        more = 1;
+        commit<CG>(&bar->empty[st]);
+        if (++st == STAGES) st = 0, parity ^= 1;
       }
-      if (ok) {
-        if constexpr (CG == 2) {
-          const uint32_t f = smem_u32(&bar->acc_full[buf]);
-          tc_commit_pair(f);
-          tc_commit_pair(mapa_shared(f, 1));
-        } else {
-          tc_commit(&bar->acc_full[buf]);
-        }
-      }
+      if (ok) commit<CG>(&bar->acc_full[buf]);
     }
   } else if (warp >= 4) {
     const int e = warp - 4, q4 = warp & 3, cg = e >> 2;  // TMEM lane quarter, group of 64 columns

@@ -317,7 +317,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int64_t gm = m0 + row0 + lane;  // rows and columns are below 2^25
       const bool live = gm < m;
       const bool none = split * kb_split >= nk;  // a share of the contracted index without any of it
-      const int64_t tgt = live ? next_target - p.col0 : -1;
+      // the target's column in this tile, if it is there
+      const int64_t away = next_target - p.col0 - n0;
+      const int tgt = live && away >= 0 && away < 256 ? (int)away : -256;
       const float nlse = -next_lse * kLog2e;
       float up = next_dloss / unit;
       if (next_target < 0 || next_target >= p.vocab) up = NAN;  // no such entry: the gradient says so
@@ -341,10 +343,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        const int hit = tgt - c0 >= 0 && tgt - c0 < 32 ? (int)(tgt - c0) : -1;
+        const int hit = tgt - c;  // 0 .. 31: in this chunk
         if constexpr (EPI == kStats) {
           const int nv = (int)min((int64_t)32, p.n - c0);
-          if (live && hit >= 0 && hit < nv) {
+          if (hit >= 0 && hit < nv) {
             float x = v[0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) x = i == hit ? v[i] : x;
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               v[i] = ex2(x);
               v[i + 1] = ex2(y);
             }
-            if (hit >= 0) {
+            if (hit >= 0 && hit < 32) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = i == hit ? v[i] - 1.f : v[i];
             }
@@ -391,7 +393,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             float x, y;
             f2_unpack(f2_mul(f2_pack(v[2 * i], v[2 * i + 1]), s2), x, y);
             pk[i] = pack_bf16(x, y);
-            if constexpr (EPI == kDlogits) pk[i] = live ? pk[i] : 0u;
+          }
+          if (EPI == kDlogits && m0 + row0 + 32 > m) {  // rows behind the last token, whatever their accumulators hold
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = live ? pk[i] : 0u;
           }
           if (ch == 0) {
             if (lane == 0) bulk_wait_read_all();

@@ -44,15 +44,16 @@ def shim_text(text: str) -> str:
 
 def reference_root() -> Path | None:
     """Where the reference checkout is mounted: $PDUM_DSL_REFERENCE, else the
-    ``reference_path`` that BASELINE.json records; None when neither names an
-    existing directory (e.g. on a GPU box, which only uses the prebuilt copy)."""
+    ``reference_path`` that BASELINE.json records; None when neither names a
+    directory with the reference's packages (an empty mount, or a GPU box, which
+    only uses the prebuilt copy)."""
     env = os.environ.get("PDUM_DSL_REFERENCE")
     cand = env
     if cand is None:
         bj = Path(__file__).resolve().parents[1] / "BASELINE.json"
         if bj.exists():
             cand = json.loads(bj.read_text()).get("reference_path")
-    if cand and Path(cand).is_dir():
+    if cand and (Path(cand) / "packages").is_dir():
         return Path(cand)
     return None
 

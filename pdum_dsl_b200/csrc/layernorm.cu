@@ -9,7 +9,9 @@
 //
 // Both directions are HBM-bound: the forward reads x and writes y, the backward
 // reads x and dy and writes dx, each once.  A row belongs to TPR threads, which
-// keep it in registers between its two reductions.
+// keep it in registers between its two reductions.  On a B200, against a copy of
+// the same bytes: forward 8192 x 4096 bf16 26.6 us (24.7), gradients with the
+// weights' 8192 x 4096 f32 69 us (67), 262144 x 128 bf16 38 us (37).
 #include <algorithm>
 
 #include "common.cuh"
@@ -531,9 +533,9 @@ __global__ void __launch_bounds__(kLoopThreads) layernorm_fwd_loop_kernel(const 
 
 // --------------------------------------------------------------- backward
 // Bytes of dynamic shared memory: the slots, or the columns' sums at the end.
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES>
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 constexpr int bwd_smem() {
-  const int slots = Rows<T, VEC, NV, TPR, BT, STAGES, 2, false>::kBytes;
+  const int slots = Rows<T, VEC, NV, TPR, BT, STAGES, 2, RAG>::kBytes;
   const int sums = BT > TPR ? BT * NV * VEC * (int)sizeof(float) : 0;
   return slots > sums ? slots : sums;
 }
@@ -805,15 +807,22 @@ int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
 // differently against 16 bytes) a thread takes 8, or 16 of long rows.
 template <typename T, int VEC, bool RAG>
 int dispatch_fwd(FwdArgs& p, cudaStream_t s) {
-  constexpr int NV = VEC == 1 ? 8 : sizeof(T) == 2 ? 32 / VEC : 16 / VEC;
-  int r = launch_fwd<T, VEC, NV, 8, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, NV, 16, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, NV, 32, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, NV, 64, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, NV, 128, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, NV, 256, 256, 3, RAG>(p, 4, s);
-  if (!r) r = launch_fwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, 2, RAG>(p, 2, s);
-  return r;
+  if constexpr (VEC == 1) {
+    int r = launch_fwd<T, 1, 8, 32, 256, 3, false>(p, 4, s);
+    if (!r) r = launch_fwd<T, 1, 8, 256, 256, 3, false>(p, 4, s);
+    if (!r) r = launch_fwd<T, 1, 16, 512, 512, 2, false>(p, 2, s);
+    return r;
+  } else {
+    constexpr int NV = (sizeof(T) == 2 ? 32 : 16) / VEC;
+    int r = launch_fwd<T, VEC, NV, 8, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 16, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 32, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 64, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 128, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 256, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 512, 512, 2, RAG>(p, 2, s);
+    return r;
+  }
 }
 
 template <typename T>
@@ -838,7 +847,7 @@ int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
   if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC * CL) return 0;
   share_rows(p, BT / TPR, (int64_t)blocks * sms() / CL);
   return launch(layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>, p, BT,
-                bwd_smem<T, VEC, NV, TPR, BT, STAGES>(), CL, s);
+                bwd_smem<T, VEC, NV, TPR, BT, STAGES, RAG>(), CL, s);
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
@@ -847,20 +856,25 @@ int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
 // little: 83 against 74 us at 8192 columns).
 template <typename T, int VEC, bool RAG>
 int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
-  constexpr int NV = VEC == 1 ? 4 : 16 / VEC, N = VEC == 1 ? 3 : 2;
-  int r = launch_bwd<T, VEC, NV, 8, 256, 3, RAG>(p, N, s);
-  if (!r) r = launch_bwd<T, VEC, NV, 16, 256, 3, RAG>(p, N, s);
-  if (!r) r = launch_bwd<T, VEC, NV, 32, 256, 3, RAG>(p, N, s);
-  if (!r) r = launch_bwd<T, VEC, NV, 64, 256, 3, RAG>(p, N, s);
-  if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, N, s);
   constexpr int S = sizeof(T) == 4 ? 2 : 3;
-  if (!r) r = launch_bwd<T, VEC, NV, 256, VEC == 1 ? 256 : 512, S, RAG>(p, VEC == 1 ? 3 : 1, s);
-  if (!r) r = launch_bwd<T, VEC, VEC == 1 ? 16 : NV, 512, 512, S, RAG>(p, 1, s);
-  if constexpr (VEC > 1) {
+  if constexpr (VEC == 1) {
+    int r = launch_bwd<T, 1, 4, 32, 256, 3, false>(p, 3, s);
+    if (!r) r = launch_bwd<T, 1, 4, 256, 256, 3, false>(p, 3, s);
+    if (!r) r = launch_bwd<T, 1, 16, 512, 512, S, false>(p, 1, s);
+    return r;
+  } else {
+    constexpr int NV = 16 / VEC;
+    int r = launch_bwd<T, VEC, NV, 8, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 16, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 32, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 64, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 256, 512, S, RAG>(p, 1, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG>(p, 1, s);
     if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 2>(p, 1, s);
     if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 4>(p, 1, s);
+    return r;
   }
-  return r;
 }
 
 template <typename T>

@@ -167,3 +167,31 @@ def test_single_tokens_agree_with_the_whole_sequence(cuda):
         # other tiles, the same 32-bit sums in another order
         assert ((e1 - lse[rows]).abs() <= 2.0 ** -20 * (1 + lse[rows].abs())).all()
         assert ((l1 - loss[rows]).abs() <= 2.0 ** -19 * (1 + lse[rows].abs())).all()
+
+
+def test_on_a_stream_of_its_own_next_to_another(cuda):
+    """Two steps at once on two streams, each on data made there: what each gives alone."""
+    import torch
+
+    from pdum_dsl_b200 import kernels as K
+
+    freq, _ = K.rotary_frequencies(D)
+    alone = []
+    for seed in (5, 6):
+        p, target = _inputs(cuda, seed)
+        alone.append(_step(p, target, freq))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for seed, s in zip((5, 6), streams):
+        with torch.cuda.stream(s):
+            p, target = _inputs(cuda, seed)
+            got.append(_step(p, target, freq))
+    torch.cuda.synchronize()
+    K.check_device_errors()
+    for (loss, d), (want, dw) in zip(got, alone):
+        assert torch.equal(loss, want)
+        for k in d:  # as above: the attention's dq varies in its last bits
+            if k in ("x", "wq", "wk", "g1", "b1"):
+                assert ((d[k].double() - dw[k].double()).norm() <= BOUND * dw[k].double().norm()), k
+            else:
+                assert torch.equal(d[k], dw[k]), k

@@ -394,8 +394,9 @@ int pdb_rotary(const pdb_rotary_desc* d, void* stream);
 /* ---- cross entropy of a linear head -----------------------------------------
  * No counterpart in the reference (a contraction, a row softmax and a gather
  * there).  x [tokens, width] hidden states, w [vocab, width] the head's weight,
- * both bf16 (PDB_ERR_UNSUPPORTED otherwise), width and row strides multiples of
- * 8; logit[n, v] = x[n] . w[v] in f32, never stored:
+ * both bf16 (tcgen05 products, f32 accumulate) or both f32 (IEEE multiply-adds,
+ * the precision of the reference's f32 column), width and row strides multiples
+ * of 16 bytes; logit[n, v] = x[n] . w[v] in f32, never stored:
  *   lse[n]  = log sum_v exp(logit[n, v])
  *   loss[n] = lse[n] - logit[n, target[n]]
  * loss and lse are f32 [tokens], either may be NULL.  target is int64 [tokens] on
@@ -404,9 +405,11 @@ int pdb_rotary(const pdb_rotary_desc* d, void* stream);
  * gradient).  The backward takes the forward's lse and dloss (f32, element stride
  * dloss_stride, 0 broadcasts one value):
  *   G[n, v] = (exp(logit[n, v] - lse[n]) - [v == target[n]]) * dloss[n]
- *   dx = G w,  dw = G^T x      (bf16, f32 accumulate; dx or dw may be NULL)
- * piece by piece of the vocabulary: its workspace holds one piece of G in bf16
- * (at most 512 MiB, or 256 columns) and f32 partial sums.  Sums are taken in a
+ *   dx = G w,  dw = G^T x      (of x's type, f32 accumulate; dx or dw may be NULL)
+ * piece by piece of the vocabulary: its workspace holds one piece of G in that
+ * type (at most 512 MiB, or 256 columns), the rows of x that count, packed, and
+ * f32 partial sums.  What ignored tokens' rows, lse and dloss hold reaches no
+ * gradient.  dx and dw must not overlap the inputs.  Sums are taken in a
  * fixed order.  Workspaces are sized by the *_workspace_size calls (0 for a
  * descriptor that is refused or has no tokens) on the device that runs the call. */
 typedef struct {

@@ -26,6 +26,9 @@
 // stores through shared memory.  On a B200, 4096 tokens x 65536 x 2048: the loss in 676
 // us cool (1.63 PFLOP/s), 820 warm under the power limit; 8192 x 128000 x 4096 gradients
 // with a tenth ignored in 16.7 to 18.4 ms (1.40 to 1.54 of all tokens' operations).
+//
+// f32 operands take the same steps on IEEE multiply-adds (the f32 column refuses
+// reduced operand types): linear_ce_f32_kernel, G in f32.
 #include <algorithm>
 #include <cfloat>
 #include <utility>
@@ -514,14 +517,14 @@ __global__ void __launch_bounds__(32 * kFinishWarps)
 // GROUPS threads share an element's shares (one after another, 135 shares of a small product took 38 us).
 constexpr int kJoinThreads = 256;
 
-template <int GROUPS>
+template <int GROUPS, typename T>
 __global__ void __launch_bounds__(kJoinThreads)
     linear_ce_join_kernel(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state,
-                          const int* token_of, __nv_bfloat16* out, int64_t ldo) {
+                          const int* token_of, T* out, int64_t ldo) {
   constexpr int EACH = kJoinThreads / GROUPS, FLIGHT = 8;
   __shared__ float4 red[GROUPS][EACH];
   const int group = threadIdx.x / EACH, l = threadIdx.x % EACH;
-  const int64_t i = ((int64_t)blockIdx.x * EACH + l) * 4;  // n is a multiple of 8
+  const int64_t i = ((int64_t)blockIdx.x * EACH + l) * 4;  // n is a multiple of 4
   grid_dep_wait();
   const bool live = i < (state ? *state : m) * n;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -548,10 +551,14 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
   }
   if (!live) return;
-  const float u = *unit;
-  uint2 o = make_uint2(pack_bf16(s.x * u, s.y * u), pack_bf16(s.z * u, s.w * u));
   const int64_t row = i / n;
-  *reinterpret_cast<uint2*>(out + (token_of ? token_of[row] : row) * ldo + i % n) = o;
+  T* at = out + (token_of ? token_of[row] : row) * ldo + i % n;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(at) = s;
+  } else {
+    const float u = *unit;
+    *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(s.x * u, s.y * u), pack_bf16(s.z * u, s.w * u));
+  }
 }
 
 // Packs the tokens that count, in their order: their rows of x (when a token is ignored, or `pack`: rows that do not
@@ -564,14 +571,15 @@ __global__ void __launch_bounds__(kJoinThreads)
 // is exact.
 //
 // A block packs `rows` tokens; for its place it counts the tokens before them itself, so one launch is enough.
+template <typename T>
 struct Pack {
-  const __nv_bfloat16* x;
+  const T* x;
   const int64_t* target;
   const float* lse;
   const float* dloss;
   int64_t tokens, width, ldx, dloss_stride, ignore;
   int rows, pack;
-  __nv_bfloat16* xp;  // [tokens][ldp]
+  T* xp;  // [tokens][ldp]
   int64_t ldp;
   int64_t* targetp;
   float* lsep;
@@ -579,13 +587,15 @@ struct Pack {
   int* token_of;
   int* state;
   float* unit;
-  __nv_bfloat16* dx;  // nullable
+  T* dx;  // nullable
   int64_t lddx;
 };
 
 constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32;
 
-__global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack p) {
+template <typename T>
+__global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack<T> p) {
+  constexpr int VEC = 16 / sizeof(T);
   __shared__ int before_s[kPackWarps], total_s[kPackWarps], place[kPackThreads];
   __shared__ float max_s[kPackWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -627,7 +637,7 @@ __global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack
     p.state[1] = pack;
     *p.unit = top > 0.f ? top : 1.f;
   }
-  const int64_t vecs = p.width / 8;
+  const int64_t vecs = p.width / VEC;
   for (int64_t c = first; c < last; c += kPackThreads) {
     const int64_t n = c + tid;
     const bool counts = n < last && p.target[n] != p.ignore;
@@ -653,7 +663,7 @@ __global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack
     const int64_t here = min((int64_t)kPackThreads, last - c);
     for (int64_t e = tid; e < here * vecs; e += kPackThreads) {
       const int r = (int)(e / vecs);
-      const int64_t col = (e - r * vecs) * 8;
+      const int64_t col = (e - r * vecs) * VEC;
       if (place[r] >= 0)
         *reinterpret_cast<uint4*>(p.xp + place[r] * p.ldp + col) = *reinterpret_cast<const uint4*>(p.x + (c + r) * p.ldx + col);
       else if (p.dx)
@@ -664,7 +674,170 @@ __global__ void __launch_bounds__(kPackThreads) linear_ce_pack_kernel(const Pack
   if (pack && blockIdx.x == gridDim.x - 1) {
     const int64_t rest = min(p.tokens, (int64_t)(total + TK - 1) / TK * TK) - total;
     for (int64_t e = tid; e < rest * vecs; e += kPackThreads)
-      *reinterpret_cast<uint4*>(p.xp + (total + e / vecs) * p.ldp + e % vecs * 8) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(p.xp + (total + e / vecs) * p.ldp + e % vecs * VEC) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------- f32 path
+// The same four products on IEEE multiply-adds (two per instruction): 128 x 128 tiles, 16 deep, 8 x 8 per thread (two
+// groups of four rows and of four columns, so that shared memory is read 16 bytes wide without conflicts), the next
+// block's loads in flight; two blocks per SM, and a long contraction under few tiles in shares that join() adds up.
+// The FMA pipes bound it: 4096 tokens of 1024 x 32000 entries take 6.0 ms (44.5 TFLOP/s; 8.7 ms with one multiply-add per
+// instruction and one block per SM) and their gradients 18.3 ms (44.0; 26.1); 64 tokens of 512 x 8000 entries' gradients
+// take 0.13 ms (0.98 before).
+constexpr int FT = 128, FK = 16, FTHREADS = 256;
+
+struct F32Args {
+  const float *a, *b;
+  int64_t m, n, k, lda, ldb;
+  const float* xp;  // packed rows of x: a of G, b of dw, when state[1]
+  int64_t ldp;
+  const int* state;
+  int dyn;  // as in Args
+  const int* token_of;
+  const int64_t* target;
+  int64_t col0, vocab;
+  float2* part;  // [n tile][m]
+  float* tlogit;
+  const float *lse, *dloss;
+  float* out;
+  int64_t ldo;
+  int add;
+  int splits;  // > 1: out is [splits][m][n], a share of the contracted index each
+};
+
+template <bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(FTHREADS, 2) linear_ce_f32_kernel(const F32Args p) {
+  __shared__ __align__(16) float As[2][FK][FT + 4], Bs[2][FK][FT + 4];
+  grid_dep_wait();
+  int64_t m = p.m, k = p.k, lda = p.lda, ldb = p.ldb;
+  const float *A = p.a, *B = p.b;
+  if (EPI != kStats && p.state) {
+    (p.dyn == 1 ? m : k) = p.state[0];
+    if (p.state[1]) {
+      if (EPI == kDlogits) A = p.xp, lda = p.ldp;
+      if (A_MN) B = p.xp, ldb = p.ldp;
+    }
+  }
+  const uint32_t tm = (uint32_t)((p.m + FT - 1) / FT);  // the grid's, whatever the number of tokens is
+  const int64_t m0 = (int64_t)(blockIdx.x % tm) * FT, n0 = (int64_t)(blockIdx.x / tm) * FT;
+  if (m0 >= m) return;
+  // this block's share of the contracted index: [k1, k)
+  const int64_t share = ((k + FK - 1) / FK + p.splits - 1) / p.splits * FK, k1 = blockIdx.y * share;
+  k = min(k, k1 + share);
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  // four elements along the operand's rows in memory; what lies outside the product is 0
+  auto load = [&](const float* x, int64_t ld, bool mn, int64_t first, int64_t rows, int64_t k0, int i) {
+    const int e = tid + i * FTHREADS;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mn) {
+      const int64_t kk = k0 + (e >> 5), r = first + (e & 31) * 4;
+      if (kk < k && r < rows) v = *reinterpret_cast<const float4*>(x + kk * ld + r);
+    } else {
+      const int64_t r = first + (e >> 2), kk = k0 + (e & 3) * 4;
+      if (r < rows && kk < k) {
+        v = *reinterpret_cast<const float4*>(x + r * ld + kk);
+        if (kk + 1 >= k) v.y = 0.f;
+        if (kk + 2 >= k) v.z = 0.f;
+        if (kk + 3 >= k) v.w = 0.f;
+      }
+    }
+    return v;
+  };
+  auto store = [&](float (&s)[FK][FT + 4], bool mn, const float4& v, int i) {
+    const int e = tid + i * FTHREADS;
+    if (mn) {
+      *reinterpret_cast<float4*>(&s[e >> 5][(e & 31) * 4]) = v;
+    } else {
+      const int r = e >> 2, kk = (e & 3) * 4;
+      s[kk][r] = v.x, s[kk + 1][r] = v.y, s[kk + 2][r] = v.z, s[kk + 3][r] = v.w;
+    }
+  };
+  uint64_t acc2[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc2[i][j] = f2_pack(0.f, 0.f);
+  float4 av[2], bv[2];
+  auto fetch = [&](int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) av[i] = load(A, lda, A_MN, m0, m, k0, i), bv[i] = load(B, ldb, B_MN, n0, p.n, k0, i);
+  };
+  fetch(k1);
+  int buf = 0;
+  for (int64_t k0 = k1; k0 < k; k0 += FK, buf ^= 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) store(As[buf], A_MN, av[i], i), store(Bs[buf], B_MN, bv[i], i);
+    __syncthreads();  // the other buffer was read before the barrier of the block before
+    if (k0 + FK < k) fetch(k0 + FK);
+#pragma unroll
+    for (int kk = 0; kk < FK; ++kk) {
+      float a[8];
+      uint64_t b2[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 x = *reinterpret_cast<const float4*>(&As[buf][kk][h * 64 + ty * 4]);
+        const float4 y = *reinterpret_cast<const float4*>(&Bs[buf][kk][h * 64 + tx * 4]);
+        a[4 * h] = x.x, a[4 * h + 1] = x.y, a[4 * h + 2] = x.z, a[4 * h + 3] = x.w;
+        b2[2 * h] = f2_pack(y.x, y.y), b2[2 * h + 1] = f2_pack(y.z, y.w);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t a2 = f2_pack(a[i], a[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc2[i][j] = f2_fma(a2, b2[j], acc2[i][j]);
+      }
+    }
+  }
+  float acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f2_unpack(acc2[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
+    const bool live = row < m;
+    const int64_t tgt = EPI != kOut && live ? p.target[row] : -1;
+    if constexpr (EPI == kStats) {
+      float2 s = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t col = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+        if (col >= p.n) acc[i][j] = -INFINITY;
+        else if (col == tgt) p.tlogit[row] = acc[i][j];
+        s.x = fmaxf(s.x, acc[i][j] * kLog2e);
+      }
+      const float base = s.x == -INFINITY ? 0.f : s.x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s.y += exp2f(fmaf(acc[i][j], kLog2e, -base));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1)
+        join_sums(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
+      if (tx == 0 && live) p.part[n0 / FT * m + row] = s;
+    } else if (live) {
+      const float lse = EPI == kDlogits ? p.lse[row] : 0.f;
+      // an index that the vocabulary does not have: the gradient says so
+      const float up = EPI != kDlogits ? 1.f : tgt < 0 || tgt >= p.vocab ? NAN : p.dloss[row];
+      float* to = p.out + blockIdx.y * p.m * p.ldo + (EPI == kOut && p.token_of ? p.token_of[row] : row) * p.ldo;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t col = n0 + h * 64 + tx * 4;
+        if (col >= p.n) continue;  // rows of the result reach the next multiple of four columns
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = acc[i][4 * h + j];
+          if constexpr (EPI == kDlogits) v[j] = (expf(v[j] - lse) - (col + j + p.col0 == tgt ? 1.f : 0.f)) * up;
+        }
+        float4* at = reinterpret_cast<float4*>(to + col);
+        if (EPI == kOut && p.add) {
+          const float4 q = *at;
+          v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+        *at = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    }
   }
 }
 
@@ -691,9 +864,9 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Launched behind the grid before it: set-up overlaps that grid's tail, and every kernel waits before it reads.
 template <typename... Params, typename... Given>
-int launch(void (*kernel)(Params...), int64_t grid, int threads, int smem, int cluster, cudaStream_t s, Given&&... args) {
+int launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster, cudaStream_t s, Given&&... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -780,15 +953,16 @@ int64_t up256(int64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 constexpr int64_t kMaxTokens = 1 << 24, kMaxVocab = 1 << 24, kMaxWidth = 1 << 16;
 
 int check(int64_t tokens, int64_t vocab, int64_t width, int64_t x_stride, int64_t w_stride, int32_t dtype) {
-  if (dtype != PDB_BF16)
-    return set_error(PDB_ERR_UNSUPPORTED, "linear cross entropy: built for bf16 operands only (dtype %d)", dtype);
+  if (dtype != PDB_BF16 && dtype != PDB_F32)
+    return set_error(PDB_ERR_UNSUPPORTED, "linear cross entropy: unknown dtype %d", dtype);
+  const int vec = dtype == PDB_BF16 ? 8 : 4;
   if (tokens < 0 || vocab <= 0 || width <= 0)
     return set_error(PDB_ERR_SHAPE, "linear cross entropy: vocab and width must be positive, tokens not negative");
   if (tokens > kMaxTokens || vocab > kMaxVocab || width > kMaxWidth)
     return set_error(PDB_ERR_SHAPE, "linear cross entropy: at most 2^24 tokens and entries, width 2^16");
-  if (width % 8 != 0) return set_error(PDB_ERR_ALIGN, "linear cross entropy: width must be a multiple of 8");
-  if (x_stride < width || w_stride < width || x_stride % 8 != 0 || w_stride % 8 != 0)
-    return set_error(PDB_ERR_ALIGN, "linear cross entropy: row strides must be multiples of 8 and at least width");
+  if (width % vec != 0 || x_stride < width || w_stride < width || x_stride % vec != 0 || w_stride % vec != 0)
+    return set_error(PDB_ERR_ALIGN,
+                     "linear cross entropy: width and row strides must be multiples of 16 bytes, strides at least width");
   return PDB_OK;
 }
 
@@ -796,9 +970,9 @@ struct FwdPlan {
   int parts;
   int64_t tlogit, bytes;  // byte offset of the targets' logits
 };
-FwdPlan plan_fwd(int64_t tokens, int64_t vocab) {
+FwdPlan plan_fwd(int64_t tokens, int64_t vocab, int32_t dtype) {
   FwdPlan f{};
-  const int w = tile_width(tokens, vocab, 1, 32, sms() / cta_group(tokens));
+  const int w = dtype == PDB_F32 ? FT : tile_width(tokens, vocab, 1, 32, sms() / cta_group(tokens));
   f.parts = (int)div_up(vocab, w);
   f.tlogit = up256((int64_t)f.parts * tokens * 8);
   f.bytes = f.tlogit + up256(tokens * 4);
@@ -815,6 +989,12 @@ void split_k(Args& p, int64_t k) {
   p.splits = (int)div_up(nk, p.kb_split);
 }
 
+// ... for the f32 products, whose tiles are one block each: shares of at least 16 blocks of 16.
+int f32_splits(int64_t m, int64_t n, int64_t k) {
+  const int64_t tiles = div_up(m, FT) * div_up(n, FT);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * sms() / tiles, div_up(k, FK) / 16, 1024}));
+}
+
 struct BwdPlan {
   int64_t piece, pieces;  // vocabulary entries per piece
   int dx_splits, dw_splits;
@@ -824,9 +1004,10 @@ struct BwdPlan {
 // G of one piece: at most this many bytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 
-BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
+BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width, int32_t dtype) {
   BwdPlan b{};
-  const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * std::max<int64_t>(tokens, 1)) / 256 * 256);
+  const int64_t size = dtype == PDB_F32 ? 4 : 2;
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / (size * std::max<int64_t>(tokens, 1)) / 256 * 256);
   b.pieces = div_up(vocab, most);
   // rows of G on 128-byte lines: with 50024 columns, 1021 x 50021 x 1000 took 94 us for dx
   b.piece = std::min(div_up(div_up(vocab, b.pieces), 256) * 256, div_up(vocab, 64) * 64);
@@ -838,7 +1019,11 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   a.m = std::min(b.piece, vocab);
   split_k(a, tokens);
   b.dw_splits = a.splits;
-  int64_t at = up256(tokens * b.piece * 2);
+  if (dtype == PDB_F32) {
+    b.dx_splits = f32_splits(tokens, width, std::min(b.piece, vocab));
+    b.dw_splits = f32_splits(std::min(b.piece, vocab), width, tokens);
+  }
+  int64_t at = up256(tokens * b.piece * size);
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += up256(bytes);
@@ -847,26 +1032,74 @@ BwdPlan plan_bwd(int64_t tokens, int64_t vocab, int64_t width) {
   b.ldp = div_up(width, 64) * 64;
   b.state = take(2 * sizeof(int));
   b.unit = take(sizeof(float));
-  b.xp = take(tokens * b.ldp * 2);
+  b.xp = take(tokens * b.ldp * size);
   b.target = take(tokens * 8);
   b.lse = take(tokens * 4);
   b.dloss = take(tokens * 4);
   b.token_of = take(tokens * 4);
   b.dx_acc = at;
-  if (b.dx_splits > 1 || b.pieces > 1) at += up256(b.dx_splits * tokens * width * 4);
+  if (b.dx_splits > 1 || (size == 2 && b.pieces > 1)) at += up256(b.dx_splits * tokens * width * 4);
   b.dw_acc = at;
   if (b.dw_splits > 1) at += up256(b.dw_splits * std::min(b.piece, vocab) * width * 4);
   b.bytes = at;
   return b;
 }
 
-int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state, const int* token_of,
-         void* out, int64_t ldo, cudaStream_t s) {
+template <typename T>
+int join(const float* acc, int splits, int64_t m, int64_t n, const float* unit, const int* state, const int* token_of, T* out,
+         int64_t ldo, cudaStream_t s) {
   auto on = [&](auto kernel, int groups) {
     return launch(kernel, div_up(m * n, 4 * kJoinThreads / groups), kJoinThreads, 0, 1, s, acc, splits, m, n, unit, state,
-                  token_of, static_cast<__nv_bfloat16*>(out), ldo);
+                  token_of, out, ldo);
   };
-  return splits > 8 ? on(linear_ce_join_kernel<16>, 16) : on(linear_ce_join_kernel<1>, 1);
+  return splits > 8 ? on(linear_ce_join_kernel<16, T>, 16) : on(linear_ce_join_kernel<1, T>, 1);
+}
+
+template <typename T>
+int pack(const pdb_linear_ce_bwd_desc& d, const BwdPlan& b, uint8_t* ws, cudaStream_t s) {
+  Pack<T> k{};
+  k.x = static_cast<const T*>(d.x);
+  k.target = d.target;
+  k.lse = d.lse;
+  k.dloss = d.dloss;
+  k.tokens = d.tokens;
+  k.width = d.width;
+  k.ldx = d.x_stride;
+  k.dloss_stride = d.dloss_stride;
+  k.ignore = d.ignore_index;
+  k.rows = (int)div_up(d.tokens, 2 * sms());
+  k.pack = sizeof(T) == 2 && d.width % 64 != 0;
+  k.xp = reinterpret_cast<T*>(ws + b.xp);
+  k.ldp = b.ldp;
+  k.targetp = reinterpret_cast<int64_t*>(ws + b.target);
+  k.lsep = reinterpret_cast<float*>(ws + b.lse);
+  k.dlossp = reinterpret_cast<float*>(ws + b.dloss);
+  k.token_of = reinterpret_cast<int*>(ws + b.token_of);
+  k.state = reinterpret_cast<int*>(ws + b.state);
+  k.unit = reinterpret_cast<float*>(ws + b.unit);
+  k.dx = static_cast<T*>(d.dx);
+  k.lddx = d.dx_stride;
+  return launch(linear_ce_pack_kernel<T>, div_up(d.tokens, k.rows), kPackThreads, 0, 1, s, k);
+}
+
+F32Args f32_product(const Matrix& a, const Matrix& b, int64_t m, int64_t n, int64_t k) {
+  F32Args p{};
+  p.a = static_cast<const float*>(a.p);
+  p.b = static_cast<const float*>(b.p);
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.lda = a.ld;
+  p.ldb = b.ld;
+  p.splits = 1;
+  return p;
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+int f32_gemm(const F32Args& p, cudaStream_t s) {
+  const int64_t tiles = div_up(p.m, FT) * div_up(p.n, FT);
+  if (tiles > 0x7fffffffLL) return set_error(PDB_ERR_SHAPE, "linear cross entropy: too many tiles");
+  return launch(linear_ce_f32_kernel<A_MN, B_MN, EPI>, dim3((unsigned)tiles, p.splits), FTHREADS, 0, 1, s, p);
 }
 
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -878,7 +1111,7 @@ using namespace pdb;
 
 extern "C" size_t pdb_linear_ce_fwd_workspace_size(const pdb_linear_ce_fwd_desc* d) {
   if (!d || check(d->tokens, d->vocab, d->width, d->x_stride, d->w_stride, d->dtype) != PDB_OK || d->tokens == 0) return 0;
-  return (size_t)plan_fwd(d->tokens, d->vocab).bytes;
+  return (size_t)plan_fwd(d->tokens, d->vocab, d->dtype).bytes;
 }
 
 extern "C" int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream) {
@@ -889,50 +1122,62 @@ extern "C" int pdb_linear_ce_fwd(const pdb_linear_ce_fwd_desc* d, void* stream) 
     return set_error(PDB_ERR_ARG, "linear cross entropy: null x / w / target, or neither loss nor lse");
   if (!a16(d->x) || !a16(d->w))
     return set_error(PDB_ERR_ALIGN, "linear cross entropy: x and w must be 16-byte aligned");
-  const FwdPlan f = plan_fwd(d->tokens, d->vocab);
+  const FwdPlan f = plan_fwd(d->tokens, d->vocab, d->dtype);
   if (!d->workspace || d->workspace_bytes < (size_t)f.bytes || !a16(d->workspace))
     return set_error(PDB_ERR_ARG, "linear cross entropy: workspace too small or not 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(d->workspace);
-  Args p{};
-  p.m = d->tokens;
-  p.n = d->vocab;
-  p.k = d->width;
-  p.splits = 1;
-  p.kb_split = (int)div_up(d->width, TK);
-  p.target = d->target;
-  p.vocab = d->vocab;
-  p.part = reinterpret_cast<float2*>(ws);
-  p.tlogit = reinterpret_cast<float*>(ws + f.tlogit);
+  float2* part = reinterpret_cast<float2*>(ws);
+  float* tlogit = reinterpret_cast<float*>(ws + f.tlogit);
   const Matrix x{d->x, d->tokens, d->width, d->x_stride}, w{d->w, d->vocab, d->width, d->w_stride};
-  if (int st = gemm<false, false, kStats>(x, w, CUtensorMap{}, Matrix{}, p, s)) return st;
-  return launch(linear_ce_finish_kernel, div_up(d->tokens, 32), 32 * kFinishWarps, 0, 1, s, p.part, f.parts, p.tlogit,
+  if (d->dtype == PDB_F32) {
+    F32Args p = f32_product(x, w, d->tokens, d->vocab, d->width);
+    p.target = d->target;
+    p.vocab = d->vocab;
+    p.part = part;
+    p.tlogit = tlogit;
+    if (int st = f32_gemm<false, false, kStats>(p, s)) return st;
+  } else {
+    Args p{};
+    p.m = d->tokens;
+    p.n = d->vocab;
+    p.k = d->width;
+    p.splits = 1;
+    p.kb_split = (int)div_up(d->width, TK);
+    p.target = d->target;
+    p.vocab = d->vocab;
+    p.part = part;
+    p.tlogit = tlogit;
+    if (int st = gemm<false, false, kStats>(x, w, CUtensorMap{}, Matrix{}, p, s)) return st;
+  }
+  return launch(linear_ce_finish_kernel, div_up(d->tokens, 32), 32 * kFinishWarps, 0, 1, s, part, f.parts, tlogit,
                 d->target, d->tokens, d->vocab, d->ignore_index, d->loss, d->lse);
 }
 
 extern "C" size_t pdb_linear_ce_bwd_workspace_size(const pdb_linear_ce_bwd_desc* d) {
   if (!d || check(d->tokens, d->vocab, d->width, d->x_stride, d->w_stride, d->dtype) != PDB_OK || d->tokens == 0) return 0;
-  return (size_t)plan_bwd(d->tokens, d->vocab, d->width).bytes;
+  return (size_t)plan_bwd(d->tokens, d->vocab, d->width, d->dtype).bytes;
 }
 
 extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) {
   if (!d) return set_error(PDB_ERR_ARG, "null descriptor");
   if (int st = check(d->tokens, d->vocab, d->width, d->x_stride, d->w_stride, d->dtype)) return st;
-  if (d->dx && (d->dx_stride < d->width || d->dx_stride % 8 != 0 || !a16(d->dx)))
-    return set_error(PDB_ERR_ALIGN, "linear cross entropy: dx must be 16-byte aligned with a row stride that is a multiple of 8");
-  if (d->dw && (d->dw_stride < d->width || d->dw_stride % 8 != 0 || !a16(d->dw)))
-    return set_error(PDB_ERR_ALIGN, "linear cross entropy: dw must be 16-byte aligned with a row stride that is a multiple of 8");
+  const int size = d->dtype == PDB_F32 ? 4 : 2;
+  if (d->dx && (d->dx_stride < d->width || d->dx_stride * size % 16 != 0 || !a16(d->dx)))
+    return set_error(PDB_ERR_ALIGN, "linear cross entropy: dx must be 16-byte aligned with rows of whole 16 bytes");
+  if (d->dw && (d->dw_stride < d->width || d->dw_stride * size % 16 != 0 || !a16(d->dw)))
+    return set_error(PDB_ERR_ALIGN, "linear cross entropy: dw must be 16-byte aligned with rows of whole 16 bytes");
   if (!d->dx && !d->dw) return set_error(PDB_ERR_ARG, "linear cross entropy: neither dx nor dw");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->tokens == 0) {  // nothing adds to dw
     if (!d->dw) return PDB_OK;
-    return cuda_status(cudaMemset2DAsync(d->dw, d->dw_stride * 2, 0, d->width * 2, d->vocab, s), "linear cross entropy: zero dw");
+    return cuda_status(cudaMemset2DAsync(d->dw, d->dw_stride * size, 0, d->width * size, d->vocab, s), "linear cross entropy: zero dw");
   }
   if (!d->x || !d->w || !d->target || !d->lse || !d->dloss)
     return set_error(PDB_ERR_ARG, "linear cross entropy: null x / w / target / lse / dloss");
   if (!a16(d->x) || !a16(d->w))
     return set_error(PDB_ERR_ALIGN, "linear cross entropy: x and w must be 16-byte aligned");
-  const BwdPlan b = plan_bwd(d->tokens, d->vocab, d->width);
+  const BwdPlan b = plan_bwd(d->tokens, d->vocab, d->width, d->dtype);
   if (!d->workspace || d->workspace_bytes < (size_t)b.bytes || !a16(d->workspace))
     return set_error(PDB_ERR_ARG, "linear cross entropy: workspace too small or not 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(d->workspace);
@@ -942,29 +1187,57 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
   int* state = reinterpret_cast<int*>(ws + b.state);
   int* token_of = reinterpret_cast<int*>(ws + b.token_of);
   const Matrix x{d->x, d->tokens, d->width, d->x_stride}, xp{ws + b.xp, d->tokens, d->width, b.ldp};
-  Pack k{};
-  k.x = static_cast<const __nv_bfloat16*>(d->x);
-  k.target = d->target;
-  k.lse = d->lse;
-  k.dloss = d->dloss;
-  k.tokens = d->tokens;
-  k.width = d->width;
-  k.ldx = d->x_stride;
-  k.dloss_stride = d->dloss_stride;
-  k.ignore = d->ignore_index;
-  k.rows = (int)div_up(d->tokens, 2 * sms());
-  k.pack = d->width % 64 != 0;
-  k.xp = reinterpret_cast<__nv_bfloat16*>(ws + b.xp);
-  k.ldp = b.ldp;
-  k.targetp = reinterpret_cast<int64_t*>(ws + b.target);
-  k.lsep = reinterpret_cast<float*>(ws + b.lse);
-  k.dlossp = reinterpret_cast<float*>(ws + b.dloss);
-  k.token_of = token_of;
-  k.state = state;
-  k.unit = unit;
-  k.dx = static_cast<__nv_bfloat16*>(d->dx);
-  k.lddx = d->dx_stride;
-  if (int st = launch(linear_ce_pack_kernel, div_up(d->tokens, k.rows), kPackThreads, 0, 1, s, k)) return st;
+  const int64_t* target = reinterpret_cast<const int64_t*>(ws + b.target);
+  const float *lse = reinterpret_cast<const float*>(ws + b.lse), *dloss = reinterpret_cast<const float*>(ws + b.dloss);
+  if (int st = d->dtype == PDB_F32 ? pack<float>(*d, b, ws, s) : pack<__nv_bfloat16>(*d, b, ws, s)) return st;
+  if (d->dtype == PDB_F32) {
+    for (int64_t i = 0; i < b.pieces; ++i) {
+      const int64_t v0 = i * b.piece, nv = std::min(b.piece, d->vocab - v0);
+      const Matrix w{static_cast<const float*>(d->w) + v0 * d->w_stride, nv, d->width, d->w_stride};
+      const Matrix g{ws, d->tokens, nv, b.piece};
+      F32Args p = f32_product(x, w, d->tokens, nv, d->width);
+      p.xp = static_cast<const float*>(xp.p);
+      p.ldp = xp.ld;
+      p.state = state;
+      p.dyn = 1;
+      p.target = target;
+      p.col0 = v0;
+      p.vocab = d->vocab;
+      p.lse = lse;
+      p.dloss = dloss;
+      p.out = reinterpret_cast<float*>(ws);
+      p.ldo = b.piece;
+      if (int st = f32_gemm<false, false, kDlogits>(p, s)) return st;
+      if (d->dw) {
+        F32Args q = f32_product(g, x, nv, d->width, d->tokens);
+        q.xp = p.xp;
+        q.ldp = p.ldp;
+        q.state = state;
+        q.dyn = 2;
+        float* dw = static_cast<float*>(d->dw) + v0 * d->dw_stride;
+        q.splits = b.dw_splits;
+        q.out = q.splits > 1 ? dw_acc : dw;
+        q.ldo = q.splits > 1 ? d->width : d->dw_stride;
+        if (int st = f32_gemm<true, true, kOut>(q, s)) return st;
+        if (q.splits > 1)
+          if (int st = join(dw_acc, q.splits, nv, d->width, nullptr, nullptr, nullptr, dw, d->dw_stride, s)) return st;
+      }
+      if (d->dx) {
+        F32Args q = f32_product(g, w, d->tokens, d->width, nv);
+        q.state = state;
+        q.dyn = 1;
+        q.splits = b.dx_splits;
+        q.token_of = q.splits > 1 ? nullptr : token_of;
+        q.out = q.splits > 1 ? dx_acc : static_cast<float*>(d->dx);
+        q.ldo = q.splits > 1 ? d->width : d->dx_stride;
+        q.add = i > 0;
+        if (int st = f32_gemm<false, true, kOut>(q, s)) return st;
+      }
+    }
+    if (d->dx && b.dx_splits > 1)
+      return join(dx_acc, b.dx_splits, d->tokens, d->width, nullptr, state, token_of, static_cast<float*>(d->dx), d->dx_stride, s);
+    return PDB_OK;
+  }
   for (int64_t i = 0; i < b.pieces; ++i) {
     const int64_t v0 = i * b.piece, nv = std::min(b.piece, d->vocab - v0);
     const Matrix w{static_cast<const __nv_bfloat16*>(d->w) + v0 * d->w_stride, nv, d->width, d->w_stride};
@@ -977,11 +1250,11 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
     p.kb_split = (int)div_up(d->width, TK);
     p.state = state;
     p.dyn = 1;
-    p.target = k.targetp;
+    p.target = target;
     p.col0 = v0;
     p.vocab = d->vocab;
-    p.lse = k.lsep;
-    p.dloss = k.dlossp;
+    p.lse = lse;
+    p.dloss = dloss;
     p.unit = unit;
     CUtensorMap tc;
     if (int st = map2d(&tc, g, 64, 32)) return st;
@@ -999,7 +1272,9 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
       float* acc = b.dw_splits > 1 ? dw_acc : nullptr;
       if (int st = gemm_out<true, true>(g, x, dw, acc, xp, q, s)) return st;
       if (acc)
-        if (int st = join(acc, q.splits, q.m, q.n, unit, nullptr, nullptr, const_cast<void*>(dw.p), dw.ld, s)) return st;
+        if (int st = join<__nv_bfloat16>(acc, q.splits, q.m, q.n, unit, nullptr, nullptr,
+                                         static_cast<__nv_bfloat16*>(d->dw) + v0 * d->dw_stride, dw.ld, s))
+          return st;
     }
     if (d->dx) {
       Args q{};
@@ -1019,6 +1294,7 @@ extern "C" int pdb_linear_ce_bwd(const pdb_linear_ce_bwd_desc* d, void* stream) 
     }
   }
   if (d->dx && (b.dx_splits > 1 || b.pieces > 1))
-    return join(dx_acc, b.dx_splits, d->tokens, d->width, unit, state, token_of, d->dx, d->dx_stride, s);
+    return join(dx_acc, b.dx_splits, d->tokens, d->width, unit, state, token_of, static_cast<__nv_bfloat16*>(d->dx),
+                d->dx_stride, s);
   return PDB_OK;
 }

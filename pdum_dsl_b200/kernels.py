@@ -446,9 +446,10 @@ def pointwise(x: torch.Tensor, program, out: torch.Tensor | None = None) -> torc
 
 
 def _head_operand(t: torch.Tensor) -> torch.Tensor:
-    """A 2-D bf16 matrix as the tensor maps take it: 16-byte aligned rows with unit stride, laid out anew otherwise."""
+    """A 2-D matrix as the products take it: 16-byte aligned rows with unit stride, laid out anew otherwise."""
     R, W = t.shape
-    ok = t.data_ptr() % 16 == 0 and (W <= 1 or t.stride(1) == 1) and (R <= 1 or (t.stride(0) >= W and t.stride(0) % 8 == 0))
+    ok = t.data_ptr() % 16 == 0 and (W <= 1 or t.stride(1) == 1) and (
+        R <= 1 or (t.stride(0) >= W and t.stride(0) * t.element_size() % 16 == 0))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -458,8 +459,8 @@ def _head_stride(t: torch.Tensor) -> int:
 
 def _head_args(what: str, x, weight, target):
     _need_cuda(x, weight, target)
-    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
-        raise TypeError(f"{what}: x and weight must be bfloat16, got {x.dtype} / {weight.dtype}")
+    if x.dtype not in _DTYPES or weight.dtype != x.dtype:
+        raise TypeError(f"{what}: x and weight must both be bfloat16 or float32, got {x.dtype} / {weight.dtype}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1]:
         raise ValueError(f"{what}: incompatible x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)}")
     if target.dtype != torch.int64:
@@ -475,7 +476,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
                          return_lse: bool = False):
     """The cross entropy of a linear head, per token, without storing its logits.
 
-    x (..., width) and weight (vocab, width) bf16, width a multiple of 8; target (...) int64.  Returns the float32
+    x (..., width) and weight (vocab, width) bf16 (tcgen05 products) or f32 (IEEE), rows of whole 16 bytes (width a
+    multiple of 8, or of 4); target (...) int64.  Returns the float32
     loss logsumexp_v(x . weight[v]) - x . weight[target], 0 where the target is ``ignore_index`` and NaN where it is
     another index outside the vocabulary; with ``return_lse`` (loss, lse), which the backward takes."""
     x2, w, t = _head_args("linear_cross_entropy", x, weight, target)
@@ -483,7 +485,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     loss = x.new_empty(x.shape[:-1], dtype=torch.float32)
     lse = torch.empty_like(loss)
     d = _lib.LinearCeFwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), None, 0,
-                             N, w.shape[0], W, _head_stride(x2), _head_stride(w), int(ignore_index), _lib.PDB_BF16, 0)
+                             N, w.shape[0], W, _head_stride(x2), _head_stride(w), int(ignore_index), _DTYPES[x.dtype], 0)
     lib = load()
     with _on_device_of(x):
         ws = x.new_empty(lib.pdb_linear_ce_fwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8)
@@ -495,7 +497,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, dloss: torch.Tensor,
                                   lse: torch.Tensor | None = None, *, ignore_index: int = -100, need_dx: bool = True,
                                   need_dweight: bool = True):
-    """(dx, dweight) of linear_cross_entropy, bf16, from the per-token float32 gradient of the loss.
+    """(dx, dweight) of linear_cross_entropy, of x's dtype, from the per-token float32 gradient of the loss.
 
     ``dloss`` broadcasts to target's shape (for a mean over n tokens: a tensor holding 1 / n); ``lse`` None recomputes
     it.  A gradient that is not needed is None."""
@@ -519,7 +521,7 @@ def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target:
     dw = x.new_empty((V, W)) if need_dweight else None
     d = _lib.LinearCeBwdDesc(x2.data_ptr(), w.data_ptr(), t.data_ptr(), lse.data_ptr(), g.data_ptr(),
                              dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dweight else None, None, 0,
-                             N, V, W, _head_stride(x2), _head_stride(w), W, W, gs, int(ignore_index), _lib.PDB_BF16, 0)
+                             N, V, W, _head_stride(x2), _head_stride(w), W, W, gs, int(ignore_index), _DTYPES[x.dtype], 0)
     lib = load()
     with _on_device_of(x):
         ws = x.new_empty(lib.pdb_linear_ce_bwd_workspace_size(C.byref(d)) + 16, dtype=torch.uint8)

@@ -153,7 +153,9 @@ def test_linear_cross_entropy_refusals():
                      ({"width": 0}, _lib.PDB_ERR_SHAPE), ({"tokens": (1 << 24) + 1}, _lib.PDB_ERR_SHAPE),
                      ({"vocab": 1 << 40}, _lib.PDB_ERR_SHAPE), ({"width": 1 << 17, "x_stride": 1 << 17}, _lib.PDB_ERR_SHAPE),
                      ({"width": 60}, _lib.PDB_ERR_ALIGN), ({"x_stride": 68}, _lib.PDB_ERR_ALIGN),
-                     ({"w_stride": 56}, _lib.PDB_ERR_ALIGN), ({"dtype": _lib.PDB_F32}, _lib.PDB_ERR_UNSUPPORTED),
+                     ({"w_stride": 56}, _lib.PDB_ERR_ALIGN), ({"dtype": 2}, _lib.PDB_ERR_UNSUPPORTED),
+                     ({"dtype": _lib.PDB_F32, "width": 62}, _lib.PDB_ERR_ALIGN),
+                     ({"dtype": _lib.PDB_F32, "x_stride": 66}, _lib.PDB_ERR_ALIGN),
                      ({"x": None}, _lib.PDB_ERR_ARG), ({"target": None}, _lib.PDB_ERR_ARG)):
         for d, run, size in ((_ce(**kw), lib.pdb_linear_ce_fwd, lib.pdb_linear_ce_fwd_workspace_size),
                              (_ce_bwd(**kw), lib.pdb_linear_ce_bwd, lib.pdb_linear_ce_bwd_workspace_size)):

@@ -3,8 +3,8 @@
 Tolerances, u = 2^-24.  A logit, a dot product of `width` bf16 products summed in f32, is off by at most
 e = (width + 16) u sum|x w|.  exp takes an approximation of 2^-22 and a rounded argument of 2 u |logit|; a row's sum
 of `vocab` positive terms takes at most 8 + vocab / 4096 + 140 steps, so lse is off by
-e + 2^-21 + (150 + vocab / 4096) u + 4 u |lse|.  G is rounded to bf16 (half a step, 2^-8 of itself) after a
-probability with the same relative error; the products that follow sum in f32 and round once more.
+e + 2^-21 + (150 + vocab / 4096) u + 4 u |lse|.  G is rounded to the operands' type (half a step: bf16 2^-8 of itself,
+f32 u) after a probability with the same relative error; the products that follow sum in f32 and round once more.
 """
 
 import pytest
@@ -15,7 +15,7 @@ U = 2.0 ** -24
 IGN = -100
 
 
-def _inputs(dev, N, V, W, seed, ignored=0.2, spread=1.5):
+def _inputs(dev, N, V, W, seed, ignored=0.2, spread=1.5, dtype="bfloat16"):
     import torch
 
     g = torch.Generator(device="cpu").manual_seed(seed)
@@ -25,7 +25,8 @@ def _inputs(dev, N, V, W, seed, ignored=0.2, spread=1.5):
     x[::2] += 1.5 * w[t[::2]]
     t[torch.rand(N, generator=g) < ignored] = IGN
     dl = torch.randn(N, generator=g) / max(N, 1)
-    return x.to(torch.bfloat16).to(dev), w.to(torch.bfloat16).to(dev), t.to(dev), dl.to(dev)
+    dtype = getattr(torch, dtype)
+    return x.to(dtype).to(dev), w.to(dtype).to(dev), t.to(dev), dl.to(dev)
 
 
 def _logits(x, w):
@@ -53,6 +54,8 @@ def _check_backward(x, w, t, dl, lse, dx, dw):
 
     N, W = x.shape
     V = w.shape[0]
+    half = torch.finfo(x.dtype).eps / 2
+    assert all(t is None or t.dtype == x.dtype for t in (dx, dw))
     z, e = _logits(x, w)
     valid = t != IGN
     up = (dl.double() * valid)[:, None]
@@ -62,16 +65,16 @@ def _check_backward(x, w, t, dl, lse, dx, dw):
     G = p.clone()
     G.scatter_add_(1, t.clamp(min=0)[:, None], torch.full((N, 1), -1.0, dtype=torch.float64, device=x.device))
     G *= up
-    gerr = up.abs() * (perr + 3 * U) * 1.01 + 2.0 ** -8 * G.abs()
+    gerr = up.abs() * (perr + 3 * U) * 1.01 + half * G.abs()
     wd, xd = w.double(), x.double()
     if dx is not None:
         ref = G @ wd
-        tol = (gerr + (V + 16) * U * G.abs()) @ wd.abs() * 1.01 + 2.0 ** -8 * ref.abs() + 1e-38
+        tol = (gerr + (V + 16) * U * G.abs()) @ wd.abs() * 1.01 + half * ref.abs() + 1e-38
         assert ((dx.double() - ref).abs() <= tol).all(), ((dx.double() - ref).abs() / tol).max()
         assert (dx[~valid] == 0).all()
     if dw is not None:
         ref = G.T @ xd
-        tol = (gerr + (N + 16) * U * G.abs()).T @ xd.abs() * 1.01 + 2.0 ** -8 * ref.abs() + 1e-38
+        tol = (gerr + (N + 16) * U * G.abs()).T @ xd.abs() * 1.01 + half * ref.abs() + 1e-38
         assert ((dw.double() - ref).abs() <= tol).all(), ((dw.double() - ref).abs() / tol).max()
 
 
@@ -80,10 +83,11 @@ SHAPES = [(1, 1, 8), (1, 500, 64), (3, 257, 72), (130, 1000, 128), (257, 256, 64
 
 
 @pytest.mark.parametrize("N,V,W", SHAPES)
-def test_loss_and_gradients(cuda, N, V, W):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_loss_and_gradients(cuda, N, V, W, dtype):
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, N, V, W, N + V + W, ignored=0.2 if N > 1 else 0.0)
+    x, w, t, dl = _inputs(cuda, N, V, W, N + V + W, ignored=0.2 if N > 1 else 0.0, dtype=dtype)
     loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     kernels.check_device_errors()
     _check_forward(x, w, t, loss, lse)
@@ -92,13 +96,14 @@ def test_loss_and_gradients(cuda, N, V, W):
     _check_backward(x, w, t, dl, lse, dx, dw)
 
 
-def test_several_pieces(cuda):
+@pytest.mark.parametrize("N,dtype", [(8192, "bfloat16"), (4096, "float32")])
+def test_several_pieces(cuda, N, dtype):
     """A vocabulary that one piece of the gradient's workspace does not hold."""
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 8192, 70001, 16, 1)
+    x, w, t, dl = _inputs(cuda, N, 70001, 16, 1, dtype=dtype)
     loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     _check_forward(x, w, t, loss, lse)
     dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
@@ -106,12 +111,13 @@ def test_several_pieces(cuda):
     _check_backward(x, w, t, dl, lse, dx, dw)
 
 
-def test_one_gradient_alone_and_lse_recomputed(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_one_gradient_alone_and_lse_recomputed(cuda, dtype):
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 200, 900, 128, 2)
+    x, w, t, dl = _inputs(cuda, 200, 900, 128, 2, dtype=dtype)
     _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
     a, none = kernels.linear_cross_entropy_backward(x, w, t, dl, need_dweight=False)
@@ -121,13 +127,14 @@ def test_one_gradient_alone_and_lse_recomputed(cuda):
     assert kernels.linear_cross_entropy_backward(x, w, t, dl, lse, need_dx=False, need_dweight=False) == (None, None)
 
 
-def test_mean_leading_dims_and_strides(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_mean_leading_dims_and_strides(cuda, dtype):
     """One dloss for all tokens; (batch, row) tokens; rows of wider matrices, aligned or not; any ignore index."""
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, _ = _inputs(cuda, 66, 400, 136, 3)
+    x, w, t, _ = _inputs(cuda, 66, 400, 136, 3, dtype=dtype)
     lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)[1]
     mean = torch.full((), 1 / 50, device=cuda)
     dx, dw = kernels.linear_cross_entropy_backward(x, w, t, mean, lse)
@@ -136,7 +143,7 @@ def test_mean_leading_dims_and_strides(cuda):
     assert l3.shape == (6, 11) and torch.equal(e3.view(-1), lse)
     d3, w3 = kernels.linear_cross_entropy_backward(x.view(6, 11, 136), w, t.view(6, 11), mean, e3)
     assert torch.equal(d3.view(66, 136), dx) and torch.equal(w3, dw)
-    for lo, hi in ((0, 128), (8, 136), (1, 129)):
+    for lo, hi in ((0, 128), (8, 136), (1, 129), (4, 132)):
         xs, ws = x[:, lo:hi], w[:, lo:hi]
         ls, es = kernels.linear_cross_entropy(xs, ws, t, return_lse=True)
         _check_forward(xs, ws, t, ls, es)
@@ -149,12 +156,13 @@ def test_mean_leading_dims_and_strides(cuda):
     assert (l0[~keep] == 0).all() and torch.equal(l0[keep], kernels.linear_cross_entropy(x, w, t)[keep])
 
 
-def test_nothing_to_do(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_nothing_to_do(cuda, dtype):
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 40, 300, 64, 4)
+    x, w, t, dl = _inputs(cuda, 40, 300, 64, 4, dtype=dtype)
     t[:] = IGN
     loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     assert (loss == 0).all()
@@ -170,12 +178,13 @@ def test_nothing_to_do(cuda):
     assert loss.shape == (0,) and dx.shape == (0, 64) and dw.shape == w.shape and (dw == 0).all()
 
 
-def test_targets_outside_the_vocabulary_give_nan(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_targets_outside_the_vocabulary_give_nan(cuda, dtype):
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 40, 300, 64, 5, ignored=0.0)
+    x, w, t, dl = _inputs(cuda, 40, 300, 64, 5, ignored=0.0, dtype=dtype)
     good = kernels.linear_cross_entropy(x, w, t)
     for bad in (300, -1, 2 ** 40, -(2 ** 62)):
         t2 = t.clone()
@@ -186,23 +195,25 @@ def test_targets_outside_the_vocabulary_give_nan(cuda):
         assert dx[11].isnan().all() and dx[:11].isfinite().all() and dx[12:].isfinite().all()
 
 
-def test_large_logits(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_large_logits(cuda, dtype):
     """Logits of hundreds, one entry holding all of a row's probability; nothing overflows."""
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 129, 600, 64, 6, spread=150.0)
+    x, w, t, dl = _inputs(cuda, 129, 600, 64, 6, spread=150.0, dtype=dtype)
     loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     _check_forward(x, w, t, loss, lse)
     dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
     _check_backward(x, w, t, dl, lse, dx, dw)
 
 
-def test_the_same_bits_every_time_on_two_streams_and_in_a_graph(cuda):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_the_same_bits_every_time_on_two_streams_and_in_a_graph(cuda, dtype):
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, 700, 5000, 256, 7)
+    x, w, t, dl = _inputs(cuda, 700, 5000, 256, 7, dtype=dtype)
 
     def both():
         loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
@@ -221,7 +232,7 @@ def test_the_same_bits_every_time_on_two_streams_and_in_a_graph(cuda):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = both()
-    x2, _, t2, dl2 = _inputs(cuda, 700, 5000, 256, 8)
+    x2, _, t2, dl2 = _inputs(cuda, 700, 5000, 256, 8, dtype=dtype)
     x.copy_(x2), t.copy_(t2), dl.copy_(dl2)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(held, both()))
@@ -279,14 +290,15 @@ def test_a_mean_does_not_scale_the_gradient(cuda, n):
 
 @pytest.mark.parametrize("N,V,W,count", [(300, 700, 72, 1), (300, 700, 72, 33), (300, 700, 72, 64), (300, 700, 72, 299),
                                          (513, 20000, 256, 255), (2000, 300, 64, 129), (700, 40000, 40, 350), (40, 700, 64, 7)])
-def test_ignored_tokens_hold_anything(cuda, N, V, W, count):
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_ignored_tokens_hold_anything(cuda, N, V, W, count, dtype):
     """Infinities and NaN in the rows, lse and dloss of ignored tokens (a padded batch) reach no gradient, for counts that
     end inside and on the products' blocks; the gradients are those of the remaining tokens alone."""
     import torch
 
     from pdum_dsl_b200 import kernels
 
-    x, w, t, dl = _inputs(cuda, N, V, W, N + count, ignored=0.0)
+    x, w, t, dl = _inputs(cuda, N, V, W, N + count, ignored=0.0, dtype=dtype)
     _, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
     keep = torch.zeros(N, dtype=torch.bool, device=cuda)
     keep[torch.randperm(N, generator=torch.Generator().manual_seed(count))[:count].to(cuda)] = True

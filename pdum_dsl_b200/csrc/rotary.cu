@@ -284,9 +284,14 @@ extern "C" int pdb_rotary(const pdb_rotary_desc* d, void* stream) {
       if (dims[k] > 1) {
         fit(p.xs[w][k]);
         fit(p.ys[w][k]);
+        if (p.x[w] == p.y[w] && p.xs[w][k] != p.ys[w][k])
+          return set_error(PDB_ERR_ARG, "rotary: a tensor turned in place has one set of strides");
       }
     }
   }
+  // threads read and write in no order between heads: a result that starts where another tensor does is a mistake
+  if (p.heads[0] && p.heads[1] && (p.y[0] == p.y[1] || p.y[0] == p.x[1] || p.y[1] == p.x[0]))
+    return set_error(PDB_ERR_ARG, "rotary: a result overlaps the other tensor");
   p.pos = d->positions;
   p.ps[0] = d->pos_stride[0];
   p.ps[1] = d->pos_stride[1];

@@ -290,7 +290,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
     pass through.  ``inv_freq`` is a host sequence of up to 128 numbers (see ``rotary_frequencies``).
     ``positions`` is an integer CUDA tensor (T,) or (B, T) (either may be broadcast), else row t has position
     start + t.  ``inverse`` turns backwards: the gradient of the forward turn.  ``out`` (a tensor, or a pair with k)
-    may be the inputs themselves.  Returns the turned q, or (q, k)."""
+    may be the inputs themselves, and shares no memory otherwise.  Returns the turned q, or (q, k)."""
     ts = (q,) if k is None else (q, k)
     _need_cuda(*ts)
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):

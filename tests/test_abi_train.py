@@ -129,6 +129,17 @@ def test_rotary_refusals():
     d = _rot()
     d.heads[1] = 1
     assert lib.pdb_rotary(C.byref(d), None) == _lib.PDB_ERR_ARG
+    # in place with other strides, and results that are another tensor
+    d = _rot()
+    d.x_stride[0][:], d.y_stride[0][:] = (256, 64, 128), (256, 128, 64)
+    assert lib.pdb_rotary(C.byref(d), None) == _lib.PDB_ERR_ARG
+    assert b"in place" in lib.pdb_last_error_string()
+    for x, y in (((16, 16), (16, 16)), ((16, 4096), (8192, 8192)), ((16, 4096), (4096, 8192)), ((16, 4096), (8192, 16))):
+        d = _rot()
+        d.heads[1] = 2
+        d.x[:], d.y[:] = x, y
+        assert lib.pdb_rotary(C.byref(d), None) == _lib.PDB_ERR_ARG
+        assert b"overlaps" in lib.pdb_last_error_string()
 
 
 def _ce(**kw):

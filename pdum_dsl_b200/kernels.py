@@ -67,19 +67,32 @@ def _param_dtype(what: str, x: torch.Tensor, cols: int, gamma, beta) -> torch.dt
     return ptype or torch.float32
 
 
-def _out_rows(what: str, out: torch.Tensor, x2: torch.Tensor) -> torch.Tensor:
-    if out.dtype != x2.dtype or out.device != x2.device or out.numel() != x2.numel():
+def _out_rows(what: str, out: torch.Tensor, x: torch.Tensor, R: int, C_: int) -> tuple[torch.Tensor, int]:
+    """out for the row kernels, and its row stride."""
+    if out.dtype != x.dtype or out.device != x.device or out.numel() != x.numel():
         raise ValueError(f"{what}: out must have x's size, dtype and device")
-    y = out.view(x2.shape)
-    if y.shape[-1] > 1 and y.stride(-1) != 1:
+    if out.is_contiguous():
+        return out, C_
+    y = out.view(R, C_)
+    if C_ > 1 and y.stride(-1) != 1:
         raise ValueError(f"{what}: out must have unit stride along its last dim")
-    return y
+    return y, y.stride(0)
 
 
 def _own_rows(x: torch.Tensor) -> torch.Tensor:
     """x as 2-D rows that do not overlap (an expanded gradient is laid out first)."""
     x2 = _rows2d(x)
     return x2.contiguous() if x2.shape[0] > 1 and x2.stride(0) < x2.shape[1] else x2
+
+
+def _rows(x: torch.Tensor, as_2d=_own_rows) -> tuple[torch.Tensor, int, int, int]:
+    """(x, rows, cols, row stride) for the row kernels; a contiguous x as it is (a view is as dear as an allocation)."""
+    if x.is_contiguous() and x.dim():
+        C_ = x.shape[-1]
+        return x, x.numel() // C_ if C_ else math.prod(x.shape[:-1]), C_, C_
+    x2 = as_2d(x)
+    R, C_ = x2.shape
+    return x2, R, C_, x2.stride(0)
 
 
 def row_softmax(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -104,28 +117,25 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Te
     _need_cuda(x)
     if x.dtype not in _DTYPES:
         raise TypeError("layernorm: float32 or bfloat16")
-    x2 = _rows2d(x)
-    R, C_ = x2.shape
+    plain = x.dtype == torch.float32 and not return_stats  # and f32 parameters
+    x2, R, C_, xs = _rows(x, _rows2d if plain else _own_rows)
     ptype = _param_dtype("layernorm", x, C_, gamma, beta)
     g = gamma.contiguous() if gamma is not None else None
     b = beta.contiguous() if beta is not None else None
     at_g, at_b = g.data_ptr() if g is not None else None, b.data_ptr() if b is not None else None
-    if x.dtype == torch.float32 and ptype == torch.float32 and not return_stats:
-        y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
-        d = LayerNormDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), R, C_, x2.stride(0) if R else C_,
-                          y.stride(0) if R else C_, float(eps))
+    y, ys = (torch.empty_like(x2), C_) if out is None else _out_rows("layernorm", out, x, R, C_)
+    if plain:
+        d = LayerNormDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), R, C_, xs if R else C_, ys if R else C_, float(eps))
         with _on_device_of(x):
             check(load().pdb_layernorm_f32(C.byref(d), _stream(x)), "pdb_layernorm_f32")
         return y.view(x.shape)
-    x2 = _own_rows(x2)
-    y = torch.empty_like(x2) if out is None else _out_rows("layernorm", out, x2)
     mean = rstd = at_m = at_r = None
     if return_stats:
-        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        mean = x.new_empty(R if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
         at_m, at_r = mean.data_ptr(), rstd.data_ptr()
-    d = _lib.LayerNormFwdDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), at_m, at_r, R, C_, x2.stride(0), y.stride(0),
-                              eps, _DTYPES[x.dtype], _DTYPES[ptype])
+    d = _lib.LayerNormFwdDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), at_m, at_r, R, C_, xs, ys, eps,
+                              _DTYPES[x.dtype], _DTYPES[ptype])
     with _on_device_of(x):
         check(load().pdb_layernorm_fwd(C.byref(d), _raw_stream(x)), "pdb_layernorm_fwd")
     if y.shape != x.shape:
@@ -144,8 +154,8 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
         raise TypeError("layernorm_backward: dout and x must both be float32 or bfloat16")
     if dout.shape != x.shape:
         raise ValueError(f"layernorm_backward: dout {tuple(dout.shape)} does not match x {tuple(x.shape)}")
-    x2, do2 = _own_rows(x), _own_rows(dout)
-    R, C_ = x2.shape
+    x2, R, C_, xs = _rows(x)
+    do2, _, _, dos = _rows(dout)
     for nm, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.numel() != R or t.device != x.device:
             raise ValueError(f"layernorm_backward: {nm} must be the forward's float32 statistic of {R} rows")
@@ -158,11 +168,11 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
     dgamma = dbeta = None
     d = _lib.LayerNormBwdDesc(do2.data_ptr(), x2.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                               g.data_ptr() if g is not None else None, dx.data_ptr(), None, None, None, 0, R, C_,
-                              do2.stride(0), x2.stride(0), C_, _DTYPES[x.dtype], _DTYPES[ptype])
+                              dos, xs, C_, _DTYPES[x.dtype], _DTYPES[ptype])
     lib = load()
     with _on_device_of(x):
         if weight_grads:
-            dgamma = x.new_empty((C_,), dtype=ptype)
+            dgamma = x.new_empty(C_, dtype=ptype)
             dbeta = torch.empty_like(dgamma)
             d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
             nbytes = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
@@ -333,7 +343,12 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
         amplitude, freq.tobytes(), bool(interleaved), bool(inverse), _DTYPES[q.dtype], 0))
     with _on_device_of(q):
         check(load().pdb_rotary(C.byref(d), _raw_stream(q)), "pdb_rotary")
-    rets = tuple(y if y.shape == t.shape else y.view(t.shape) for y, t in zip(ys, ts)) if out is None else outs
+    if out is not None:
+        rets = outs
+    elif q.dim() == 4 == ts[-1].dim():
+        rets = tuple(ys)
+    else:
+        rets = tuple(y.view(t.shape) for y, t in zip(ys, ts))
     return rets[0] if k is None else rets
 
 

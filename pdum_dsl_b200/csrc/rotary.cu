@@ -303,7 +303,7 @@ extern "C" int pdb_rotary(const pdb_rotary_desc* d, void* stream) {
     const double f = d->inv_freq[j], per = std::fabs(f) / 6.283185307179586476925286766559;  // turns per position
     if (!(per < 1e9)) return set_error(PDB_ERR_ARG, "rotary: inv_freq[%d] is not a usable frequency", j);
     // whole turns per position change nothing; a backward turn is the negated integer
-    const uint64_t turns = (uint64_t)std::ldexp(per - std::floor(per), 64);
+    const uint64_t turns = (uint64_t)((per - (double)(int64_t)per) * 0x1p64);
     p.turns[j] = (f < 0) != (d->inverse != 0) ? 0 - turns : turns;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -396,7 +396,8 @@ int pdb_rotary(const pdb_rotary_desc* d, void* stream);
  * there).  x [tokens, width] hidden states, w [vocab, width] the head's weight,
  * both bf16 (tcgen05 products, f32 accumulate) or both f32 (IEEE multiply-adds,
  * the precision of the reference's f32 column), width and row strides multiples
- * of 16 bytes; logit[n, v] = x[n] . w[v] in f32, never stored:
+ * of 16 bytes; logit[n, v] = x[n] . w[v] in f32 (beyond 2^127 it may count as
+ * infinite), never stored:
  *   lse[n]  = log sum_v exp(logit[n, v])
  *   loss[n] = lse[n] - logit[n, target[n]]
  * loss and lse are f32 [tokens], either may be NULL.  target is int64 [tokens] on

@@ -282,3 +282,23 @@ def test_in_place(cuda, C, t):
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
         _lib.check(lib.pdb_layernorm_bwd(CT.byref(d), torch.cuda.current_stream().cuda_stream), "pdb_layernorm_bwd")
         assert torch.equal(dx, want[0]) and torch.equal(dw[0], want[1]) and torch.equal(dw[1], want[2])
+
+
+@pytest.mark.parametrize("C", [512, 777])
+def test_rows_that_lie_beyond_32_bits(cuda, C):
+    """Five rows 2^30 + 1 elements apart: offsets pass 2^32 elements, and a row's place against 16 bytes changes."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, dy, gam, bet = _inputs(cuda, 5, C, torch.bfloat16, torch.float32, C)
+    far = torch.empty(4 * (2 ** 30 + 1) + C, dtype=torch.bfloat16, device=cuda)
+    for away in (2 ** 30 + 1, 2 ** 30):
+        xs = far.as_strided((5, C), (away, 1))
+        xs.copy_(x)
+        y, mean, rstd = kernels.layernorm(xs, gam, bet, return_stats=True)
+        _check_forward(xs, gam, bet, 1e-5, y, mean, rstd)
+        dx, dg, db = kernels.layernorm_backward(dy, xs, mean, rstd, gam)
+        _check_backward(xs, dy, mean, rstd, gam, dx, dg, db)
+        out = kernels.layernorm(x, gam, bet, out=xs)
+        assert torch.equal(out, kernels.layernorm(x, gam, bet)) and torch.equal(xs, out)

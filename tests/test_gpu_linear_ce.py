@@ -323,3 +323,47 @@ def test_ignored_tokens_over_several_pieces(cuda):
     dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
     kernels.check_device_errors()
     _check_backward(x, w, t, dl, lse, dx, dw)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_rows_that_lie_beyond_32_bits(cuda, dtype):
+    """Rows of x 2^31 and of the weight 2^24 elements apart: offsets pass 2^32 elements."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 3, 300, 72, 13, ignored=0.0, dtype=dtype)
+    far = torch.empty(299 * 2 ** 24 + 2 ** 20, dtype=x.dtype, device=cuda)
+    xs, ws = far[1024:].as_strided((3, 72), (2 ** 31, 1)), far.as_strided((300, 72), (2 ** 24, 1))
+    xs.copy_(x), ws.copy_(w)
+    for t in (t, torch.tensor([IGN, 299, 0], device=cuda)):
+        loss, lse = kernels.linear_cross_entropy(xs, ws, t, return_lse=True)
+        _check_forward(x, w, t, loss, lse)
+        dx, dw = kernels.linear_cross_entropy_backward(xs, ws, t, dl, lse)
+        kernels.check_device_errors()
+        _check_backward(x, w, t, dl, lse, dx, dw)
+
+
+@pytest.mark.parametrize("lowest", [True, False])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_masked_entries(cuda, dtype, lowest):
+    """Entries whose logits are the type's lowest value, or minus infinity (forward alone: its gradient multiplies them),
+    whole tiles of them: the loss and the gradients are those of the other entries alone."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, w, t, dl = _inputs(cuda, 150, 1000, 72, 14, dtype=dtype)
+    live = torch.zeros(1000, dtype=torch.bool, device=cuda)
+    live[300:420] = live[999] = True
+    x[:, 0] = 1.0
+    w[:, 0] = torch.where(live, 0.0, torch.finfo(w.dtype).min if lowest else -float("inf"))
+    few = torch.where(t == IGN, IGN, t % 121)  # among the entries that count, and in the whole vocabulary
+    t = torch.where(few == IGN, IGN, torch.where(few == 120, 999, few + 300))
+    loss, lse = kernels.linear_cross_entropy(x, w, t, return_lse=True)
+    _check_forward(x, w[live], few, loss, lse)
+    if lowest:
+        dx, dw = kernels.linear_cross_entropy_backward(x, w, t, dl, lse)
+        _check_backward(x, w[live], few, dl, lse, dx, dw[live])
+        assert (dw[~live] == 0).all()
+    kernels.check_device_errors()

@@ -182,3 +182,23 @@ def test_in_a_graph(cuda):
         pos += 1
         graph.replay()
         assert torch.equal(out, kernels.rotary(q, inv_freq=f, positions=pos))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_heads_that_lie_beyond_32_bits(cuda, interleaved):
+    """Strides of 2^31 and 2^30 elements between batches, heads and rows, read and written in place."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    f, _ = kernels.rotary_frequencies(64)
+    x = _draw(cuda, (2, 2, 3, 64), "bfloat16", 9)
+    pos = torch.arange(3, device=cuda).expand(2, 3)
+    far = torch.empty(2 ** 32 + 2 ** 31 + 4096, dtype=torch.bfloat16, device=cuda)
+    for strides in ((2 ** 32, 2 ** 31, 64, 1), (64 * 3, 2 ** 32, 64, 1), (128, 64, 2 ** 31, 1)):
+        xs = far.as_strided((2, 2, 3, 64), strides)
+        xs.copy_(x)
+        got = kernels.rotary(xs, inv_freq=f, interleaved=interleaved)
+        _check(got, x, f, pos, interleaved)
+        kernels.rotary(xs, inv_freq=f, interleaved=interleaved, out=xs)
+        assert torch.equal(xs, got)

@@ -84,32 +84,47 @@ struct BwdArgs {
   float inv_cols;
 };
 
-// Sum over the TPR threads of a row.  Up to a warp: shuffles.  More: each warp
-// leaves its sum in one of two buffers that alternate from row to row, so one
-// barrier of the row's own threads is enough (a buffer is written again only
-// after the barrier of the row between).
+// Sum over the TPR threads of a row.  Up to a warp: shuffles; of two sums, the halves of the row's lanes take one each
+// after the first step.  More: each warp leaves its sums in one of two buffers that alternate from row to row, so one
+// barrier of the row's own threads is enough (a buffer is written again only after the barrier of the row between).
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int slot, int& phase) {
-  constexpr int W = TPR < 32 ? TPR : 32;
+  static_assert(N <= 2 && TPR >= 8, "one or two sums");
+  constexpr int W = TPR < 32 ? TPR : 32, NW = TPR / 32;
+  const bool up = N == 2 && (threadIdx.x & (W / 2));
+  float s = up ? v[N - 1] : v[0];
+  s += __shfl_xor_sync(0xffffffffu, N == 1 || up ? v[0] : v[N - 1], W / 2);
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-  if constexpr (TPR > 32) {
-    constexpr int NW = TPR / 32;
+  for (int o = W / 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if constexpr (TPR <= 32) {
+    if constexpr (N == 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, s, W / 2);
+      v[0] = up ? other : s;
+      v[1] = up ? s : other;
+    } else {
+      v[0] = s;
+    }
+  } else {
     float* buf = red + (slot * 2 + phase) * NW * N;
     phase ^= 1;
     const int w = (threadIdx.x % TPR) >> 5, lane = threadIdx.x & 31;
-    if (lane == 0)
-#pragma unroll
-      for (int n = 0; n < N; ++n) buf[w * N + n] = v[n];
+    if (lane % (W / N) == 0) buf[w * N + up] = s;
     asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "n"(TPR) : "memory");
+    if constexpr (N == 2) {
+      uint64_t a = 0, b = 0;  // a pair of zeros
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      float s = 0.f;
+      for (int i = 0; i < NW; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(buf + i * N);
+        a = f2_add(a, q.x), b = f2_add(b, q.y);
+      }
+      f2_unpack(f2_add(a, b), v[0], v[N - 1]);
+    } else {
+      uint64_t a = 0;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) s += buf[i * N + n];
-      v[n] = s;
+      for (int i = 0; i < NW; i += 2) a = f2_add(a, *reinterpret_cast<const uint64_t*>(buf + i));
+      float lo, hi;
+      f2_unpack(a, lo, hi);
+      v[0] = lo + hi;
     }
   }
 }
@@ -410,7 +425,7 @@ __device__ __forceinline__ int row_shift(const void* p, int64_t stride, int cls)
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
-  __shared__ float red[RPB * 2 * NW];
+  __shared__ __align__(16) float red[RPB * 2 * NW];
   extern __shared__ __align__(16) uint8_t dyn[];
   const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
   const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x);
@@ -536,7 +551,7 @@ __global__ void __launch_bounds__(kLoopThreads) layernorm_fwd_loop_kernel(const 
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 constexpr int bwd_smem() {
   const int slots = Rows<T, VEC, NV, TPR, BT, STAGES, 2, RAG>::kBytes;
-  const int sums = BT > TPR ? BT * NV * VEC * (int)sizeof(float) : 0;
+  const int sums = BT * NV * VEC * (int)sizeof(float);
   return slots > sums ? slots : sums;
 }
 
@@ -546,7 +561,7 @@ constexpr int bwd_smem() {
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL>
 __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernorm_bwd_kernel(const BwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
-  __shared__ float red[RPB * 2 * NW * 2], sums[2 * CL * 2];
+  __shared__ __align__(16) float red[RPB * 2 * NW * 2], sums[2 * CL * 2];
   extern __shared__ __align__(16) uint8_t dyn[];
   const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR, rank = CL > 1 ? (int)cluster_rank() : 0;
   const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x / CL);
@@ -612,33 +627,36 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
   if (!p.partial) return;
   const int64_t half = (int64_t)p.groups * p.cols;
   float* out = p.partial + (int64_t)(blockIdx.x / CL) * p.cols;
-  float* columns = reinterpret_cast<float*>(dyn);  // [RPB][TPR * NV * VEC]
+  // Through shared memory, so that a warp writes whole lines (a thread's own columns, stored from its registers, cost
+  // 8 us per call at 16384 columns); a thread's vectors lie there as they do in the row.
   constexpr int WIDTH = TPR * NV * VEC;
+  float* columns = reinterpret_cast<float*>(dyn);  // [RPB][WIDTH]
+  const int first = rank * WIDTH - shift;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float f[NV * VEC];
 #pragma unroll
     for (int e = 0; e < N2; ++e) f2_unpack(which ? ab[e] : ag[e], f[2 * e], f[2 * e + 1]);
-    if constexpr (RPB == 1) {
+    __syncthreads();
 #pragma unroll
-      for (int e = 0; e < NV * VEC; ++e) {
-        const int c = first_col + e / VEC * TPR * VEC + e % VEC;
-        if (c >= 0 && c < p.cols) out[which * half + c] = f[e];
-      }
-    } else {
-      __syncthreads();
+    for (int i = 0; i < NV; ++i) {
+      float* at = columns + slot * WIDTH + (i * TPR + l) * VEC;
+      if constexpr (VEC == 1) {
+        *at = f[i];
+      } else {
 #pragma unroll
-      for (int e = 0; e < NV * VEC; ++e) {
-        const int c = first_col + e / VEC * TPR * VEC + e % VEC;
-        if (c >= 0) columns[slot * WIDTH + c] = f[e];
+        for (int j = 0; j < VEC; j += 4)
+          *reinterpret_cast<float4*>(at + j) = make_float4(f[i * VEC + j], f[i * VEC + j + 1], f[i * VEC + j + 2], f[i * VEC + j + 3]);
       }
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.cols; c += BT) {
-        float s = 0.f;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < WIDTH; e += BT) {
+      const int c = first + e;
+      if (c < 0 || c >= p.cols) continue;
+      float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < RPB; ++r) s += columns[r * WIDTH + c];
-        out[which * half + c] = s;
-      }
+      for (int r = 0; r < RPB; ++r) s += columns[r * WIDTH + e];
+      out[which * half + c] = s;
     }
   }
 }
@@ -684,14 +702,15 @@ __global__ void __launch_bounds__(kColThreads) layernorm_bwd_columns_kernel(cons
   p.partial[((int64_t)p.groups + blockIdx.y) * p.cols + c] = b;
 }
 
-// The partial rows of all blocks, added in a fixed order: a block takes 32 columns
-// of one of the two gradients, its 32 warps a share of the partial rows each, eight
-// loads in flight (one after another, 300 rows took longer than the pass before).
-constexpr int kFinWarps = 32, kFinUnroll = 8;
+// The partial rows of all blocks, added in a fixed order: a block takes 32 columns of one of the two gradients, its warps
+// a share of the partial rows each, eight loads in flight (one after another, 300 rows took longer than the pass before).
+// 32 warps, or 8 where there are columns enough for every SM's threads all the same.
+constexpr int kFinUnroll = 8;
 
-__global__ void __launch_bounds__(32 * kFinWarps)
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
     layernorm_bwd_finish_kernel(const float* partial, int groups, int cols, void* dgamma, void* dbeta, int param_bf16) {
-  __shared__ float s[kFinWarps][33];
+  __shared__ float s[WARPS][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   grid_dep_wait();
@@ -699,22 +718,24 @@ __global__ void __launch_bounds__(32 * kFinWarps)
   float v = 0.f;
   if (c < cols) {
     int r = w;
-    for (; r + (kFinUnroll - 1) * kFinWarps < groups; r += kFinUnroll * kFinWarps) {
+    for (; r + (kFinUnroll - 1) * WARPS < groups; r += kFinUnroll * WARPS) {
       float q[kFinUnroll];
 #pragma unroll
-      for (int i = 0; i < kFinUnroll; ++i) q[i] = src[(int64_t)(r + i * kFinWarps) * cols];
+      for (int i = 0; i < kFinUnroll; ++i) q[i] = src[(int64_t)(r + i * WARPS) * cols];
 #pragma unroll
       for (int i = 0; i < kFinUnroll; ++i) v += q[i];
     }
-    for (; r < groups; r += kFinWarps) v += src[(int64_t)r * cols];
+    for (; r < groups; r += WARPS) v += src[(int64_t)r * cols];
   }
   s[w][lane] = v;
   __syncthreads();
-  // the block's 32 x 32 sums turned: a warp adds one column's 32 shares
-  v = s[lane][w];
+  // the block's sums turned: WARPS neighbouring threads add one column's shares
+  const int col = threadIdx.x / WARPS, share = threadIdx.x % WARPS;
+  v = s[share][col];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0 && blockIdx.x * 32 + w < cols) param_store(blockIdx.y ? dbeta : dgamma, param_bf16, blockIdx.x * 32 + w, v);
+  for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (share == 0 && blockIdx.x * 32 + col < cols)
+    param_store(blockIdx.y ? dbeta : dgamma, param_bf16, blockIdx.x * 32 + col, v);
 }
 
 // ------------------------------------------------------------------- host
@@ -954,14 +975,16 @@ extern "C" int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream) 
   // its blocks may be scheduled while the pass before drains; they wait for that pass's memory
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((d->cols + 31) / 32), 2);
-  cfg.blockDim = dim3(32 * kFinWarps);
+  const bool wide = (int)cfg.gridDim.x > sms();
+  cfg.blockDim = dim3(32 * (wide ? 8 : 32));
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, layernorm_bwd_finish_kernel, (const float*)p.partial,
-                                        d->rows > 0 ? p.groups : 0, p.cols, d->dgamma, d->dbeta, p.param_bf16),
+  return cuda_status(cudaLaunchKernelEx(&cfg, wide ? layernorm_bwd_finish_kernel<8> : layernorm_bwd_finish_kernel<32>,
+                                        (const float*)p.partial, d->rows > 0 ? p.groups : 0, p.cols, d->dgamma, d->dbeta,
+                                        p.param_bf16),
                      "layernorm backward finish launch");
 }

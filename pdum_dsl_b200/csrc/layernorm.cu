@@ -13,6 +13,7 @@
 // the same bytes: forward 8192 x 4096 bf16 26.6 us (24.7), gradients with the
 // weights' 8192 x 4096 f32 69 us (67), 262144 x 128 bf16 38 us (37).
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -167,7 +168,7 @@ struct ClusterSums {
     }
     const bool ok = mbar_wait_cluster(&ready[ph], (n >> 1) & 1, &abort, err);
     if (!__all_sync(0xffffffffu, ok)) return false;
-    float2 q = sums[ph][lane];
+    float2 q = CL * NW >= 32 || lane < CL * NW ? sums[ph][lane] : make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 32; i < CL * NW; i += 32) q.x += sums[ph][i + lane].x, q.y += sums[ph][i + lane].y;
     s = up ? q.y : q.x;
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
   const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = (rank * NV * TPR + l) * VEC - shift;
   const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, rank);
   if constexpr (CL > 1) {
-    static_assert(RPB == 1 && CL * NW % 32 == 0, "one row per cluster");
+    static_assert(RPB == 1 && (CL * NW < 32 || CL * NW % 32 == 0), "one row per cluster");
     cluster.init();
     cluster_sync_all();  // every block of the cluster is there, its mbarriers too
   }
@@ -850,6 +851,29 @@ int launch(void (*kernel)(Args), const Args& p, int threads, int smem, int cl, c
   return 1;
 }
 
+// Clusters of CL blocks that the device holds at once (less than its SMs suggest: a cluster's blocks share a GPC).
+template <typename Args>
+int cluster_places(void (*kernel)(Args), int threads, int smem, int cl, std::atomic<int> (&known)[16]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int n = dev < 16 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(cl);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cl;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+  if (dev < 16) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // 1: launched, 0: the row is too long for this shape, -1: an error
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
 int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
@@ -902,9 +926,15 @@ int forward(FwdArgs& p, cudaStream_t s) {
 template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL = 1>
 int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
   if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC * CL) return 0;
-  share_rows(p, BT / TPR, (int64_t)blocks * sms() / CL);
-  return launch(layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>, p, BT,
-                bwd_smem<T, VEC, NV, TPR, BT, STAGES, RAG>(), CL, s);
+  const auto kernel = layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>;
+  constexpr int smem = bwd_smem<T, VEC, NV, TPR, BT, STAGES, RAG>();
+  int64_t places = (int64_t)blocks * sms();
+  if constexpr (CL > 1) {
+    static std::atomic<int> known[16];
+    places = cluster_places(kernel, BT, smem, CL, known);
+  }
+  share_rows(p, BT / TPR, places);
+  return launch(kernel, p, BT, smem, CL, s);
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
@@ -928,8 +958,8 @@ int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
     if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, 2, s);
     if (!r) r = launch_bwd<T, VEC, NV, 256, 512, S, RAG>(p, 1, s);
     if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG>(p, 1, s);
-    if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 2>(p, 1, s);
-    if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG, 4>(p, 1, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 256, 256, S, RAG, 4>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 256, 256, S, RAG, 8>(p, 2, s);
     return r;
   }
 }

@@ -70,6 +70,8 @@ struct FwdArgs {
   int64_t rows, xs, ys, chunk;  // chunk: rows per block
   int cols, param_bf16, param_vec, groups, period, classes;
   float eps, inv_cols;
+  int* err;
+  int cl;  // blocks per row, where a cluster shares it
 };
 
 struct BwdArgs {
@@ -84,6 +86,7 @@ struct BwdArgs {
   int cols, param_bf16, param_vec, groups, period, classes;
   float inv_cols;
   int* err;
+  int cl;  // blocks per row, where a cluster shares it
 };
 
 // Sum over the TPR threads of a row.  Up to a warp: shuffles; of two sums, the halves of the row's lanes take one each
@@ -131,13 +134,15 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int slot, int
   }
 }
 
-// ... of the CL blocks of a cluster that share a row: every warp sends its two sums to every block, whose mbarrier counts
-// their bytes, and each thread adds up what arrived.  Buffers and mbarriers alternate from row to row: one is filled
-// again only after every warp has sent its sums of the row between, which it does after reading this one.  (A block's
-// barrier and then the cluster's took 0.9 us of a row's 2.0.)
-template <int CL, int NW>
+// ... and over the blocks (cl of them) of a cluster that share a row: every warp sends its sums to every block, whose mbarrier counts
+// their bytes, and each thread adds up what arrived.  Buffers and mbarriers alternate: one is filled again only after
+// every warp has sent its sums of the time between, which it does after reading this one.  (A block's barrier and then
+// the cluster's took 0.9 us of the 2.0 that a row of the gradients took.)
+constexpr int kMaxCluster = 8;
+
+template <int NW, int N>
 struct ClusterSums {
-  float2 sums[2][CL * NW];  // the pairs of [block][warp], each sent as two halves
+  float sums[2][kMaxCluster * NW * N];  // of [block][warp]
   uint64_t ready[2];
   int abort;
 
@@ -148,36 +153,45 @@ struct ClusterSums {
       abort = 0;
       fence_barrier_init();
     }
+    cluster_sync_all();  // every block of the cluster is there, its mbarriers too
   }
-  // n: the number of the row.  False, of whole warps, when the others' sums do not come.
-  __device__ __forceinline__ bool sum(float (&v)[2], int rank, uint32_t n, int* err) {
-    const uint32_t ph = n & 1;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const bool up = lane & 16;
-    if (threadIdx.x == 0) mbar_expect_tx(&ready[ph], CL * NW * 8);
-    float s = up ? v[1] : v[0];
-    s += __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+  // A warp's sums: of two, the lower half of the lanes gets the first, the upper half the second.
+  static __device__ __forceinline__ float warp_sum(float x, float y, bool up) {
+    float s = up ? y : x;
+    s += __shfl_xor_sync(0xffffffffu, N == 1 || up ? x : y, 16);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if ((lane & 15) < CL) {
-      const uint32_t dst = mapa_shared(smem_u32(&sums[ph][rank * NW + w]) + (up ? 4 : 0), lane & 15);
-      const uint32_t bar = mapa_shared(smem_u32(&ready[ph]), lane & 15);
+    return s;
+  }
+  // n: the number of the call.  False, of whole warps, when the others' sums do not come.
+  __device__ __forceinline__ bool sum(float (&v)[N], int rank, int cl, uint32_t n, int* err) {
+    const uint32_t ph = n & 1;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const bool up = N == 2 && (lane & 16);
+    if (threadIdx.x == 0) mbar_expect_tx(&ready[ph], cl * NW * N * 4);
+    float s = warp_sum(v[0], v[N - 1], up);
+    const int to = lane % (32 / N);
+    if (to < cl) {
+      const uint32_t dst = mapa_shared(smem_u32(&sums[ph][(rank * NW + w) * N + up]), to);
+      const uint32_t bar = mapa_shared(smem_u32(&ready[ph]), to);
       asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(dst),
                    "r"(__float_as_uint(s)), "r"(bar)
                    : "memory");
     }
     const bool ok = mbar_wait_cluster(&ready[ph], (n >> 1) & 1, &abort, err);
     if (!__all_sync(0xffffffffu, ok)) return false;
-    float2 q = CL * NW >= 32 || lane < CL * NW ? sums[ph][lane] : make_float2(0.f, 0.f);
+    float x = 0.f, y = 0.f;
 #pragma unroll
-    for (int i = 32; i < CL * NW; i += 32) q.x += sums[ph][i + lane].x, q.y += sums[ph][i + lane].y;
-    s = up ? q.y : q.x;
-    s += __shfl_xor_sync(0xffffffffu, up ? q.x : q.y, 16);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float other = __shfl_xor_sync(0xffffffffu, s, 16);
-    v[0] = up ? other : s;
-    v[1] = up ? s : other;
+    for (int i = lane; i < kMaxCluster * NW; i += 32)
+      if (i < cl * NW) x += sums[ph][i * N], y += sums[ph][i * N + N - 1];
+    s = warp_sum(x, y, up);
+    if constexpr (N == 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+      v[0] = up ? other : s;
+      v[1] = up ? s : other;
+    } else {
+      v[0] = s;
+    }
     return true;
   }
 };
@@ -451,16 +465,19 @@ __device__ __forceinline__ int row_shift(const void* p, int64_t stride, int cls)
 }
 
 // ---------------------------------------------------------------- forward
-// A block takes a run of rows; scale and shift stay in registers.
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+// A block takes a run of rows; scale and shift stay in registers.  CL blocks share longer rows.
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, bool CL>
 __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
-  __shared__ __align__(16) float red[RPB * 2 * NW];
+  __shared__ __align__(16) float red[CL ? 4 : RPB * 2 * NW];
+  __shared__ __align__(16) ClusterSums<NW, 1> cluster;
   extern __shared__ __align__(16) uint8_t dyn[];
-  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR;
-  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x);
-  const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = l * VEC - shift;
-  const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, 0);
+  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR, rank = CL ? (int)cluster_rank() : 0, cl = CL ? p.cl : 1;
+  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x / cl);
+  const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = (rank * NV * TPR + l) * VEC - shift;
+  const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, rank);
+  static_assert(!CL || RPB == 1, "one row per cluster");
+  if constexpr (CL) cluster.init();
   Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG> rows;
   rows.first_col = first_col;
   rows.cols = p.cols;
@@ -470,6 +487,7 @@ __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdAr
   load_params<VEC, NV, RAG>(p.gamma, p.param_bf16, p.param_vec, first_col, TPR * VEC, p.cols, 1.f, g);
   load_params<VEC, NV, RAG>(p.beta, p.param_bf16, p.param_vec, first_col, TPR * VEC, p.cols, 0.f, b);
   int phase = 0;
+  uint32_t sum_number = 0;
   for (int64_t j0 = run.first; j0 < run.last; j0 += RPB) {
     if (TPR >= 32 && j0 + slot >= run.last) break;  // whole warps (and whole barrier groups) leave together
     uint64_t v[1][N2];
@@ -478,7 +496,8 @@ __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdAr
 #pragma unroll
     for (int e = 0; e < N2; ++e) a = f2_add(a, v[0][e]);
     float s[1] = {f2_total(a)};
-    row_sum<TPR, 1>(s, red, slot, phase);
+    if constexpr (!CL) row_sum<TPR, 1>(s, red, slot, phase);
+    else if (!cluster.sum(s, rank, cl, sum_number++, p.err)) break;
     const float mean = s[0] * p.inv_cols;
     const uint64_t m2 = f2_pack(mean, mean);
     a = f2_pack(0.f, 0.f);
@@ -512,11 +531,12 @@ __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdAr
       }
     }
     s[0] = f2_total(a);
-    row_sum<TPR, 1>(s, red, slot, phase);
+    if constexpr (!CL) row_sum<TPR, 1>(s, red, slot, phase);
+    else if (!cluster.sum(s, rank, cl, sum_number++, p.err)) break;
     const float rstd = 1.0f / sqrtf(s[0] * p.inv_cols + p.eps);
     if (j0 + slot < run.last) {
       const int64_t row = run.row(j0 + slot);
-      if (l == 0) {
+      if (l == 0 && rank == 0) {
         if (p.mean) p.mean[row] = mean;
         if (p.rstd) p.rstd[row] = rstd;
       }
@@ -527,6 +547,7 @@ __global__ void __launch_bounds__(BT, 512 / BT) layernorm_fwd_kernel(const FwdAr
     }
   }
   rows.drain();
+  if constexpr (CL) cluster_sync_all();  // no sums on their way to a block that is gone
 }
 
 // Rows too long for registers: one block per row, re-read in each of three passes.
@@ -588,21 +609,18 @@ constexpr int bwd_smem() {
 // A block takes a run of rows and keeps, per thread, the sums of dy z and dy over its
 // rows for the columns that the thread owns; the row slots of the block are added in
 // shared memory at the end, one partial row per block.  CL blocks share longer rows.
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL>
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, bool CL>
 __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernorm_bwd_kernel(const BwdArgs p) {
   constexpr int RPB = BT / TPR, NW = TPR > 32 ? TPR / 32 : 1, N2 = NV * VEC / 2;
-  __shared__ __align__(16) float red[CL == 1 ? RPB * 2 * NW * 2 : 4];
-  __shared__ __align__(16) ClusterSums<CL, NW> cluster;
+  __shared__ __align__(16) float red[CL ? 4 : RPB * 2 * NW * 2];
+  __shared__ __align__(16) ClusterSums<NW, 2> cluster;
   extern __shared__ __align__(16) uint8_t dyn[];
-  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR, rank = CL > 1 ? (int)cluster_rank() : 0;
-  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x / CL);
+  const int slot = threadIdx.x / TPR, l = threadIdx.x % TPR, rank = CL ? (int)cluster_rank() : 0, cl = CL ? p.cl : 1;
+  const Run run(p.rows, p.period, p.classes, p.chunk, blockIdx.x / cl);
   const int shift = row_shift<T, RAG>(p.x, p.xs, run.cls), first_col = (rank * NV * TPR + l) * VEC - shift;
   const Edges<VEC> edges = find_edges<T, VEC, NV, TPR>(shift, p.cols, l, rank);
-  if constexpr (CL > 1) {
-    static_assert(RPB == 1 && (CL * NW < 32 || CL * NW % 32 == 0), "one row per cluster");
-    cluster.init();
-    cluster_sync_all();  // every block of the cluster is there, its mbarriers too
-  }
+  static_assert(!CL || RPB == 1, "one row per cluster");
+  if constexpr (CL) cluster.init();
   Rows<T, VEC, NV, TPR, BT, STAGES, 2, RAG> rows;
   rows.first_col = first_col;
   rows.cols = p.cols;
@@ -649,8 +667,8 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
       s1 = f2_fma(dz[e], z[e], s1);
     }
     float s[2] = {f2_total(s0), f2_total(s1)};
-    if constexpr (CL == 1) row_sum<TPR, 2>(s, red, slot, phase);
-    else if (!cluster.sum(s, rank, row_number++, p.err)) break;
+    if constexpr (!CL) row_sum<TPR, 2>(s, red, slot, phase);
+    else if (!cluster.sum(s, rank, cl, row_number++, p.err)) break;
     const float k0 = -s[0] * p.inv_cols * rstd, k1 = -s[1] * p.inv_cols * rstd;
     const uint64_t k02 = f2_pack(k0, k0), k12 = f2_pack(k1, k1);
 #pragma unroll
@@ -660,10 +678,10 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
                                    edges);
   }
   rows.drain();
-  if constexpr (CL > 1) cluster_sync_all();  // no sums on their way to a block that is gone
+  if constexpr (CL) cluster_sync_all();  // no sums on their way to a block that is gone
   if (!p.partial) return;
   const int64_t half = (int64_t)p.groups * p.cols;
-  float* out = p.partial + (int64_t)(blockIdx.x / CL) * p.cols;
+  float* out = p.partial + (int64_t)(blockIdx.x / cl) * p.cols;
   // Through shared memory, so that a warp writes whole lines (a thread's own columns, stored from its registers, cost
   // 8 us per call at 16384 columns); a thread's vectors lie there as they do in the row.
   constexpr int WIDTH = TPR * NV * VEC;
@@ -851,12 +869,12 @@ int launch(void (*kernel)(Args), const Args& p, int threads, int smem, int cl, c
   return 1;
 }
 
-// Clusters of CL blocks that the device holds at once (less than its SMs suggest: a cluster's blocks share a GPC).
+// Clusters of cl blocks that the device holds at once (less than its SMs suggest: a cluster's blocks share a GPC).
 template <typename Args>
-int cluster_places(void (*kernel)(Args), int threads, int smem, int cl, std::atomic<int> (&known)[16]) {
+int cluster_places(void (*kernel)(Args), int threads, int smem, int cl, std::atomic<int> (&known)[16][kMaxCluster + 1]) {
   int dev = 0;
   cudaGetDevice(&dev);
-  int n = dev < 16 ? known[dev].load(std::memory_order_relaxed) : 0;
+  int n = dev < 16 ? known[dev][cl].load(std::memory_order_relaxed) : 0;
   if (n > 0) return n;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   cudaLaunchConfig_t cfg{};
@@ -870,17 +888,25 @@ int cluster_places(void (*kernel)(Args), int threads, int smem, int cl, std::ato
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
-  if (dev < 16) known[dev].store(n, std::memory_order_relaxed);
+  if (dev < 16) known[dev][cl].store(n, std::memory_order_relaxed);
   return n;
 }
 
 // 1: launched, 0: the row is too long for this shape, -1: an error
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG>
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, bool CL = false>
 int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
-  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC) return 0;
-  share_rows(p, BT / TPR, (int64_t)blocks * sms());
-  return launch(layernorm_fwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG>, p, BT,
-                Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG>::kBytes, 1, s);
+  const int need = p.cols + (RAG ? VEC - 1 : 0);
+  p.cl = (need + TPR * NV * VEC - 1) / (TPR * NV * VEC);
+  if (p.cl > (CL ? kMaxCluster : 1)) return 0;
+  const auto kernel = layernorm_fwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>;
+  constexpr int smem = Rows<T, VEC, NV, TPR, BT, STAGES, 1, RAG>::kBytes;
+  int64_t places = (int64_t)blocks * sms();
+  if constexpr (CL) {
+    static std::atomic<int> known[16][kMaxCluster + 1];
+    places = cluster_places(kernel, BT, smem, p.cl, known);
+  }
+  share_rows(p, BT / TPR, places);
+  return launch(kernel, p, BT, smem, p.cl, s);
 }
 
 // 32 elements per thread in the forward (16 of f32), 256 threads per block and 4 blocks per SM; measured over 32 MiB
@@ -902,6 +928,7 @@ int dispatch_fwd(FwdArgs& p, cudaStream_t s) {
     if (!r) r = launch_fwd<T, VEC, NV, 128, 256, 3, RAG>(p, 4, s);
     if (!r) r = launch_fwd<T, VEC, NV, 256, 256, 3, RAG>(p, 4, s);
     if (!r) r = launch_fwd<T, VEC, NV, 512, 512, 2, RAG>(p, 2, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 256, 256, 3, RAG, true>(p, 4, s);
     return r;
   }
 }
@@ -923,18 +950,20 @@ int forward(FwdArgs& p, cudaStream_t s) {
   return cuda_status(cudaGetLastError(), "layernorm forward launch");
 }
 
-template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, int CL = 1>
+template <typename T, int VEC, int NV, int TPR, int BT, int STAGES, bool RAG, bool CL = false>
 int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
-  if (p.cols + (RAG ? VEC - 1 : 0) > TPR * NV * VEC * CL) return 0;
+  const int need = p.cols + (RAG ? VEC - 1 : 0);
+  p.cl = (need + TPR * NV * VEC - 1) / (TPR * NV * VEC);
+  if (p.cl > (CL ? kMaxCluster : 1)) return 0;
   const auto kernel = layernorm_bwd_kernel<T, VEC, NV, TPR, BT, STAGES, RAG, CL>;
   constexpr int smem = bwd_smem<T, VEC, NV, TPR, BT, STAGES, RAG>();
   int64_t places = (int64_t)blocks * sms();
-  if constexpr (CL > 1) {
-    static std::atomic<int> known[16];
-    places = cluster_places(kernel, BT, smem, CL, known);
+  if constexpr (CL) {
+    static std::atomic<int> known[16][kMaxCluster + 1];
+    places = cluster_places(kernel, BT, smem, p.cl, known);
   }
   share_rows(p, BT / TPR, places);
-  return launch(kernel, p, BT, smem, CL, s);
+  return launch(kernel, p, BT, smem, p.cl, s);
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
@@ -958,8 +987,7 @@ int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
     if (!r) r = launch_bwd<T, VEC, NV, 128, 256, 3, RAG>(p, 2, s);
     if (!r) r = launch_bwd<T, VEC, NV, 256, 512, S, RAG>(p, 1, s);
     if (!r) r = launch_bwd<T, VEC, NV, 512, 512, S, RAG>(p, 1, s);
-    if (!r) r = launch_bwd<T, VEC, NV, 256, 256, S, RAG, 4>(p, 2, s);
-    if (!r) r = launch_bwd<T, VEC, NV, 256, 256, S, RAG, 8>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 256, 256, S, RAG, true>(p, 2, s);
     return r;
   }
 }
@@ -1005,7 +1033,8 @@ extern "C" int pdb_layernorm_fwd(const pdb_layernorm_fwd_desc* d, void* stream) 
   if (!typed(d->x, d->dtype) || !typed(d->y, d->dtype) || !typed(d->gamma, d->param_dtype) || !typed(d->beta, d->param_dtype))
     return set_error(PDB_ERR_ALIGN, "layernorm: a tensor is not aligned to its type");
   FwdArgs p{d->x, d->gamma, d->beta, d->y, d->mean, d->rstd, d->rows, d->x_row_stride, d->y_row_stride,
-                  0, (int)d->cols, d->param_dtype == PDB_BF16, param_vec(d->gamma, d->beta), 0, 1, 1, (float)d->eps, (float)(1.0 / (double)d->cols)};
+                  0, (int)d->cols, d->param_dtype == PDB_BF16, param_vec(d->gamma, d->beta), 0, 1, 1, (float)d->eps,
+                  (float)(1.0 / (double)d->cols), device_error_flag()};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return d->dtype == PDB_F32 ? forward<float>(p, s) : forward<__nv_bfloat16>(p, s);
 }

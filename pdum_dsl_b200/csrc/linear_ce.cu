@@ -149,10 +149,13 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
     tc_commit(bar);
 }
 
-template <int CG>
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
-  if constexpr (CG == 2) return mbar_wait_cluster(bar, parity, abort, err);
-  else return mbar_wait(bar, parity, abort, err);
+// A warp's accumulator columns are read (tmem_wait_ld has returned): one arrival at rank 0's barrier.  Relaxed, since
+// nothing but tensor memory is handed over: a release at cluster scope waits for all of the warp's memory traffic.
+__device__ __forceinline__ void warp_arrive_rank0(uint64_t* bar) {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0)
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0)) : "memory");
 }
 
 template <int CG, bool A_MN, bool B_MN, int EPI>
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int ma = m0 + (int)rank * 128, nb = n0 + (int)rank * b_rows;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
         const int st = g % STAGES;
-        if (!(ok = wait_bar<CG>(&bar->empty[st], ((g / STAGES) & 1) ^ 1, abort, p.err))) break;
+        if (!(ok = mbar_wait(&bar->empty[st], ((g / STAGES) & 1) ^ 1, abort, p.err))) break;
         if (rank == 0) mbar_expect_tx(&bar->full[st], bytes);
         const uint32_t full0 = CG == 2 ? mapa_shared(smem_u32(&bar->full[st]), 0) : 0;
         auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
@@ -274,12 +277,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int split = (int)((uint32_t)t / (uint32_t)(tm * tn));
       const int kb0 = split * kb_split, kb1 = min(nk, kb0 + kb_split);
       const int buf = tt & 1;
-      if (!(ok = wait_bar<CG>(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
+      if (!(ok = mbar_wait(&bar->acc_empty[buf], ((tt >> 1) & 1) ^ 1, abort, p.err))) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256;
       uint32_t more = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = wait_bar<CG>(&bar->full[st], parity, abort, p.err))) break;
+        if (!(ok = mbar_wait(&bar->full[st], parity, abort, p.err))) break;
         tc_fence_after();
         const uint64_t da = da0 + st * (kTileA >> 4), db = db0 + st * (L::kTileB >> 4);
 #pragma unroll
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       float up = next_dloss / unit;
       if (next_target < 0 || next_target >= p.vocab) up = NAN;  // no such entry: the gradient says so
       look(t + units);
-      if (!wait_bar<CG>(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
+      if (!mbar_wait(&bar->acc_full[buf], (tt >> 1) & 1, abort, p.err)) break;
       tc_fence_after();
       float base = -INFINITY, sum = 0.f;
 #pragma unroll 1
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
-      if constexpr (CG == 2) warp_arrive_cluster_after_tc(mapa_shared(smem_u32(&bar->acc_empty[buf]), 0));
+      if constexpr (CG == 2) warp_arrive_rank0(&bar->acc_empty[buf]);
       else warp_arrive_after_tc(&bar->acc_empty[buf]);
       if constexpr (EPI == kStats) {
         // the four warps with these rows join their columns: three leave theirs in shared memory for the first

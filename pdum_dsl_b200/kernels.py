@@ -183,11 +183,12 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
 
 
 def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dim() == 2:
+    n = t.dim()
+    if n == 2:
         t = t[None, None]
-    elif t.dim() == 3:
+    elif n == 3:
         t = t[None]
-    elif t.dim() != 4:
+    elif n != 4:
         raise ValueError(f"{name}: expected (T, D), (H, T, D) or (B, H, T, D), got {tuple(t.shape)}")
     if t.stride(-1) != 1:
         t = t.contiguous()
@@ -303,28 +304,32 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
     may be the inputs themselves, and shares no memory otherwise.  Returns the turned q, or (q, k)."""
     ts = (q,) if k is None else (q, k)
     _need_cuda(*ts)
-    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+    dt = q.dtype
+    if dt not in _DTYPES or (k is not None and k.dtype != dt):
         raise TypeError("rotary: q and k must both be float32 or bfloat16")
-    xs = [_as4d(t, n) for t, n in zip(ts, ("q", "k"))]
-    B, _, T, D = xs[0].shape
-    if k is not None and (xs[1].shape[0] != B or xs[1].shape[2:] != (T, D) or k.device != q.device):
+    x0 = _as4d(q, "q")
+    x1 = x0 if k is None else _as4d(k, "k")
+    B, H, T, D = x0.shape
+    Bk, Hk, Tk, Dk = x1.shape
+    if k is not None and (Bk != B or Tk != T or Dk != D or k.device != q.device):
         raise ValueError(f"rotary: incompatible q {tuple(q.shape)} and k {tuple(k.shape)}")
     freq = np.ascontiguousarray(inv_freq, dtype=np.float64)
     n = len(freq) if freq.ndim == 1 else -1
     if n < 0 or n > _lib.ROTARY_MAX_PAIRS or 2 * n > D:
         raise ValueError(f"rotary: inv_freq must be a vector of at most {_lib.ROTARY_MAX_PAIRS} pairs within the head's {D} features")
     if out is None:
-        ys = [torch.empty_like(t) for t in xs]
+        y0 = torch.empty_like(x0)
+        y1 = y0 if k is None else torch.empty_like(x1)
     else:
         outs = (out,) if k is None else tuple(out)
         if len(outs) != len(ts):
             raise ValueError("rotary: out must be one tensor for each input")
         for o, t in zip(outs, ts):
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+            if o.shape != t.shape or o.dtype != dt or o.device != t.device:
                 raise ValueError("rotary: out must have the inputs' shape, dtype and device")
-            if (o.shape[-1] > 1 and o.stride(-1) != 1) or any(m > 1 and st == 0 for m, st in zip(o.shape, o.stride())):
+            if (o.stride(-1) != 1 and not o.is_contiguous()) or any(m > 1 and st == 0 for m, st in zip(o.shape, o.stride())):
                 raise ValueError("rotary: out must have unit stride along the features and no broadcast dim")
-        ys = [_as4d(o, "out") for o in outs]
+        y0, y1 = _as4d(outs[0], "out"), _as4d(outs[-1], "out")
     at_p, ps = 0, (0, 0)
     if positions is not None:
         if positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
@@ -336,20 +341,19 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
             p = p.expand(B, T)
         at_p, ps = p.data_ptr(), p.stride()
     # one packed record: a third of the time of setting the descriptor's fields one by one
-    x0, y0, x1, y1 = xs[0], ys[0], xs[-1], ys[-1]
     d = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(
-        x0.data_ptr(), x1.data_ptr(), y0.data_ptr(), y1.data_ptr(), x0.shape[1], 0 if k is None else x1.shape[1],
+        x0.data_ptr(), x1.data_ptr(), y0.data_ptr(), y1.data_ptr(), H, 0 if k is None else Hk,
         *x0.stride()[:3], *x1.stride()[:3], *y0.stride()[:3], *y1.stride()[:3], at_p, *ps, start, B, T, D, 2 * n,
-        amplitude, freq.tobytes(), bool(interleaved), bool(inverse), _DTYPES[q.dtype], 0))
+        amplitude, freq.tobytes(), bool(interleaved), bool(inverse), _DTYPES[dt], 0))
     with _on_device_of(q):
         check(load().pdb_rotary(C.byref(d), _raw_stream(q)), "pdb_rotary")
     if out is not None:
-        rets = outs
-    elif q.dim() == 4 == ts[-1].dim():
-        rets = tuple(ys)
-    else:
-        rets = tuple(y.view(t.shape) for y, t in zip(ys, ts))
-    return rets[0] if k is None else rets
+        return outs[0] if k is None else outs
+    if x0 is not q:
+        y0 = y0.view(q.shape)
+    if k is None:
+        return y0
+    return y0, y1 if x1 is k else y1.view(k.shape)
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,

@@ -94,7 +94,7 @@ struct BwdArgs {
 // barrier of the row's own threads is enough (a buffer is written again only after the barrier of the row between).
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int slot, int& phase) {
-  static_assert(N <= 2 && TPR >= 8, "one or two sums");
+  static_assert(N <= 2 && TPR >= 4, "one or two sums");
   constexpr int W = TPR < 32 ? TPR : 32, NW = TPR / 32;
   const bool up = N == 2 && (threadIdx.x & (W / 2));
   float s = up ? v[N - 1] : v[0];
@@ -921,7 +921,8 @@ int dispatch_fwd(FwdArgs& p, cudaStream_t s) {
     return r;
   } else {
     constexpr int NV = (sizeof(T) == 2 ? 32 : 16) / VEC;
-    int r = launch_fwd<T, VEC, NV, 8, 256, 3, RAG>(p, 4, s);
+    int r = launch_fwd<T, VEC, NV, 4, 256, 3, RAG>(p, 4, s);
+    if (!r) r = launch_fwd<T, VEC, NV, 8, 256, 3, RAG>(p, 4, s);
     if (!r) r = launch_fwd<T, VEC, NV, 16, 256, 3, RAG>(p, 4, s);
     if (!r) r = launch_fwd<T, VEC, NV, 32, 256, 3, RAG>(p, 4, s);
     if (!r) r = launch_fwd<T, VEC, NV, 64, 256, 3, RAG>(p, 4, s);
@@ -980,7 +981,8 @@ int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
     return r;
   } else {
     constexpr int NV = 16 / VEC;
-    int r = launch_bwd<T, VEC, NV, 8, 256, 3, RAG>(p, 2, s);
+    int r = launch_bwd<T, VEC, NV, 4, 256, 3, RAG>(p, 2, s);
+    if (!r) r = launch_bwd<T, VEC, NV, 8, 256, 3, RAG>(p, 2, s);
     if (!r) r = launch_bwd<T, VEC, NV, 16, 256, 3, RAG>(p, 2, s);
     if (!r) r = launch_bwd<T, VEC, NV, 32, 256, 3, RAG>(p, 2, s);
     if (!r) r = launch_bwd<T, VEC, NV, 64, 256, 3, RAG>(p, 2, s);

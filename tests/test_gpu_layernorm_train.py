@@ -95,7 +95,8 @@ def _check_backward(x, dy, mean, rstd, gam, dx, dg, db):
 
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (1, 4096), (300, 64), (1000, 128), (37, 1001), (257, 520), (301, 2048), (70, 4096),
-          (9, 5000), (50, 9344), (33, 12001), (150, 20000), (7, 30001), (64, 1002), (200, 515), (20, 4099), (90, 16), (13, 8191), (700, 8192), (5, 8200), (3, 16384), (4, 32768), (2, 40003)]
+          (9, 5000), (50, 9344), (33, 12001), (150, 20000), (7, 30001), (64, 1002), (200, 515), (20, 4099), (90, 16), (13, 8191), (700, 8192), (5, 8200), (3, 16384), (4, 32768), (2, 40003), (5000, 32),
+          (3001, 57), (2000, 100)]
 
 
 @pytest.mark.parametrize("R,C", SHAPES)

@@ -24,8 +24,8 @@
 // the contracted index): G^T, x and w enter dw and dx that way, as they lie in memory.
 // Sixteen warps run the epilogue, 64 columns of 32 rows each, and hand results to TMA
 // stores through shared memory.  On a B200, 4096 tokens x 65536 x 2048: the loss in 676
-// us cool (1.63 PFLOP/s), 820 warm under the power limit; 8192 x 128000 x 4096 gradients
-// with a tenth ignored in 16.7 to 18.4 ms (1.40 to 1.54 of all tokens' operations).
+// us cool (1.63 PFLOP/s), 810 warm under the power limit; 8192 x 128000 x 4096 gradients
+// with a tenth ignored in 16.4 to 18.4 ms (1.40 to 1.57 of all tokens' operations).
 //
 // f32 operands take the same steps on IEEE multiply-adds (the f32 column refuses
 // reduced operand types): linear_ce_f32_kernel, G in f32.

@@ -888,7 +888,10 @@ int cluster_places(void (*kernel)(Args), int threads, int smem, int cl, std::ato
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();  // the launch itself says what is wrong
+    return 1;
+  }
   if (dev < 16) known[dev][cl].store(n, std::memory_order_relaxed);
   return n;
 }

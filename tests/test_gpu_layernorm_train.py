@@ -303,3 +303,35 @@ def test_rows_that_lie_beyond_32_bits(cuda, C):
         _check_backward(xs, dy, mean, rstd, gam, dx, dg, db)
         out = kernels.layernorm(x, gam, bet, out=xs)
         assert torch.equal(out, kernels.layernorm(x, gam, bet)) and torch.equal(xs, out)
+
+
+@pytest.mark.parametrize("C", [12000, 20000, 28001])
+def test_long_rows_captured_first_and_called_twice_at_once(cuda, C):
+    """Rows on clusters (3, 5 and 7 blocks of the gradients): captured before any other call of their width, replayed on
+    new inputs, and two calls at once on two streams; all the same bits."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, dy, gam, bet = _inputs(cuda, 300, C, torch.bfloat16, torch.float32, C)
+    sx, sdy = torch.zeros_like(x), torch.zeros_like(dy)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = kernels.layernorm(sx, gam, bet, return_stats=True)
+        captured += kernels.layernorm_backward(sdy, sx, captured[1], captured[2], gam)
+    sx.copy_(x), sdy.copy_(dy)
+    graph.replay()
+    streams, results = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            y, mean, rstd = kernels.layernorm(x, gam, bet, return_stats=True)
+            results.append((y, mean, rstd) + kernels.layernorm_backward(dy, x, mean, rstd, gam))
+    torch.cuda.synchronize()
+    kernels.check_device_errors()
+    for r in results:
+        assert all(torch.equal(a, b) for a, b in zip(captured, r))
+    y, mean, rstd, dx, dg, db = results[0]
+    _check_forward(x, gam, bet, 1e-5, y, mean, rstd)
+    _check_backward(x, dy, mean, rstd, gam, dx, dg, db)

@@ -150,36 +150,39 @@ def layernorm_backward(dout: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, 
     dgamma / dbeta are vectors of gamma's dtype (float32 without gamma), summed in
     float32 in a fixed order; None without ``weight_grads``."""
     _need_cuda(dout, x, mean, rstd)
-    if x.dtype not in _DTYPES or dout.dtype != x.dtype:
+    dt = x.dtype
+    if dt not in _DTYPES or dout.dtype != dt:
         raise TypeError("layernorm_backward: dout and x must both be float32 or bfloat16")
     if dout.shape != x.shape:
         raise ValueError(f"layernorm_backward: dout {tuple(dout.shape)} does not match x {tuple(x.shape)}")
     x2, R, C_, xs = _rows(x)
     do2, _, _, dos = _rows(dout)
-    for nm, t in (("mean", mean), ("rstd", rstd)):
-        if t.dtype != torch.float32 or t.numel() != R or t.device != x.device:
-            raise ValueError(f"layernorm_backward: {nm} must be the forward's float32 statistic of {R} rows")
-    if dout.device != x.device:
+    dev, f32 = x.device, torch.float32
+    for t in (mean, rstd):
+        if t.dtype != f32 or t.numel() != R or t.device != dev:
+            raise ValueError(f"layernorm_backward: mean and rstd must be the forward's float32 statistics of {R} rows")
+    if dout.device != dev:
         raise ValueError("layernorm_backward: tensors on different devices")
     ptype = _param_dtype("layernorm_backward", x, C_, gamma, None)
     g = gamma.contiguous() if gamma is not None else None
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dx = torch.empty_like(x2)
-    dgamma = dbeta = None
+    dgamma = dbeta = at_g = at_b = None
+    if weight_grads:
+        dgamma = x.new_empty(C_, dtype=ptype)
+        dbeta = torch.empty_like(dgamma)
+        at_g, at_b = dgamma.data_ptr(), dbeta.data_ptr()
     d = _lib.LayerNormBwdDesc(do2.data_ptr(), x2.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                              g.data_ptr() if g is not None else None, dx.data_ptr(), None, None, None, 0, R, C_,
-                              dos, xs, C_, _DTYPES[x.dtype], _DTYPES[ptype])
+                              g.data_ptr() if g is not None else None, dx.data_ptr(), at_g, at_b, None, 0, R, C_,
+                              dos, xs, C_, _DTYPES[dt], _DTYPES[ptype])
     lib = load()
     with _on_device_of(x):
         if weight_grads:
-            dgamma = x.new_empty(C_, dtype=ptype)
-            dbeta = torch.empty_like(dgamma)
-            d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
             nbytes = lib.pdb_layernorm_bwd_workspace_size(C.byref(d))
             ws = x.new_empty(nbytes + 16, dtype=torch.uint8)
             d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
         check(lib.pdb_layernorm_bwd(C.byref(d), _raw_stream(x)), "pdb_layernorm_bwd")
-    return dx if dx.shape == x.shape else dx.view(x.shape), dgamma, dbeta
+    return dx if x2 is x else dx.view(x.shape), dgamma, dbeta
 
 
 def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:

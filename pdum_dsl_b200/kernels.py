@@ -198,6 +198,13 @@ def _as4d(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
+def _result_like(t: torch.Tensor) -> torch.Tensor:
+    """A tensor for t's result, its features together.  empty_like keeps t's order of dims, and where two of them have
+    stride 1 (overlapping windows) it may put the features further apart."""
+    y = torch.empty_like(t)
+    return y if y.stride(-1) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _s3(t: torch.Tensor):
     return _lib.I64x3(t.stride(0), t.stride(1), t.stride(2))
 
@@ -321,8 +328,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, inv_freq, position
     if n < 0 or n > _lib.ROTARY_MAX_PAIRS or 2 * n > D:
         raise ValueError(f"rotary: inv_freq must be a vector of at most {_lib.ROTARY_MAX_PAIRS} pairs within the head's {D} features")
     if out is None:
-        y0 = torch.empty_like(x0)
-        y1 = y0 if k is None else torch.empty_like(x1)
+        y0 = _result_like(x0)
+        y1 = y0 if k is None else _result_like(x1)
     else:
         outs = (out,) if k is None else tuple(out)
         if len(outs) != len(ts):

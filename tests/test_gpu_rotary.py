@@ -202,3 +202,30 @@ def test_heads_that_lie_beyond_32_bits(cuda, interleaved):
         _check(got, x, f, pos, interleaved)
         kernels.rotary(xs, inv_freq=f, interleaved=interleaved, out=xs)
         assert torch.equal(xs, got)
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_views_with_a_second_unit_stride(cuda, interleaved, t):
+    """Windows that slide by one element along heads, rows or both, alone and as either of two tensors; the results
+    are laid out with their features together whatever the input's strides."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    f, m = kernels.rotary_frequencies(8, scaling="by_parts", factor=4.0, context=64)
+    flat = _draw(cuda, (400,), t, 11)
+    pos = torch.tensor([[3, 70, 4000], [9, 11, 100]], device=cuda)
+    plain = _draw(cuda, (2, 4, 3, 8), t, 12)
+    for strides in ((100, 1, 20, 1), (100, 20, 1, 1), (50, 1, 1, 1), (1, 1, 1, 1)):
+        x = flat.as_strided((2, 4, 3, 8), strides)
+        kw = dict(inv_freq=f, positions=pos, interleaved=interleaved, amplitude=m)
+        got = kernels.rotary(x, **kw)
+        _check(got, x.contiguous(), f, pos, interleaved, m)
+        a, b = kernels.rotary(x, plain, **kw)
+        c, d = kernels.rotary(plain, x, **kw)
+        assert torch.equal(a, got) and torch.equal(d, got) and torch.equal(b, c)
+        _check(b, plain, f, pos, interleaved, m)
+    three = flat.as_strided((4, 3, 8), (1, 20, 1))
+    _check(kernels.rotary(three, inv_freq=f, interleaved=interleaved)[None], three.contiguous()[None], f,
+           torch.arange(3, device=cuda)[None], interleaved)

@@ -201,7 +201,11 @@ class _Runner:
         if isinstance(spec, ScoreProgramSpec):
             return run_score_program(spec, tensors)
         if isinstance(spec, RowSpec):
+            import torch
+
             x = tensors[spec.x]
+            if x.dtype != torch.float32:  # the region's column is f32, whatever else the kernels' entry points take
+                raise TypeError(f"row-reduction runners take float32 tensors, got {x.dtype}")
             perm = [spec.x_dims.index(n) for n in spec.x_dims if n != spec.dim] + [spec.x_dims.index(spec.dim)]
             xv = x.permute(*perm)
             lead = xv.shape[:-1]

@@ -249,3 +249,21 @@ def test_frequency_refusals():
     f, m = kernels.rotary_frequencies(0)
     assert len(f) == 0 and m == 1.0
     assert np.array_equal(kernels.rotary_frequencies(2)[0], [1.0])
+
+
+def test_row_reduction_runners_are_f32():
+    """A row-reduction region has an f32 kernel only: its runner refuses device tensors of another type."""
+    import torch
+
+    from pdum_dsl_b200.recognize import RowSpec
+    from pdum_dsl_b200.tile import _Runner
+
+    for kind in ("softmax", "layernorm"):
+        run = object.__new__(_Runner)
+        run.dtype = "f32"
+        run.spec = RowSpec(kind, 0, None, None, 1e-5, "c", ("r", "c"), ("r", "c"))
+        for t in (torch.bfloat16, torch.float64):
+            with pytest.raises(TypeError, match="float32"):
+                run.run_t(torch.zeros(2, 8, dtype=t))
+        with pytest.raises(ValueError, match="CUDA"):
+            run.run_t(torch.zeros(2, 8))

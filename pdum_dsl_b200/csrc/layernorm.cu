@@ -655,12 +655,12 @@ __global__ void __launch_bounds__(BT, (NV * VEC < 16 ? 768 : 512) / BT) layernor
     uint64_t v[2][N2];
     rows.take(v, edges);
     auto &z = v[0], &dz = v[1];
-    // z as one fused step: the rounding of mean * rstd is of the size of mean's own
-    const uint64_t r2 = f2_pack(rstd, rstd), mr2 = f2_pack(-mean * rstd, -mean * rstd);
+    // the difference first, as in the forward: as x rstd - mean rstd, z would be off by up to 2^-24 |mean| rstd
+    const uint64_t r2 = f2_pack(rstd, rstd), m2 = f2_pack(mean, mean);
     uint64_t s0 = zero2, s1 = zero2;
 #pragma unroll
     for (int e = 0; e < N2; ++e) {
-      z[e] = f2_fma(z[e], r2, mr2);
+      z[e] = f2_mul(f2_sub(z[e], m2), r2);
       ab[e] = f2_add(ab[e], dz[e]);
       ag[e] = f2_fma(dz[e], z[e], ag[e]);
       dz[e] = f2_mul(dz[e], g[e]);

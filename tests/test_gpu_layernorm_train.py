@@ -335,3 +335,70 @@ def test_long_rows_captured_first_and_called_twice_at_once(cuda, C):
     y, mean, rstd, dx, dg, db = results[0]
     _check_forward(x, gam, bet, 1e-5, y, mean, rstd)
     _check_backward(x, dy, mean, rstd, gam, dx, dg, db)
+
+
+def _check_backward_given(x, dy, mean, rstd, gam, dx, dg, db):
+    """As _check_backward, with the statistics taken as given: the difference from the mean is rounded once, to u of
+    itself, and so is its product with rstd, so z is off by at most (1 + u)^2 - 1 <= 3 u of itself, however far the row
+    lies from 0."""
+    import torch
+
+    R, C = x.shape
+    K = (82 + C / 512) * U
+    xd, dyd, m, r = x.double(), dy.double(), mean.double()[:, None], rstd.double()[:, None]
+    gd = gam.double() if gam is not None else torch.ones(C, dtype=torch.float64, device=x.device)
+    z = (xd - m) * r
+    dz = dyd * gd
+    m0, m1 = dz.mean(1, keepdim=True), (dz * z).mean(1, keepdim=True)
+    zerr = 3 * U * z.abs()
+    e0 = K * dz.abs().mean(1, keepdim=True)
+    e1 = (K + 3 * U) * (dz * z).abs().mean(1, keepdim=True)
+    slack = r * (e0 + z.abs() * e1 + zerr * m1.abs() + 6 * U * (dz.abs() + m0.abs() + (z * m1).abs()))
+    _within(dx, r * (dz - m0 - z * m1), dx.dtype, slack, "dx")
+    n = (R + 64) * U
+    _within(dg, (dyd * z).sum(0), dg.dtype, (n + 3 * U) * (dyd * z).abs().sum(0), "dgamma")
+    _within(db, dyd.sum(0), db.dtype, n * dyd.abs().sum(0), "dbeta")
+
+
+# (cols, elements by which x and dout lie behind a 16-byte boundary): in registers on 4 to 512 threads, ragged, element
+# by element, on clusters (ragged too), and read again
+OFFSET_ROWS = [(64, 0, 0), (96, 0, 0), (768, 0, 0), (4096, 0, 0), (8192, 0, 0), (57, 0, 0), (1001, 0, 0), (5003, 0, 0),
+               (100, 1, 2), (1001, 1, 4), (6000, 3, 0), (12000, 0, 0), (20000, 0, 0), (28001, 0, 0), (50000, 0, 0)]
+
+
+def _offset_inputs(dev, C, at, t, seed, offset, spread):
+    import torch
+
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    wide = torch.empty(13, C + 8, device=dev, dtype=t), torch.empty(13, C + 8, device=dev, dtype=t)
+    x, dy = wide[0][:, at[0]:at[0] + C], wide[1][:, at[1]:at[1] + C]
+    where = offset * (1 + torch.rand(13, 1, generator=g)) * torch.tensor([1.0, -1.0]).repeat(7)[:13, None]
+    x.copy_(where + spread * torch.randn(13, C, generator=g))
+    dy.copy_(torch.randn(13, C, generator=g))
+    return x, dy, (1 + 0.1 * torch.randn(C, generator=g)).to(dev)
+
+
+@pytest.mark.parametrize("C,at_x,at_dy", OFFSET_ROWS)
+@pytest.mark.parametrize("t,offset", [("f32", 1e2), ("f32", 1e4), ("bf16", 1e2)])
+def test_gradients_of_rows_far_from_zero(cuda, C, at_x, at_dy, t, offset):
+    """Rows whose mean is 100 and 10 000 times their spread."""
+    from pdum_dsl_b200 import kernels
+
+    x, dy, gam = _offset_inputs(cuda, C, (at_x, at_dy), _types()[t], C, offset, 1.0)
+    _, mean, rstd = kernels.layernorm(x, gam, return_stats=True)
+    _check_backward_given(x, dy, mean, rstd, gam, *kernels.layernorm_backward(dy, x, mean, rstd, gam))
+
+
+@pytest.mark.parametrize("C,at_x,at_dy", OFFSET_ROWS)
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_gradients_of_constant_rows(cuda, C, at_x, at_dy, t):
+    """Rows of one value, which is their mean: z is 0, and so are the scale's gradients, exactly."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    x, dy, gam = _offset_inputs(cuda, C, (at_x, at_dy), _types()[t], C + 1, 1000.7, 0.0)
+    mean, rstd = x[:, 0].float(), torch.full((13,), 1e-5 ** -0.5, device=cuda)
+    dx, dg, db = kernels.layernorm_backward(dy, x, mean, rstd, gam)
+    assert (dg == 0).all()
+    _check_backward_given(x, dy, mean, rstd, gam, dx, dg, db)

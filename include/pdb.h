@@ -328,7 +328,8 @@ int pdb_score_program_f32(const pdb_score_program_desc* d, void* stream);
  * The backward writes dx, and dgamma[c] = sum_r dout * z, dbeta[c] = sum_r dout
  * when both are given (both NULL: dx alone), in a fixed order of summation; its
  * workspace (f32 partial sums) is sized by pdb_layernorm_bwd_workspace_size.
- * dx may be dout or x.  With rows == 0 the weight gradients are zeros. */
+ * y may be x, and dx may be dout or x, at the same row stride; they overlap
+ * nothing else.  With rows == 0 the weight gradients are zeros. */
 typedef struct {
   const void* x;
   const void* gamma; /* nullable */

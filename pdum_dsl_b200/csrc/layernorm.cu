@@ -1039,6 +1039,8 @@ extern "C" int pdb_layernorm_fwd(const pdb_layernorm_fwd_desc* d, void* stream) 
     return set_error(PDB_ERR_SHAPE, "layernorm: rows without columns have no statistics");
   if (d->rows == 0 || d->cols == 0) return PDB_OK;
   if (!d->x || !d->y) return set_error(PDB_ERR_ARG, "null x / y");
+  if (d->rows > 1 && d->y == d->x && d->y_row_stride != d->x_row_stride)
+    return set_error(PDB_ERR_ARG, "layernorm: rows that are normed in place have one row stride");
   if (!typed(d->x, d->dtype) || !typed(d->y, d->dtype) || !typed(d->gamma, d->param_dtype) || !typed(d->beta, d->param_dtype))
     return set_error(PDB_ERR_ALIGN, "layernorm: a tensor is not aligned to its type");
   FwdArgs p{d->x, d->gamma, d->beta, d->y, d->mean, d->rstd, d->rows, d->x_row_stride, d->y_row_stride,
@@ -1063,6 +1065,9 @@ extern "C" int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream) 
     return set_error(PDB_ERR_ARG, "dgamma and dbeta are computed together: give both or neither");
   if (d->rows > 0 && (!d->x || !d->dout || !d->dx || !d->mean || !d->rstd))
     return set_error(PDB_ERR_ARG, "null x / dout / dx / mean / rstd");
+  if (d->rows > 1 && ((d->dx == d->x && d->dx_row_stride != d->x_row_stride) ||
+                      (d->dx == d->dout && d->dx_row_stride != d->dout_row_stride)))
+    return set_error(PDB_ERR_ARG, "layernorm backward: a gradient that is taken in place has its tensor's row stride");
   if (d->dgamma && (!d->workspace || d->workspace_bytes < pdb_layernorm_bwd_workspace_size(d)))
     return set_error(PDB_ERR_ARG, "layernorm backward: workspace too small");
   if (!typed(d->x, d->dtype) || !typed(d->dout, d->dtype) || !typed(d->dx, d->dtype) || !typed(d->gamma, d->param_dtype) ||

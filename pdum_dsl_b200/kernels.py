@@ -67,16 +67,19 @@ def _param_dtype(what: str, x: torch.Tensor, cols: int, gamma, beta) -> torch.dt
     return ptype or torch.float32
 
 
-def _out_rows(what: str, out: torch.Tensor, x: torch.Tensor, R: int, C_: int) -> tuple[torch.Tensor, int]:
-    """out for the row kernels, and its row stride."""
+def _out_rows(what: str, out: torch.Tensor, x: torch.Tensor, R: int, C_: int, xs: int) -> tuple[torch.Tensor, int]:
+    """out for the row kernels, and its row stride; x's rows lie xs apart."""
     if out.dtype != x.dtype or out.device != x.device or out.numel() != x.numel():
         raise ValueError(f"{what}: out must have x's size, dtype and device")
-    if out.is_contiguous():
-        return out, C_
-    y = out.view(R, C_)
-    if C_ > 1 and y.stride(-1) != 1:
-        raise ValueError(f"{what}: out must have unit stride along its last dim")
-    return y, y.stride(0)
+    y, ys = out, C_
+    if not out.is_contiguous():
+        y = out.view(R, C_)
+        if C_ > 1 and y.stride(-1) != 1:
+            raise ValueError(f"{what}: out must have unit stride along its last dim")
+        ys = y.stride(0)
+    if R > 1 and ys != xs and y.data_ptr() == x.data_ptr():
+        raise ValueError(f"{what}: out over x must have x's row stride")
+    return y, ys
 
 
 def _own_rows(x: torch.Tensor) -> torch.Tensor:
@@ -112,7 +115,8 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Te
               eps: float = 1e-5, out: torch.Tensor | None = None, return_stats: bool = False):
     """Two-pass layernorm over the last dim (row-statistics), f32 or bf16 (sums and statistics in f32).
 
-    gamma / beta are f32 vectors, or of x's dtype.  ``return_stats`` returns
+    gamma / beta are f32 vectors, or of x's dtype.  ``out`` may be x, and shares no memory with it otherwise.
+    ``return_stats`` returns
     (y, mean, rstd), the rows' float32 statistics that ``layernorm_backward`` reads."""
     _need_cuda(x)
     if x.dtype not in _DTYPES:
@@ -123,7 +127,7 @@ def layernorm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Te
     g = gamma.contiguous() if gamma is not None else None
     b = beta.contiguous() if beta is not None else None
     at_g, at_b = g.data_ptr() if g is not None else None, b.data_ptr() if b is not None else None
-    y, ys = (torch.empty_like(x2), C_) if out is None else _out_rows("layernorm", out, x, R, C_)
+    y, ys = (torch.empty_like(x2), C_) if out is None else _out_rows("layernorm", out, x2, R, C_, xs)
     if plain:
         d = LayerNormDesc(x2.data_ptr(), at_g, at_b, y.data_ptr(), R, C_, xs if R else C_, ys if R else C_, float(eps))
         with _on_device_of(x):

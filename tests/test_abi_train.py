@@ -267,3 +267,35 @@ def test_row_reduction_runners_are_f32():
                 run.run_t(torch.zeros(2, 8, dtype=t))
         with pytest.raises(ValueError, match="CUDA"):
             run.run_t(torch.zeros(2, 8))
+
+
+def test_layernorm_in_place_needs_one_row_stride():
+    """y over x, dx over x or over dout: a row's result lies where the row does, or the call is refused."""
+    lib = _lib.load()
+    d = _norm()
+    d.y_row_stride = 16
+    assert lib.pdb_layernorm_fwd(C.byref(d), None) == _lib.PDB_ERR_ARG
+    assert b"in place" in lib.pdb_last_error_string()
+    for dx in ("x", "dout"):
+        d = _norm_bwd()
+        d.workspace, d.workspace_bytes = 16, 1 << 20
+        d.x, d.dout, d.dx = 1 << 20, 1 << 21, 1 << (20 if dx == "x" else 21)
+        setattr(d, f"{dx}_row_stride", 16)
+        assert lib.pdb_layernorm_bwd(C.byref(d), None) == _lib.PDB_ERR_ARG
+        assert b"in place" in lib.pdb_last_error_string()
+
+
+def test_layernorm_out_over_x_needs_its_row_stride():
+    """The same in Python, before the kernels of either kind are called."""
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    buf = torch.zeros(4, 16)
+    x, dense = buf[:, :8], buf.view(-1)[:32].view(4, 8)
+    for a, b in ((x, dense), (dense, x)):
+        with pytest.raises(ValueError, match="over x"):
+            kernels._out_rows("layernorm", b, a, 4, 8, a.stride(0))
+    assert kernels._out_rows("layernorm", x, x, 4, 8, 16)[1] == 16
+    assert kernels._out_rows("layernorm", buf[:, 8:], x, 4, 8, 16)[1] == 16
+    assert kernels._out_rows("layernorm", dense[:1], x[:1], 1, 8, 16)[1] == 8

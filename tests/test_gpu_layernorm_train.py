@@ -402,3 +402,19 @@ def test_gradients_of_constant_rows(cuda, C, at_x, at_dy, t):
     dx, dg, db = kernels.layernorm_backward(dy, x, mean, rstd, gam)
     assert (dg == 0).all()
     _check_backward_given(x, dy, mean, rstd, gam, dx, dg, db)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_in_place_over_rows_of_another_stride_is_refused(cuda, t):
+    import torch
+
+    from pdum_dsl_b200 import kernels
+
+    buf = torch.randn(4, 16, device=cuda).to(_types()[t])
+    x, dense = buf[:, :8], buf.view(-1)[:32].view(4, 8)
+    for stats in (False, True):
+        for a, b in ((x, dense), (dense, x)):
+            with pytest.raises(ValueError, match="over x"):
+                kernels.layernorm(a, out=b, return_stats=stats)
+    want = kernels.layernorm(x)
+    assert kernels.layernorm(x, out=x).data_ptr() == buf.data_ptr() and torch.equal(x, want)

@@ -373,8 +373,10 @@ int pdb_layernorm_bwd(const pdb_layernorm_bwd_desc* d, void* stream);
  * head_dim] views (strides per batch, head, row; feature stride 1); heads[1] =
  * 0 for one tensor; y[i] may be x[i] with the same strides, and overlaps nothing
  * else.  positions: int64 on the device, read at strides (batch, row); NULL means
- * start + row.  Any int64 position is exact up to whole turns.  inv_freq (radians
- * per position) is read on the host during the call. */
+ * start + row.  Whole turns are dropped exactly for any int64 position; the angle
+ * is off by |position| * (2^-52 |inv_freq| + 2^-61) radians, what a product in 64
+ * bits loses, and by f32's rounding within a turn.  inv_freq (radians per position)
+ * is read on the host during the call. */
 #define PDB_ROTARY_MAX_PAIRS 128
 typedef struct {
   const void* x[2];

@@ -11,8 +11,11 @@
 // error of 0.06 rad at position 10^6).  Here a frequency is a fraction of a turn
 // per position in 64-bit fixed point: the integer product position * turns mod
 // 2^64 drops whole turns exactly, for any int64 position, and what is left, the
-// fraction of a turn, goes through sincospi.  The error is position * 2^-65 of a
-// turn from the table plus f32's on [-1, 1].
+// fraction of a turn, goes through sincospi.  What remains is the table's own
+// error, times the position: |inv_freq| / 2 pi in f64 (the division and the
+// constant, together 2^-52 of the frequency at most) cut to 2^-64 of a turn, so an
+// angle is off by |position| (2^-52 |inv_freq| + 2^-61) radians, about what the
+// product position * inv_freq would lose in f64, and by f32's on [-1, 1].
 //
 // HBM-bound: every element is read and written once.  A thread holds the cos and
 // sin of one 16-byte group of pairs and turns that group in several heads of its

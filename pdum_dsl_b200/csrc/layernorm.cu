@@ -9,10 +9,11 @@
 //
 // Both directions are HBM-bound: the forward reads x and writes y, the backward
 // reads x and dy and writes dx, each once.  A row belongs to TPR threads, which
-// keep it in registers between its two reductions.  On a B200, against a copy of
-// the same bytes: forward 8192 x 4096 bf16 26.6 us (24.7), gradients with the
+// keep it in registers between its two reductions.  On a B200, calls in a row, against a
+// copy of the same bytes: forward 8192 x 4096 bf16 26.6 us (24.7), gradients with the
 // weights' 8192 x 4096 f32 70 us (67), 262144 x 128 bf16 38 us (37); rows too long for
-// one block lie on a cluster: gradients 2048 x 16384 bf16 48 us, forward 1000 x 32768 39.
+// one block lie on a cluster, from a cold L2: gradients 2048 x 16384 bf16 50 us, forward
+// 1000 x 32768 39.
 #include <algorithm>
 #include <atomic>
 
@@ -913,11 +914,13 @@ int launch_fwd(FwdArgs& p, int blocks, cudaStream_t s) {
   return launch(kernel, p, BT, smem, p.cl, s);
 }
 
-// 32 elements per thread in the forward (16 of f32), 256 threads per block and 4 blocks per SM; measured over 32 MiB
-// elements of bf16: 24.7-25 us at 256 to 8192 columns, a copy's time; 29 us at 128 columns, on four threads each (35 on
-// eight, half of whose vectors are empty).  Rows above 16384 columns (f32: 8192) go to clusters of as many blocks as they
-// need: 1000 x 32768 bf16 39 us, where one block per row that reads it three times took 78.  Element by element (tensors
-// whose rows lie differently against 16 bytes) a thread takes 8, or 16 of long rows.
+// 32 elements per thread in the forward (16 of f32), 256 threads per block and runs for 4 blocks per SM (two are resident
+// at 126 registers, so the grid takes two waves); measured over 32 MiB elements of bf16 from a cold L2: 27 to 29 us at the
+// powers of two from 128 to 8192 columns, a copy 26.6; 33 us at 64 columns, where half of four threads' vectors are empty,
+// as a quarter are at 768 and 1536 (31 us) and three eighths at 5120 (35).  128 columns on eight threads, half of whose
+// vectors would be empty, took 6 us more than on four.  Rows above 16384 columns (f32: 8192) go to clusters of as many
+// blocks as they need: 1000 x 32768 bf16 39 us, where one block per row that reads it three times took 78.  Element by
+// element (tensors whose rows lie differently against 16 bytes) a thread takes 8, or 16 of long rows.
 template <typename T, int VEC, bool RAG>
 int dispatch_fwd(FwdArgs& p, cudaStream_t s) {
   if constexpr (VEC == 1) {
@@ -974,10 +977,12 @@ int launch_bwd(BwdArgs& p, int blocks, cudaStream_t s) {
 }
 
 // 16 elements per thread, whose sums and scale fill its registers: 512 threads per SM, three rows ahead.  32 MiB
-// elements of bf16 with the sums' join: 38-40 us at 128 to 4096 columns, a copy of as many bytes 37; 45 us at 8192,
-// where an SM has one row at a time.  Blocks of 512 threads on f32 keep two rows (three, 196 KB, leave the caches too
-// little: 83 against 74 us at 8192 columns).  Rows above 8192 columns go to clusters of as many blocks of 256 threads as
-// they need (48 us at 16384, 54 at 32768); at 4100 to 8192 columns a cluster of two is no faster than one block of 512.
+// elements of bf16 with the sums' join, from a cold L2: 43 us at the powers of two from 64 to 4096 columns (38 where calls
+// follow one another), a copy of as many bytes 37; 45 us at 8192, where an SM has one row at a time, and at 768 and 1536,
+// where a quarter of the vectors are empty; 55 at 5120 (three eighths).  Blocks of 512 threads on f32 keep two rows
+// (three, 196 KB, leave the caches too little: 83 against 74 us at 8192 columns).  Rows above 8192 columns go to clusters
+// of as many blocks of 256 threads as they need (50 us at 16384, 54 at 32768); at 4100 to 8192 columns a cluster of two
+// is no faster than one block of 512.
 template <typename T, int VEC, bool RAG>
 int dispatch_bwd(BwdArgs& p, cudaStream_t s) {
   constexpr int S = sizeof(T) == 4 ? 2 : 3;

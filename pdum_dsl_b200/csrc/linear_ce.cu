@@ -17,15 +17,18 @@
 //
 // All of it is bound by the tensor cores: 2 (forward) and 6 (backward) x tokens x
 // vocab x width operations.  One persistent kernel serves the four products: tiles of
-// 256 rows on CTA pairs (cta_group::2), or of 128 rows on single CTAs where there are
-// at most that many rows, by up to 256 columns; operands by TMA into a ring, two f32
-// accumulators in TMEM so that a tile's epilogue runs under the next tile's products.
+// 256 rows on CTA pairs (cta_group::2), or of 128 rows on single CTAs where the rows
+// make an odd number of 128-row blocks up to seven, by up to 256 columns; operands by
+// TMA into a ring, two f32 accumulators in TMEM so that a tile's epilogue runs under
+// the next tile's products.
 // An operand is read K-major (its rows are the tile's rows) or MN-major (its rows are
 // the contracted index): G^T, x and w enter dw and dx that way, as they lie in memory.
 // Sixteen warps run the epilogue, 64 columns of 32 rows each, and hand results to TMA
-// stores through shared memory.  On a B200, 4096 tokens x 65536 x 2048: the loss in 676
-// us cool (1.63 PFLOP/s), 810 warm under the power limit; 8192 x 128000 x 4096 gradients
-// with a tenth ignored in 16.4 to 18.4 ms (1.40 to 1.57 of all tokens' operations).
+// stores through shared memory (rows of dx whose tokens were packed go to their places
+// by 16-byte stores).  On a B200, 4096 tokens x 65536 x 2048: the loss in 676 us cool
+// (1.63 PFLOP/s), 820 warm under the power limit (1.34); 8192 x 128000 x 4096 gradients
+// with a tenth ignored in 16.4 ms cool, 18.4 warm (1.41 and 1.26 PFLOP/s of the tokens
+// that count).
 //
 // f32 operands take the same steps on IEEE multiply-adds (the f32 column refuses
 // reduced operand types): linear_ce_f32_kernel, G in f32.
